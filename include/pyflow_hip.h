@@ -33,7 +33,7 @@ const char* pf_last_error(void);
 #define PF_ABI_VERSION 7
 int pf_version(void);
 /* sizeof() of the descriptor structs as this library was compiled: 0 pf_gemm_desc, 1 pf_conv_desc, 2 pf_attn_desc,
- * 3 pf_attn_small_desc (-1 otherwise) -- lets a foreign-language binding (ctypes / cgo / JNI struct mirrors) verify its
+ * 3 pf_attn_small_desc, 4 pf_heads_desc, 5 pf_attn_ranges_desc (-1 otherwise) -- lets a foreign-language binding (ctypes / cgo / JNI struct mirrors) verify its
  * layout at load time instead of corrupting a launch. */
 int pf_struct_size(int which);
 
@@ -347,6 +347,65 @@ typedef struct {
     int causal; float scale;
 } pf_attn_small_desc;
 int pf_attention_small_bf16(const pf_attn_small_desc* d, pf_stream_t stream);
+
+/* ------------------------------------------------------------------ attention over key ranges ----
+ * Operators beside pf_qk_norm_rope / pf_attention_bf16 / pf_attention_small_bf16 for sequences those do not cover (several
+ * position axes without a table, shared key heads, head_dim 128, capped scores, a bias by distance, packed documents, caches)
+ * and for training (the gradients).  All tensors bf16 (positions, gains, bias, log-sum-exp and their gradients fp32), sums
+ * and softmax statistics fp32.  A view names element (batch b, row r, head h, channel c) = p[b batch + r row + h head + c];
+ * strides in elements, >= 0, multiples of 8; p 16-byte aligned. */
+typedef struct { void* p; long long batch, row, head; } pf_rows_view;
+
+/* pf_qk_norm_rope_axes: RMSNorm (gains wq / wk fp32 [D]; NULL = none) of every head of Q [B][L][H][D] and K [B][L][Hkv][D], then the
+ *   rotation of the first 2 n_pairs channels: pair p turns by pos[b][row][axis[p]] * freq[p] radians (pos fp32 with strides
+ *   pos_batch / pos_row, n_axes per row; freq double [n_pairs]; axis int [n_pairs]); pairs are (2p, 2p + 1), or (p, p + n_pairs)
+ *   with `halves` (n_pairs % 8 == 0 then).  Q is multiplied by q_scale before its one rounding.  D = 64 or 128; H or Hkv may be
+ *   0.  Qo / Ko may be Q / K (in place), and must not overlap them otherwise.
+ * pf_qk_norm_rope_axes_bwd: dQ, dK = gradients of the results, Q, K = the inputs of the forward; writes the gradients of the
+ *   inputs to Qo, Ko (may be dQ, dK) and, where not NULL, of the gains to dwq / dwk fp32 [D] (workspace of
+ *   pf_qk_norm_rope_axes_bwd_workspace_bytes, 16-byte aligned; the same bits every time). */
+typedef struct {
+    pf_rows_view Q, K, Qo, Ko, dQ, dK;
+    const float* wq; const float* wk;
+    const float* pos; long long pos_batch, pos_row;
+    const double* freq; const int* axis;
+    int n_axes, n_pairs, halves, B, L, H, Hkv, D;
+    float eps, q_scale;
+} pf_heads_desc;
+int pf_qk_norm_rope_axes(const pf_heads_desc* d, pf_stream_t stream);
+long long pf_qk_norm_rope_axes_bwd_workspace_bytes(const pf_heads_desc* d); /* -1 = invalid descriptor */
+int pf_qk_norm_rope_axes_bwd(const pf_heads_desc* d, float* dwq, float* dwk, void* workspace, long long workspace_bytes,
+                             pf_stream_t stream);
+
+/* pf_attention_ranges_bf16: O = softmax(t) V over the keys row i of batch entry b sees: [a_lo, a_hi) and [b_lo, b_hi) (int
+ *   [Lq], batch stride range_batch, 0 = shared; clipped to [0, Lk); a key in both counts once; b_* NULL = one range; a_*
+ *   NULL = all keys), with  t = cap tanh(scale q.k / cap) + bias[h][clamp(j - pos_i, -R, R) + R]  (cap 0: uncapped;
+ *   bias fp32 [H][2 R + 1] or NULL, R = bias_radius <= 512; pos_i = q_pos[b][i], batch stride q_pos_batch, or i + Lk - Lq).  A bias
+ *   entry <= -1e30 hides its distance.  Head h reads key head h / (H / Hkv).  A row that sees nothing gets zeros and LSE =
+ *   -inf, whatever Q, K and V hold; a hidden key never reaches a row's result, be it infinite or NaN.  LSE fp32 [B][H][Lq]
+ *   (natural logarithm of sum exp t) or NULL.  D = 64 or 128.  O may be Q.
+ *   workspace: pf_attention_ranges_workspace_bytes(d) bytes, 16-byte aligned (0 for most calls: only problems with few rows
+ *   split the keys); not shared by launches that may overlap.
+ * pf_attention_ranges_which: 1 = 128 rows of one head per workgroup, 2 = 32 (row, head) pairs of one key head per workgroup with the
+ *   keys split over waves and workgroups, -1 = invalid descriptor.
+ * pf_attention_ranges_bwd: given dO, O, LSE of the forward, writes dQ, dK, dV and (dbias != NULL) the bias's gradient fp32
+ *   [H][2 R + 1]; the same bits every time.  Gradients of shared key heads are summed over their H / Hkv query heads.  Rows that
+ *   see nothing get zeros, keys nobody sees too.  dQ, dK, dV must not overlap the inputs. */
+typedef struct {
+    pf_rows_view Q, K, V, O, dO, dQ, dK, dV;
+    float* LSE;
+    const int* a_lo; const int* a_hi; const int* b_lo; const int* b_hi; long long range_batch;
+    const int* q_pos; long long q_pos_batch;
+    const float* bias; float* dbias;
+    int bias_radius, B, H, Hkv, Lq, Lk, D;
+    float scale, cap;
+    void* workspace; long long workspace_bytes;
+} pf_attn_ranges_desc;
+long long pf_attention_ranges_workspace_bytes(const pf_attn_ranges_desc* d);     /* -1 = invalid descriptor */
+long long pf_attention_ranges_bwd_workspace_bytes(const pf_attn_ranges_desc* d); /* -1 = invalid descriptor */
+int pf_attention_ranges_which(const pf_attn_ranges_desc* d);
+int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, pf_stream_t stream);
+int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, pf_stream_t stream);
 
 /* ------------------------------------------------------------------ multi-GPU communicator --------
  * RCCL over xGMI, one process per GPU.  Replaces the torch.distributed calls of the reference's multi-GPU paths:

@@ -1,0 +1,1207 @@
+// Attention over key ranges, forward and backward, head_dim 64 / 128, shared key heads.
+//
+// Row i of batch entry b sees the keys of [a_lo, a_hi) and [b_lo, b_hi).  With z = q.k scale, c = cap tanh(z / cap) (or z),
+// t = c + bias[h][clamp(j - pos_i)]:
+//     forward    P = exp(t - lse), lse = log sum over visible keys of exp t, O = P V
+//     backward   dV = P^T dO, dP = dO V^T, dT = P (dP - delta), delta = sum_c dO O, dbias = sum of dT by distance,
+//                dZ = dT (1 - (c / cap)^2), dQ = scale dZ K, dK = scale dZ^T Q
+// Scores live in base 2 (t log2 e), maxima and sums in 32 bits; P and dZ are rounded to bf16 once, as operands of the next
+// matrix product (half a step of 2^-9 per weight, the size of the rounding of the result itself).
+//
+// All products are 32 x 32 x 16 MFMAs in the "swapped" form: the result of the first product has the long axis of the second
+// one's contraction in its registers (rows 4 (l / 32) + 8 (r / 4) + r % 4 of lane l, register r), which is how the second
+// product wants its B operand if its A operand is read with the same permutation -- ds_read_b64_tr_b16 on the row-major LDS
+// tile does that.  So P and dZ never leave the registers.  Tiles arrive by 16-byte LDS-DMA into a layout whose 16-byte chunks
+// are XOR-swizzled by row so that both kinds of reads hit all banks (swz below).
+//
+// A hidden key must not reach a row's result even as 0 x inf: the matrix products cannot tell, so a result row that came out
+// non-finite although some of the row's keys were hidden is recomputed by a plain loop over its visible keys (exact_*).
+#include "common.h"
+#include "pyflow_hip.h"
+
+int pf_set_err(const char* m);
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, HIDDEN = -1.0e30f;
+constexpr float DEFER = 6.0f;          // the running maximum follows when a row outgrows it by 2^6: P stays below 64
+constexpr int MAX_RADIUS = 512;        // the bias table and four accumulators of its gradient share LDS with the tiles
+
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef short s8_t __attribute__((ext_vector_type(8)));
+
+struct View { bf16_t* p; long long bs, ld, hs; };
+
+struct RArgs {
+    View q, k, v, o, dO, dq, dk, dv;
+    float* lse;
+    const int* a_lo; const int* a_hi; const int* b_lo; const int* b_hi; long long range_bs;
+    const int* q_pos; long long pos_bs;
+    const float* bias; int R;
+    float zs, cap2, scale;             // z zs = base-2 score (uncapped) or the tanh's argument; cap log2 e, 0 = uncapped
+    int B, H, Hk, G, Lq, Lk;
+    int nqt, nkt, nrb, nsplit;
+    float* parts;                      // split forward: [unit][split][32][D + 2]
+    float* delta;                      // backward: [B][H][Lq]
+    int* tiles;                        // backward: [B][ceil(Lq / 64)][8] bounds of 64-row tiles
+    float* dbias_parts; float* dbias;  // backward: [B][H][nqt][2 R + 1]
+};
+
+// ---------------------------------------------------------------------------------------------- visibility
+struct Vis { int alo, na, blo, nb; };          // keys [alo, alo + na) and [blo, blo + nb), inside [0, Lk)
+
+PF_DEVICE Vis load_vis(const RArgs& p, int b, int row) {
+    Vis v = {0, 0, 0, 0};
+    if (row >= p.Lq) return v;
+    if (!p.a_lo) {
+        v.na = p.Lk;
+        return v;
+    }
+    const long long at = b * p.range_bs + row;
+    v.alo = max(p.a_lo[at], 0);
+    v.na = max(min(p.a_hi[at], p.Lk) - v.alo, 0);
+    if (v.na == 0) v.alo = 0;
+    if (p.b_lo) {
+        v.blo = max(p.b_lo[at], 0);
+        v.nb = max(min(p.b_hi[at], p.Lk) - v.blo, 0);
+        if (v.nb == 0) v.blo = 0;
+    }
+    return v;
+}
+PF_DEVICE bool sees(const Vis& v, int key) {
+    return (unsigned)(key - v.alo) < (unsigned)v.na || (unsigned)(key - v.blo) < (unsigned)v.nb;
+}
+PF_DEVICE bool sees_any(const Vis& v, int j0, int j1) {
+    return (v.na && v.alo < j1 && v.alo + v.na > j0) || (v.nb && v.blo < j1 && v.blo + v.nb > j0);
+}
+PF_DEVICE bool sees_all(const Vis& v, int j0, int j1) {
+    return (v.alo <= j0 && v.alo + v.na >= j1) || (v.blo <= j0 && v.blo + v.nb >= j1);
+}
+
+PF_DEVICE int wave_min(int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = min(x, __shfl_xor(x, o));
+    return x;
+}
+PF_DEVICE int wave_max(int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = max(x, __shfl_xor(x, o));
+    return x;
+}
+PF_DEVICE float wave_add(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+// the key tiles (of KB keys) that a set of rows needs: the union of its two key ranges' tiles, each tile once
+struct TileList {
+    int s0, n0, s1, n;                         // tiles s0 .. s0 + n0 - 1, then s1 .. ; n in all
+    PF_DEVICE int at(int i) const { return i < n0 ? s0 + i : s1 + (i - n0); }
+};
+template <int KB>
+PF_DEVICE TileList tile_list(int amin, int amax, int bmin, int bmax) {
+    int as = 0, ae = 0, bs = 0, be = 0;
+    if (amax > amin) { as = amin / KB; ae = (amax + KB - 1) / KB; }
+    if (bmax > bmin) { bs = bmin / KB; be = (bmax + KB - 1) / KB; }
+    if (ae == as) { as = bs; ae = be; bs = be = 0; }
+    if (be > bs) {
+        if (bs < as) { int t = as; as = bs; bs = t; t = ae; ae = be; be = t; }
+        bs = max(bs, ae);
+        be = max(be, bs);
+    }
+    return {as, ae - as, bs, (ae - as) + (be - bs)};
+}
+
+// ---------------------------------------------------------------------------------------------- LDS tiles
+// Row-major bf16 rows of D channels, 16-byte chunk c of row r at c ^ swz(r).  A row read (ds_read_b128, one chunk of 16
+// consecutive rows per 256 bytes) needs swz to differ over 16 rows modulo the row pitch; a transposed read
+// (ds_read_b64_tr_b16: four chunks of four consecutive rows) needs swz to move those four rows to different quarters.
+template <int D>
+PF_DEVICE int swz(int r) {
+    if constexpr (D == 64) return ((r & 2) << 1) | ((r & 4) >> 1) | ((r & 8) >> 3);
+    else return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+// rows [row0, row0 + ROWS) of a head -> LDS, by the NW waves that share the tile.  Rows behind `last` repeat it (hidden later).
+template <int D, int ROWS, int NW>
+PF_DEVICE void stage(const bf16_t* base, long long ld, int row0, int last, char* lds, int wid, int lane) {
+    constexpr int LPR = D / 8, RPP = 64 / LPR, N = ROWS / RPP / NW;            // lanes per row, rows per 1-KiB piece
+    static_assert(N >= 1 && N * RPP * NW == ROWS, "the tile is a whole number of pieces per wave");
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int i = wid * N + j, r = i * RPP + lane / LPR, c = (lane % LPR) ^ swz<D>(r);
+        glds16(base + (long long)min(row0 + r, last) * ld + c * 8, lds + i * 1024);
+    }
+}
+
+// A operand of a product over channels: row lane % 32 (+ 32 i), channels 16 ks + 8 (lane / 32) ..
+template <int D>
+PF_DEVICE unsigned row_offset(int lane) {
+    const int r = lane & 31, hi = lane >> 5;
+    return (unsigned)(r * (2 * D) + ((hi ^ swz<D>(r)) << 4));
+}
+template <int D>
+PF_DEVICE bf16x8_t row_frag(const char* tile, unsigned off, int i, int ks) {
+    return *(const bf16x8_t*)(tile + i * (64 * D) + (off ^ (unsigned)(ks << 5)));
+}
+// A operand of a product over rows: channel lane % 32 (+ 32 c), rows 16 g + 4 (lane / 32) + {0..3} and + 8
+template <int D>
+PF_DEVICE unsigned tr_offset(int lane, int plus) {
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2) + plus;
+    const int c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    return (unsigned)(r * (2 * D) + ((c ^ swz<D>(r)) << 4) + 8 * (lane & 1));
+}
+template <int D>
+PF_DEVICE bf16x8_t tr_frag(const char* tile, unsigned off0, unsigned off8, int c, int g) {
+    const char* t = tile + g * (32 * D);
+    const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(t + (off0 ^ (unsigned)(c << 6))));
+    const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(t + (off8 ^ (unsigned)(c << 6))));
+    return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// LDS-DMA is not ordered by the compiler's own counts: everything issued so far has landed, every LDS read has returned
+PF_DEVICE void drain() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+PF_DEVICE void drain_barrier() {
+    drain();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+PF_DEVICE f32x16_t mfma(bf16x8_t a, bf16x8_t b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+PF_DEVICE f32x16_t zero16() {
+    f32x16_t z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+PF_DEVICE bf16x8_t half_of(const f32x16_t& s, int g) {
+    bf16x8_t v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (bf16_t)s[8 * g + e];
+    return v;
+}
+PF_DEVICE constexpr int reg_row(int r) { return (r & 3) + 8 * (r >> 2); }      // + 4 (lane / 32)
+
+PF_DEVICE float other_half(float x) {
+    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return (threadIdx.x & 32) ? __uint_as_float(w[0]) : __uint_as_float(w[1]);
+}
+
+// ---------------------------------------------------------------------------------------------- scores
+// odd series below 0.3 (next term 0.0089 x^10: 5e-8), else 1 - 2 / (1 + e^2x): no cancellation of the 1 where x is small
+PF_DEVICE float tanh_f(float x) {
+    const float y = x * x;
+    const float near = x * __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x));
+    return fabsf(x) < 0.3f ? near : far;
+}
+PF_DEVICE float bias2(float b) { return b <= HIDDEN ? -__builtin_inff() : b * LOG2E; }
+
+// base-2 score of one pair from global memory (exact_* and nothing else); th = the capped score's tanh
+PF_DEVICE float score2(const RArgs& p, float z, int h, int dist, float& th) {
+    float t = z * p.zs;
+    th = 0.f;
+    if (p.cap2 != 0.f) {
+        th = tanh_f(t);
+        t = p.cap2 * th;
+    }
+    if (p.bias) t += bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(dist, -p.R), p.R) + p.R]);
+    return t;
+}
+PF_DEVICE int row_pos(const RArgs& p, int b, int row) { return p.q_pos ? p.q_pos[b * p.pos_bs + row] : row + p.Lk - p.Lq; }
+
+template <int D>
+PF_DEVICE float dot_row(const bf16_t* a, const bf16_t* b) {
+    float s = 0.f;
+#pragma unroll 2
+    for (int c = 0; c < D; c += 8) {
+        float x[8], y[8];
+        unpack8(*(const u32x4_t*)(a + c), x);
+        unpack8(*(const u32x4_t*)(b + c), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = __builtin_fmaf(x[e], y[e], s);
+    }
+    return s;
+}
+
+// acc (channels lane D / 64 ..) += w(lane t) row(j0 + t) over the lanes with `use`
+template <int D>
+PF_DEVICE void add_rows(const bf16_t* base, long long ld, int j0, unsigned long long use, float w, float* acc) {
+    const int lane = threadIdx.x & 63;
+    while (use) {
+        const int t = __builtin_ctzll(use);
+        use &= use - 1;
+        const float wt = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), t));
+        const bf16_t* r = base + (long long)(j0 + t) * ld + lane * (D / 64);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) acc[c] = __builtin_fmaf(wt, (float)r[c], acc[c]);
+    }
+}
+template <int D>
+PF_DEVICE void store_row(bf16_t* row, const float* acc) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) row[lane * (D / 64) + c] = (bf16_t)acc[c];
+}
+
+// one whole wave: O of row i of head h from its visible keys alone (m: base-2 maximum, l: sum of 2^(t - m))
+template <int D>
+PF_DEVICE void exact_o(const RArgs& p, int b, int h, int i, float m, float l) {
+    const int lane = threadIdx.x & 63, hk = h / p.G;
+    const Vis v = load_vis(p, b, i);
+    const int pos = row_pos(p, b, i);
+    const bf16_t* q = p.q.p + b * p.q.bs + i * p.q.ld + h * p.q.hs;
+    const bf16_t* K = p.k.p + b * p.k.bs + hk * p.k.hs;
+    const bf16_t* V = p.v.p + b * p.v.bs + hk * p.v.hs;
+    float acc[2] = {0.f, 0.f};
+    for (int j0 = 0; j0 < p.Lk; j0 += 64) {
+        const int j = j0 + lane;
+        bool use = j < p.Lk && sees(v, j);
+        if (__builtin_amdgcn_ballot_w64(use) == 0) continue;
+        float w = 0.f, th;
+        if (use) {
+            const float t = score2(p, dot_row<D>(q, K + j * p.k.ld), h, j - pos, th);
+            use = t != -__builtin_inff();
+            w = __builtin_amdgcn_exp2f(t - m) / l;
+        }
+        add_rows<D>(V, p.v.ld, j0, __builtin_amdgcn_ballot_w64(use), w, acc);
+    }
+    store_row<D>(p.o.p + b * p.o.bs + i * p.o.ld + h * p.o.hs, acc);
+}
+
+// P and dZ of one visible pair, from global memory
+template <int D>
+PF_DEVICE bool exact_pair(const RArgs& p, int b, int h, int hk, int i, int j, float& P, float& dz) {
+    float th;
+    const float z = dot_row<D>(p.q.p + b * p.q.bs + i * p.q.ld + h * p.q.hs, p.k.p + b * p.k.bs + j * p.k.ld + hk * p.k.hs);
+    const float t = score2(p, z, h, j - row_pos(p, b, i), th);
+    if (t == -__builtin_inff()) return false;
+    const long long at = ((long long)b * p.H + h) * p.Lq + i;
+    P = __builtin_amdgcn_exp2f(t - p.lse[at] * LOG2E);
+    const float dp = dot_row<D>(p.dO.p + b * p.dO.bs + i * p.dO.ld + h * p.dO.hs, p.v.p + b * p.v.bs + j * p.v.ld + hk * p.v.hs);
+    dz = P * (dp - p.delta[at]) * (1.f - th * th);
+    return true;
+}
+template <int D>
+PF_DEVICE void exact_dq(const RArgs& p, int b, int h, int i) {
+    const int lane = threadIdx.x & 63, hk = h / p.G;
+    const Vis v = load_vis(p, b, i);
+    float acc[2] = {0.f, 0.f};
+    for (int j0 = 0; j0 < p.Lk; j0 += 64) {
+        const int j = j0 + lane;
+        bool use = j < p.Lk && sees(v, j);
+        if (__builtin_amdgcn_ballot_w64(use) == 0) continue;
+        float P = 0.f, dz = 0.f;
+        if (use) use = exact_pair<D>(p, b, h, hk, i, j, P, dz);
+        add_rows<D>(p.k.p + b * p.k.bs + hk * p.k.hs, p.k.ld, j0, __builtin_amdgcn_ballot_w64(use), dz * p.scale, acc);
+    }
+    store_row<D>(p.dq.p + b * p.dq.bs + i * p.dq.ld + h * p.dq.hs, acc);
+}
+template <int D>
+PF_DEVICE void exact_dkv(const RArgs& p, int b, int hk, int j) {
+    const int lane = threadIdx.x & 63;
+    float ak[2] = {0.f, 0.f}, av[2] = {0.f, 0.f};
+    for (int h = hk * p.G; h < (hk + 1) * p.G; ++h)
+        for (int i0 = 0; i0 < p.Lq; i0 += 64) {
+            const int i = i0 + lane;
+            bool use = i < p.Lq && sees(load_vis(p, b, i), j);
+            if (__builtin_amdgcn_ballot_w64(use) == 0) continue;
+            float P = 0.f, dz = 0.f;
+            if (use) use = exact_pair<D>(p, b, h, hk, i, j, P, dz);
+            const unsigned long long m = __builtin_amdgcn_ballot_w64(use);
+            add_rows<D>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, i0, m, dz * p.scale, ak);
+            add_rows<D>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, i0, m, P, av);
+        }
+    store_row<D>(p.dk.p + b * p.dk.bs + j * p.dk.ld + hk * p.dk.hs, ak);
+    store_row<D>(p.dv.p + b * p.dv.bs + j * p.dv.ld + hk * p.dv.hs, av);
+}
+
+// lane l holds column l % 32 of a [D][32] result, channels reg_row(r) + 4 (l / 32) + 32 c: 8-byte stores into its row
+template <int D>
+PF_DEVICE void store_cols(bf16_t* row, const f32x16_t* o, float f) {
+    const int hi = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            u32x2_t w;
+            w[0] = pack2(o[c][4 * q4] * f, o[c][4 * q4 + 1] * f);
+            w[1] = pack2(o[c][4 * q4 + 2] * f, o[c][4 * q4 + 3] * f);
+            *(u32x2_t*)(row + c * 32 + q4 * 8 + 4 * hi) = w;
+        }
+}
+template <int N>
+PF_DEVICE bool any_nonfinite(const f32x16_t* o) {
+    float t = 0.f;                                     // 0 x finite = 0; 0 x (inf | NaN) = NaN
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t = __builtin_fmaf(o[c][r], 0.f, t);
+    return t != t;
+}
+
+// the bias table of head h in LDS, base 2
+PF_DEVICE void load_table(const RArgs& p, int h, float* tab) {
+    for (int i = threadIdx.x; i < 2 * p.R + 1; i += 256) tab[i] = bias2(p.bias[(long long)h * (2 * p.R + 1) + i]);
+}
+
+// raw products -> base-2 scores with cap and bias; rel0 = key of register 0 minus the row's position (keys in registers)
+PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0, f32x16_t* th) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        float t = s[r] * p.zs;
+        if (p.cap2 != 0.f) {
+            const float x = tanh_f(t);
+            if (th) (*th)[r] = x;
+            t = p.cap2 * x;
+        }
+        if (p.bias) t += tab[min(max(rel0 + reg_row(r), -p.R), p.R) + p.R];
+        s[r] = t;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- forward, many rows
+// One workgroup = 128 rows of one head, 4 waves x 32; key tiles of 64, two in flight.  EX: cap and / or bias (scores are formed
+// in base 2 before the maximum), else scores stay raw and the exponent's multiply-add scales them.
+template <int D, bool EX>
+__global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
+    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    float* const tab = (float*)(smem + 2 * BUF);
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = xcd_remap(blockIdx.x, p.nqt * p.H * p.B);
+    const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
+    const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+    const int hi = lane >> 5, row = qt * 128 + wid * 32 + (lane & 31);
+    const Vis vis = load_vis(p, b, row);
+    const int pos = EX && p.bias ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
+
+    // ---- the workgroup's key tiles
+    int* const red = (int*)smem;
+    {
+        const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
+        const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
+        if (lane == 0) { red[4 * wid] = amin; red[4 * wid + 1] = amax; red[4 * wid + 2] = bmin; red[4 * wid + 3] = bmax; }
+    }
+    if (EX && p.bias) load_table(p, h, tab);
+    __syncthreads();
+    TileList tl;
+    {
+        int x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = red[i];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) x[i] = (i & 1) ? max(x[i], red[4 * w + i]) : min(x[i], red[4 * w + i]);
+            x[i] = __builtin_amdgcn_readfirstlane(x[i]);
+        }
+        tl = tile_list<64>(x[0], x[1], x[2], x[3]);
+    }
+    const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
+    const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
+    bf16x8_t qf[D / 16];
+    {
+        const bf16_t* q = p.q.p + b * p.q.bs + (long long)min(row, p.Lq - 1) * p.q.ld + h * p.q.hs + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8_t*)(q + ks * 16);
+    }
+    const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
+    f32x16_t o[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] = zero16();
+    float m = -__builtin_inff(), l = 0.f;
+    bool whole = true;                             // wave-uniform: no row of the wave had a hidden key in any tile
+    drain_barrier();                               // `red` is read: its memory becomes tile memory
+    auto issue = [&](int n) {
+        const int j0 = tl.at(n) * 64;
+        char* buf = smem + (n & 1) * BUF;
+        stage<D, 64, 4>(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
+        stage<D, 64, 4>(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
+    };
+    if (tl.n > 0) issue(0);
+    for (int n = 0; n < tl.n; ++n) {
+        drain_barrier();
+        if (n + 1 < tl.n) issue(n + 1);
+        const int j0 = tl.at(n) * 64;
+        const char* sk = smem + (n & 1) * BUF;
+        const char* sv = sk + TILE;
+        const bool full = __builtin_amdgcn_ballot_w64(!sees_all(vis, j0, j0 + 64)) == 0;
+        if (!full) {
+            whole = false;
+            if (__builtin_amdgcn_ballot_w64(sees_any(vis, j0, j0 + 64)) == 0) continue;
+        }
+        f32x16_t s[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s[i] = zero16();
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) s[i] = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s[i]);
+        }
+        if (EX) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) cap_bias(p, s[i], tab, j0 + 32 * i + 4 * hi - pos, nullptr);
+        }
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] = sees(vis, j0 + 32 * i + 4 * hi + reg_row(r)) ? s[i][r] : -__builtin_inff();
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[i][r]);
+        mt = fmaxf(mt, other_half(mt));
+        const float zs = EX ? 1.f : p.zs;
+        mt *= zs;
+        if (__builtin_amdgcn_ballot_w64(mt > m + DEFER) != 0) {
+            const float mn = fmaxf(m, mt);
+            const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[c][r] *= alpha;
+        }
+        const float ms = m == -__builtin_inff() ? 0.f : m;
+        float ps = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], zs, -ms));
+                s[i][r] = e;
+                ps += e;
+            }
+        l += ps;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const bf16x8_t pf = half_of(s[g >> 1], g & 1);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) o[c] = mfma(tr_frag<D>(sv, t0, t8, c, g), pf, o[c]);
+        }
+    }
+    l += other_half(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const bool bad = any_nonfinite<D / 32>(o) && !whole && l == l && row < p.Lq;
+    unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
+    redo = (redo | (redo >> 32)) & 0xffffffffull;
+    const bool mine = (redo >> (lane & 31)) & 1;
+    if (row < p.Lq) {
+        if (!mine) store_cols<D>(p.o.p + b * p.o.bs + row * p.o.ld + h * p.o.hs, o, inv);
+        if (p.lse && hi == 0) p.lse[((long long)b * p.H + h) * p.Lq + row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+    }
+    while (redo) {
+        const int i = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        exact_o<D>(p, b, h, qt * 128 + wid * 32 + i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), i)),
+                   __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), i)));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- forward, few rows
+// One workgroup = 32 (row, head) pairs that share a key head, one part of the keys; its 4 waves take every fourth 32-key tile of
+// the part and meet in LDS at the end.  Tiles are private to a wave: no barrier in the loop, the next tile is in flight while the
+// current one is used.  nsplit > 1: parts go to the workspace, range_join_kernel adds them.
+template <int D, bool EX>
+__global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
+    constexpr int TILE = 32 * 2 * D, BUF = 2 * TILE, WAVE = 2 * BUF, NP = 2 * 32 / (512 / D);
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int unit = blockIdx.x / p.nsplit, part = blockIdx.x - unit * p.nsplit;
+    const int bk = unit / p.nrb, rb = unit - bk * p.nrb;
+    const int b = bk / p.Hk, hk = bk - b * p.Hk;
+    const int hi = lane >> 5;
+    const int rho = rb * 32 + (lane & 31);                          // row rho / G of head hk G + rho % G
+    const bool valid = rho < p.Lq * p.G;
+    const int row = valid ? rho / p.G : p.Lq - 1, h = hk * p.G + (valid ? rho % p.G : 0);
+    Vis vis = load_vis(p, b, row);
+    if (!valid) vis.na = vis.nb = 0;
+    const int pos = EX && p.bias ? row_pos(p, b, row) : 0;
+    const float* const bias = EX && p.bias ? p.bias + (long long)h * (2 * p.R + 1) + p.R : nullptr;
+    const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
+    const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
+    const TileList tl = tile_list<32>(__builtin_amdgcn_readfirstlane(amin), __builtin_amdgcn_readfirstlane(amax),
+                                      __builtin_amdgcn_readfirstlane(bmin), __builtin_amdgcn_readfirstlane(bmax));
+    const int n0 = (int)((long long)tl.n * part / p.nsplit), n1 = (int)((long long)tl.n * (part + 1) / p.nsplit);
+    const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
+    const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
+    bf16x8_t qf[D / 16];
+    {
+        const bf16_t* q = p.q.p + b * p.q.bs + row * p.q.ld + h * p.q.hs + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8_t*)(q + ks * 16);
+    }
+    const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
+    f32x16_t o[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] = zero16();
+    float m = -__builtin_inff(), l = 0.f;
+    char* const mem = smem + wid * WAVE;
+    drain();                                                        // the counted waits below see tile pieces only
+    auto issue = [&](int n, int buf) {
+        const int j0 = tl.at(n) * 32;
+        stage<D, 32, 1>(K, p.k.ld, j0, p.Lk - 1, mem + buf * BUF, 0, lane);
+        stage<D, 32, 1>(V, p.v.ld, j0, p.Lk - 1, mem + buf * BUF + TILE, 0, lane);
+    };
+    if (n0 + wid < n1) issue(n0 + wid, 0);
+    int buf = 0;
+    for (int n = n0 + wid; n < n1; n += 4, buf ^= 1) {
+        if (n + 4 < n1) {
+            issue(n + 4, buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NP) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const int j0 = tl.at(n) * 32;
+        const char* sk = mem + buf * BUF;
+        const char* sv = sk + TILE;
+        f32x16_t s = zero16();
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) s = mfma(row_frag<D>(sk, roff, 0, ks), qf[ks], s);
+        const int k0 = j0 + 4 * hi;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float t = s[r] * p.zs;
+            if (EX && p.cap2 != 0.f) t = p.cap2 * tanh_f(t);
+            if (EX && bias) t += bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]);
+            s[r] = sees(vis, k0 + reg_row(r)) ? t : -__builtin_inff();
+        }
+        float mt = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
+        mt = fmaxf(mt, other_half(mt));
+        const float mn = fmaxf(m, mt);
+        const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        const float ms = m == -__builtin_inff() ? 0.f : m;
+        float ps = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(s[r] - ms);
+            ps += s[r];
+        }
+        l = l * alpha + ps;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[c][r] *= alpha;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const bf16x8_t pf = half_of(s, g);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) o[c] = mfma(tr_frag<D>(sv, t0, t8, c, g), pf, o[c]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the tile is read: its buffer may be refilled
+    }
+    l += other_half(l);
+    // ---- the four waves meet: [wave][32][D + 4] fp32 (O, m, l), a row per lane pair
+    constexpr int PITCH = D + 4;
+    __syncthreads();
+    float* const acc = (float*)smem;
+    {
+        float* r = acc + (wid * 32 + (lane & 31)) * PITCH;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                f32x4_t w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = o[c][4 * q4 + e];
+                *(f32x4_t*)(r + 32 * c + 8 * q4 + 4 * hi) = w;
+            }
+        if (hi == 0) { r[D] = m; r[D + 1] = l; }
+    }
+    __syncthreads();
+    const int rows = min(32, p.Lq * p.G - rb * 32);
+    for (int r = wid; r < rows; r += 4) {                           // one row per wave: lanes over channels
+        float mm = -__builtin_inff(), f[4], ll = 0.f, v[2] = {0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, acc[(w * 32 + r) * PITCH + D]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float* a = acc + (w * 32 + r) * PITCH;
+            f[w] = a[D] == mm ? (mm == -__builtin_inff() ? 0.f : 1.f) : __builtin_amdgcn_exp2f(a[D] - mm);
+            ll += f[w] == 0.f && a[D + 1] == 0.f ? 0.f : f[w] * a[D + 1];
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) v[c] += f[w] == 0.f && a[D + 1] == 0.f ? 0.f : f[w] * a[lane * (D / 64) + c];
+        }
+        const int pr = rb * 32 + r, i = pr / p.G, hh = hk * p.G + pr % p.G;
+        if (p.nsplit > 1) {
+            float* out = p.parts + (((long long)unit * p.nsplit + part) * 32 + r) * (D + 2);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) out[lane * (D / 64) + c] = v[c];
+            if (lane == 0) { out[D] = mm; out[D + 1] = ll; }
+            continue;
+        }
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) bad = bad || !(fabsf(v[c]) < __builtin_inff());
+        if (__builtin_amdgcn_ballot_w64(bad) != 0 && ll == ll) {
+            exact_o<D>(p, b, hh, i, mm, ll);
+        } else {
+            const float inv = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) v[c] *= inv;
+            store_row<D>(p.o.p + b * p.o.bs + i * p.o.ld + hh * p.o.hs, v);
+        }
+        if (p.lse && lane == 0) p.lse[((long long)b * p.H + hh) * p.Lq + i] = ll == 0.f ? -__builtin_inff() : (mm + __builtin_amdgcn_logf(ll)) * LN2;
+    }
+}
+
+// one wave per (row, head): the parts' maxima, then the weighted sums, in part order
+template <int D>
+__global__ __launch_bounds__(256) void range_join_kernel(const RArgs p) {
+    const int lane = threadIdx.x & 63;
+    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int per = p.Lq * p.G;
+    if (w >= (long long)p.B * p.Hk * per) return;
+    const int bk = (int)(w / per), pr = (int)(w - (long long)bk * per);
+    const int b = bk / p.Hk, hk = bk - b * p.Hk, i = pr / p.G, h = hk * p.G + pr % p.G;
+    const float* base = p.parts + (((long long)bk * p.nrb + pr / 32) * p.nsplit * 32 + pr % 32) * (D + 2);
+    const long long step = 32 * (D + 2);
+    float m = -__builtin_inff();
+    for (int s = lane; s < p.nsplit; s += 64) m = fmaxf(m, base[s * step + D]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    float l = 0.f, v[2] = {0.f, 0.f};
+    for (int s = 0; s < p.nsplit; ++s) {
+        const float* a = base + s * step;
+        const float ls = a[D + 1];
+        if (ls == 0.f) continue;                                     // the part saw no key
+        const float f = a[D] == m ? 1.f : __builtin_amdgcn_exp2f(a[D] - m);
+        l += f * ls;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) v[c] += f * a[lane * (D / 64) + c];
+    }
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) bad = bad || !(fabsf(v[c]) < __builtin_inff());
+    if (__builtin_amdgcn_ballot_w64(bad) != 0 && l == l) {
+        exact_o<D>(p, b, h, i, m, l);
+    } else {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) v[c] *= inv;
+        store_row<D>(p.o.p + b * p.o.bs + i * p.o.ld + h * p.o.hs, v);
+    }
+    if (p.lse && lane == 0) p.lse[((long long)b * p.H + h) * p.Lq + i] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// ---------------------------------------------------------------------------------------------- backward
+// delta[b][h][i] = sum_c dO O (four lanes per row), and for each 64-row tile the bounds of its key ranges: 0..3 the smallest start
+// and largest end of the a and b ranges that are not empty; 4..7 the largest start and smallest end over ALL its rows.
+template <int D>
+__global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
+    const int qt = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const int row = qt * 64 + (threadIdx.x >> 2), sub = threadIdx.x & 3;
+    float s = 0.f;
+    if (row < p.Lq) {
+        const bf16_t* x = p.dO.p + b * p.dO.bs + row * p.dO.ld + h * p.dO.hs + sub * (D / 4);
+        const bf16_t* y = p.o.p + b * p.o.bs + row * p.o.ld + h * p.o.hs + sub * (D / 4);
+        s = dot_row<D / 4>(x, y);
+    }
+    s += __shfl_xor(s, 1);
+    s += __shfl_xor(s, 2);
+    if (row < p.Lq && sub == 0) p.delta[((long long)b * p.H + h) * p.Lq + row] = s;
+    if (h == 0 && threadIdx.x < 64) {
+        const int r = qt * 64 + threadIdx.x;
+        const Vis v = load_vis(p, b, r);
+        int x[8] = {v.na ? v.alo : 0x7fffffff, v.na ? v.alo + v.na : 0, v.nb ? v.blo : 0x7fffffff, v.nb ? v.blo + v.nb : 0,
+                    v.na ? v.alo : 0x7fffffff, v.na ? v.alo + v.na : 0, v.nb ? v.blo : 0x7fffffff, v.nb ? v.blo + v.nb : 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (i == 0 || i == 2 || i == 5 || i == 7) ? wave_min(x[i]) : wave_max(x[i]);
+        if (threadIdx.x == 0) {
+            int* t = p.tiles + ((long long)b * ((p.Lq + 63) / 64) + qt) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = x[i];
+        }
+    }
+}
+
+// dK, dV of 128 keys of one key head: 4 waves x 32 keys held in registers, looping over the 64-row tiles (of every query head that
+// shares the key head) that see any of them.
+template <int D, bool EX>
+__global__ __launch_bounds__(256, 1) void range_dkv_kernel(const RArgs p) {
+    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    float* const rowf = (float*)(smem + 2 * BUF);                   // [2][2][64]: lse (base 2), delta
+    int* const rowi = (int*)(rowf + 256);                           // [2][5][64]: ranges, position
+    float* const tab = (float*)(rowi + 640);
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = xcd_remap(blockIdx.x, p.nkt * p.Hk * p.B);
+    const int bk = t / p.nkt, kt = t - bk * p.nkt;
+    const int b = bk / p.Hk, hk = bk - b * p.Hk;
+    const int hi = lane >> 5;
+    const int w0 = kt * 128 + wid * 32, key = w0 + (lane & 31);
+    const int nq = (p.Lq + 63) / 64;
+    const int* const tiles = p.tiles + (long long)b * nq * 8;
+    bf16x8_t kf[D / 16], vf[D / 16];
+    {
+        const long long kr = min(key, p.Lk - 1);
+        const bf16_t* k = p.k.p + b * p.k.bs + kr * p.k.ld + hk * p.k.hs + hi * 8;
+        const bf16_t* v = p.v.p + b * p.v.bs + kr * p.v.ld + hk * p.v.hs + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            kf[ks] = *(const bf16x8_t*)(k + ks * 16);
+            vf[ks] = *(const bf16x8_t*)(v + ks * 16);
+        }
+    }
+    const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
+    f32x16_t dk[D / 32], dv[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = zero16();
+    const int wg0 = kt * 128, wg1 = min(wg0 + 128, p.Lk);
+    // tiles are numbered g nq + qt; the next one at or behind n that sees a key of this workgroup
+    auto next = [&](int n) {
+        for (; n < p.G * nq; ++n) {
+            const int* x = tiles + (n % nq) * 8;
+            if ((x[0] < wg1 && x[1] > wg0) || (x[2] < wg1 && x[3] > wg0)) break;
+        }
+        return n;
+    };
+    auto issue = [&](int n, int buf) {
+        const int h = hk * p.G + n / nq, i0 = (n % nq) * 64;
+        char* base = smem + buf * BUF;
+        stage<D, 64, 4>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, i0, p.Lq - 1, base, wid, lane);
+        stage<D, 64, 4>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, i0, p.Lq - 1, base + TILE, wid, lane);
+        const int r = i0 + lane, rc = min(r, p.Lq - 1);
+        const long long at = ((long long)b * p.H + h) * p.Lq + rc;
+        if (wid == 0) rowf[buf * 128 + lane] = p.lse[at] * LOG2E;
+        if (wid == 1) rowf[buf * 128 + 64 + lane] = p.delta[at];
+        if (wid == 2) {
+            const Vis v = load_vis(p, b, r);
+            int* x = rowi + buf * 320;
+            x[lane] = v.alo; x[64 + lane] = v.na; x[128 + lane] = v.blo; x[192 + lane] = v.nb;
+        }
+        if (wid == 3 && EX && p.bias) rowi[buf * 320 + 256 + lane] = row_pos(p, b, rc);
+    };
+    int n = next(0), buf = 0, table_of = -1;
+    if (n < p.G * nq) issue(n, 0);
+    while (n < p.G * nq) {
+        drain_barrier();
+        if (EX && p.bias && n / nq != table_of) {                   // uniform: another head, another bias table
+            table_of = n / nq;
+            load_table(p, hk * p.G + table_of, tab);
+            drain_barrier();
+        }
+        const int n2 = next(n + 1);
+        if (n2 < p.G * nq) issue(n2, buf ^ 1);
+        const int* x = tiles + (n % nq) * 8;
+        const bool any = (x[0] < w0 + 32 && x[1] > w0) || (x[2] < w0 + 32 && x[3] > w0);
+        const bool full = (x[4] <= w0 && x[5] >= w0 + 32) || (x[6] <= w0 && x[7] >= w0 + 32);
+        if (any) {
+            const char* sq = smem + buf * BUF;
+            const char* so = sq + TILE;
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+                f32x16_t s = zero16(), dp = zero16(), th;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    s = mfma(row_frag<D>(sq, roff, qb, ks), kf[ks], s);
+                    dp = mfma(row_frag<D>(so, roff, qb, ks), vf[ks], dp);
+                }
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const int r0 = qb * 32 + 8 * q4 + 4 * hi;
+                    const f32x4_t ls = *(const f32x4_t*)(rowf + buf * 128 + r0), de = *(const f32x4_t*)(rowf + buf * 128 + 64 + r0);
+                    const int* ri = rowi + buf * 320 + r0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * q4 + e;
+                        float z = s[r] * p.zs, fac = 1.f;
+                        bool ok = full;
+                        if (!full) ok = sees(Vis{ri[e], ri[64 + e], ri[128 + e], ri[192 + e]}, key);
+                        if (EX && p.cap2 != 0.f) {
+                            const float y = tanh_f(z);
+                            z = p.cap2 * y;
+                            fac = __builtin_fmaf(-y, y, 1.f);
+                        }
+                        if (EX && p.bias) {
+                            z += tab[min(max(key - ri[256 + e], -p.R), p.R) + p.R];
+                            ok = ok && z != -__builtin_inff();
+                        }
+                        const float P = __builtin_amdgcn_exp2f(z - ls[e]);
+                        const float dz = P * (dp[r] - de[e]) * fac;
+                        s[r] = ok ? P : 0.f;
+                        dp[r] = ok ? dz : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const bf16x8_t pf = half_of(s, g), zf = half_of(dp, g);
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        dv[c] = mfma(tr_frag<D>(so, t0, t8, c, 2 * qb + g), pf, dv[c]);
+                        dk[c] = mfma(tr_frag<D>(sq, t0, t8, c, 2 * qb + g), zf, dk[c]);
+                    }
+                }
+            }
+        }
+        n = n2;
+        buf ^= 1;
+    }
+    const bool bad = key < p.Lk && (any_nonfinite<D / 32>(dk) || any_nonfinite<D / 32>(dv));
+    unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
+    redo = (redo | (redo >> 32)) & 0xffffffffull;
+    if (key < p.Lk && !((redo >> (lane & 31)) & 1)) {
+        store_cols<D>(p.dk.p + b * p.dk.bs + key * p.dk.ld + hk * p.dk.hs, dk, p.scale);
+        store_cols<D>(p.dv.p + b * p.dv.bs + key * p.dv.ld + hk * p.dv.hs, dv, 1.f);
+    }
+    while (redo) {
+        const int j = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        exact_dkv<D>(p, b, hk, w0 + j);
+    }
+}
+
+// dQ of 128 rows of one head (4 waves x 32 rows held in registers) over its key tiles, and this workgroup's part of dbias: every
+// wave adds dT of its pairs into a table of its own (LDS float adds of one wave run in program order; pairs behind the table's
+// ends are summed in registers), the four tables are added in wave order.
+template <int D, bool EX>
+__global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
+    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    float* const tab = (float*)(smem + 2 * BUF);
+    const int NB = 2 * p.R + 1;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float* const hist = tab + NB + wid * NB;
+    const int t = xcd_remap(blockIdx.x, p.nqt * p.H * p.B);
+    const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
+    const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+    const int hi = lane >> 5, row = qt * 128 + wid * 32 + (lane & 31), rc = min(row, p.Lq - 1);
+    const Vis vis = load_vis(p, b, row);
+    const int pos = EX && p.bias ? row_pos(p, b, rc) : 0;
+    int* const red = (int*)smem;
+    {
+        const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
+        const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
+        if (lane == 0) { red[4 * wid] = amin; red[4 * wid + 1] = amax; red[4 * wid + 2] = bmin; red[4 * wid + 3] = bmax; }
+    }
+    if (EX && p.bias) {
+        load_table(p, h, tab);
+        if (p.dbias)
+            for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
+    }
+    __syncthreads();
+    TileList tl;
+    {
+        int x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = red[i];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) x[i] = (i & 1) ? max(x[i], red[4 * w + i]) : min(x[i], red[4 * w + i]);
+            x[i] = __builtin_amdgcn_readfirstlane(x[i]);
+        }
+        tl = tile_list<64>(x[0], x[1], x[2], x[3]);
+    }
+    const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
+    const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
+    bf16x8_t qf[D / 16], of[D / 16];
+    {
+        const bf16_t* q = p.q.p + b * p.q.bs + rc * p.q.ld + h * p.q.hs + hi * 8;
+        const bf16_t* g = p.dO.p + b * p.dO.bs + rc * p.dO.ld + h * p.dO.hs + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            qf[ks] = *(const bf16x8_t*)(q + ks * 16);
+            of[ks] = *(const bf16x8_t*)(g + ks * 16);
+        }
+    }
+    const long long at = ((long long)b * p.H + h) * p.Lq + rc;
+    const float ls = p.lse[at] * LOG2E, de = p.delta[at];
+    const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
+    f32x16_t dq[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dq[c] = zero16();
+    float below = 0.f, above = 0.f;                 // dbias of distances <= -R and >= R
+    const int pmin = wave_min(row < p.Lq ? pos : 0x7fffffff), pmax = wave_max(row < p.Lq ? pos : -0x7fffffff);
+    bool whole = true;
+    drain_barrier();
+    auto issue = [&](int n) {
+        const int j0 = tl.at(n) * 64;
+        char* buf = smem + (n & 1) * BUF;
+        stage<D, 64, 4>(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
+        stage<D, 64, 4>(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
+    };
+    if (tl.n > 0) issue(0);
+    for (int n = 0; n < tl.n; ++n) {
+        drain_barrier();
+        if (n + 1 < tl.n) issue(n + 1);
+        const int j0 = tl.at(n) * 64;
+        const char* sk = smem + (n & 1) * BUF;
+        const char* sv = sk + TILE;
+        const bool full = __builtin_amdgcn_ballot_w64(!sees_all(vis, j0, j0 + 64)) == 0;
+        if (!full) {
+            whole = false;
+            if (__builtin_amdgcn_ballot_w64(sees_any(vis, j0, j0 + 64)) == 0) continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f32x16_t s = zero16(), dp = zero16();
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+                s = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s);
+                dp = mfma(row_frag<D>(sv, roff, i, ks), of[ks], dp);
+            }
+            const int k0 = j0 + 32 * i + 4 * hi;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float z = s[r] * p.zs, fac = 1.f;
+                bool ok = full || sees(vis, k0 + reg_row(r));
+                if (EX && p.cap2 != 0.f) {
+                    const float y = tanh_f(z);
+                    z = p.cap2 * y;
+                    fac = __builtin_fmaf(-y, y, 1.f);
+                }
+                if (EX && p.bias) {
+                    z += tab[min(max(k0 + reg_row(r) - pos, -p.R), p.R) + p.R];
+                    ok = ok && z != -__builtin_inff();
+                }
+                const float P = __builtin_amdgcn_exp2f(z - ls);
+                const float dt = P * (dp[r] - de);
+                if (EX) s[r] = ok ? dt : 0.f;
+                dp[r] = ok ? dt * fac : 0.f;
+            }
+            if (EX && p.bias && p.dbias) {
+                const int lo = j0 + 32 * i - pmax, hi_ = j0 + 32 * i + 31 - pmin;     // distances of this block, wave-uniform
+                if (hi_ <= -p.R || lo >= p.R) {
+                    float a = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) a += s[r];
+                    if (lo >= p.R) above += a;
+                    else below += a;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int d = k0 + reg_row(r) - pos;
+                        if (d <= -p.R) below += s[r];
+                        else if (d >= p.R) above += s[r];
+                        else __hip_atomic_fetch_add(hist + d + p.R, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    }
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const bf16x8_t zf = half_of(dp, g);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) dq[c] = mfma(tr_frag<D>(sk, t0, t8, c, 2 * i + g), zf, dq[c]);
+            }
+        }
+    }
+    const bool bad = any_nonfinite<D / 32>(dq) && !whole && row < p.Lq;
+    unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
+    redo = (redo | (redo >> 32)) & 0xffffffffull;
+    if (row < p.Lq && !((redo >> (lane & 31)) & 1)) store_cols<D>(p.dq.p + b * p.dq.bs + row * p.dq.ld + h * p.dq.hs, dq, p.scale);
+    while (redo) {
+        const int i = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        exact_dq<D>(p, b, h, qt * 128 + wid * 32 + i);
+    }
+    if (EX && p.bias && p.dbias) {
+        below = wave_add(below);
+        above = wave_add(above);
+        if (lane == 0) {
+            hist[0] = below;
+            hist[2 * p.R] = p.R == 0 ? below + above : above;
+        }
+        __syncthreads();
+        float* out = p.dbias_parts + ((long long)bh * p.nqt + qt) * NB;
+        for (int i = threadIdx.x; i < NB; i += 256) out[i] = (tab[NB + i] + tab[2 * NB + i]) + (tab[3 * NB + i] + tab[4 * NB + i]);
+    }
+}
+
+// dbias[h][i] = sum over batch entries and row tiles of the parts, in order: 64 entries per workgroup, 4 groups of parts
+__global__ __launch_bounds__(256) void range_dbias_kernel(const RArgs p) {
+    __shared__ float red[4][64];
+    const int NB = 2 * p.R + 1, i = blockIdx.x * 64 + (threadIdx.x & 63), h = blockIdx.y, grp = threadIdx.x >> 6;
+    float a = 0.f;
+    if (i < NB)
+        for (int u = grp; u < p.B * p.nqt; u += 4) a += p.dbias_parts[(((long long)(u / p.nqt) * p.H + h) * p.nqt + u % p.nqt) * NB + i];
+    red[grp][threadIdx.x & 63] = a;
+    __syncthreads();
+    if (grp == 0 && i < NB) p.dbias[(long long)h * NB + i] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+bool bad_view(const pf_rows_view& v) {
+    return !v.p || ((uintptr_t)v.p & 15) || v.batch < 0 || v.row < 0 || v.head < 0 || ((v.batch | v.row | v.head) & 7);
+}
+View view(const pf_rows_view& v) { return {(bf16_t*)v.p, v.batch, v.row, v.head}; }
+
+const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
+    if (!d) return "pf_attention_ranges: null descriptor";
+    if (d->D != 64 && d->D != 128) return "pf_attention_ranges: head_dim must be 64 or 128";
+    if (d->B < 0 || d->H < 0 || d->Hkv < 0 || d->Lq < 0 || d->Lk < 0) return "pf_attention_ranges: negative size";
+    if ((d->H == 0) != (d->Hkv == 0) || (d->H && d->H % d->Hkv)) return "pf_attention_ranges: the number of heads must be a multiple of the key heads";
+    if (d->Lq > (1 << 30) || d->Lk > (1 << 30)) return "pf_attention_ranges: more than 2^30 rows or keys";
+    if (!(d->scale - d->scale == 0.f) || d->scale <= 0.f) return "pf_attention_ranges: scale must be positive and finite";
+    if (!(d->cap >= 0.f) || d->cap > 1e30f) return "pf_attention_ranges: cap must be 0 (none) or positive and finite";
+    if ((d->a_lo == nullptr) != (d->a_hi == nullptr) || (d->b_lo == nullptr) != (d->b_hi == nullptr) || (d->b_lo && !d->a_lo))
+        return "pf_attention_ranges: a range needs its start and its end, the second one the first";
+    if (d->range_batch < 0 || d->q_pos_batch < 0) return "pf_attention_ranges: negative stride";
+    if (d->bias && (d->bias_radius < 0 || d->bias_radius > MAX_RADIUS)) return "pf_attention_ranges: bias_radius must be in 0..512";
+    if (d->dbias && !d->bias) return "pf_attention_ranges: a bias gradient without a bias";
+    const bool rows = d->B && d->H && d->Lq, keys = d->B && d->H && d->Lk;
+    const char* const bad = "pf_attention_ranges: tensors must be 16-byte aligned with strides that are multiples of 8 elements";
+    if ((rows && (bad_view(d->Q) || bad_view(d->O))) || (keys && (bad_view(d->K) || bad_view(d->V)))) return bad;
+    if (grad) {
+        if ((rows && (bad_view(d->dO) || bad_view(d->dQ))) || (keys && (bad_view(d->dK) || bad_view(d->dV)))) return bad;
+        if (rows && !d->LSE) return "pf_attention_ranges_bwd: null LSE";
+    }
+    return nullptr;
+}
+
+// the form with 32 (row, head) pairs per workgroup and the keys split: where 128-row workgroups would leave compute units empty
+bool few_rows(const pf_attn_ranges_desc* d) {
+    return (long long)((d->Lq + 127) / 128) * d->H * d->B < 256;
+}
+int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * (d->H / d->Hkv) + 31) / 32); }
+int splits(const pf_attn_ranges_desc* d) {
+    const long long units = (long long)row_blocks(d) * d->Hkv * d->B, tiles = (d->Lk + 31) / 32;
+    long long n = 512 / units;
+    if (n > tiles / 8) n = tiles / 8;                     // two tiles per wave at least
+    return (int)(n < 1 ? 1 : n);
+}
+long long fwd_bytes(const pf_attn_ranges_desc* d) {
+    if (!d->B || !d->H || !d->Lq || !few_rows(d)) return 0;
+    const int s = splits(d);
+    return s > 1 ? (long long)row_blocks(d) * d->Hkv * d->B * s * 32 * (d->D + 2) * 4 : 0;
+}
+long long up16(long long n) { return (n + 15) / 16 * 16; }
+struct BwdSizes { long long delta, tiles, parts; };
+BwdSizes bwd_sizes(const pf_attn_ranges_desc* d) {
+    BwdSizes s;
+    s.delta = up16((long long)d->B * d->H * d->Lq * 4);
+    s.tiles = up16((long long)d->B * ((d->Lq + 63) / 64) * 32);
+    s.parts = d->dbias ? up16((long long)d->B * d->H * ((d->Lq + 127) / 128) * (2 * d->bias_radius + 1) * 4) : 0;
+    return s;
+}
+
+RArgs range_args(const pf_attn_ranges_desc* d) {
+    RArgs a{};
+    a.q = view(d->Q); a.k = view(d->K); a.v = view(d->V); a.o = view(d->O);
+    a.dO = view(d->dO); a.dq = view(d->dQ); a.dk = view(d->dK); a.dv = view(d->dV);
+    a.lse = d->LSE;
+    a.a_lo = d->a_lo; a.a_hi = d->a_hi; a.b_lo = d->b_lo; a.b_hi = d->b_hi; a.range_bs = d->range_batch;
+    a.q_pos = d->q_pos; a.pos_bs = d->q_pos_batch;
+    a.bias = d->bias; a.R = d->bias ? d->bias_radius : 0;
+    a.scale = d->scale;
+    a.cap2 = d->cap * LOG2E;
+    a.zs = d->cap > 0.f ? d->scale / d->cap : d->scale * LOG2E;
+    a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
+    a.nqt = (d->Lq + 127) / 128; a.nkt = (d->Lk + 127) / 128;
+    return a;
+}
+
+#define CHECK_LAUNCH()                                              \
+    do {                                                            \
+        hipError_t e_ = hipGetLastError();                          \
+        if (e_ != hipSuccess) return pf_set_err(hipGetErrorString(e_)); \
+    } while (0)
+
+template <int D, bool EX>
+int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
+    if (!few) {
+        const size_t lds = 4 * 64 * 2 * D + (EX ? (2 * MAX_RADIUS + 1) * 4 : 0);
+        PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, EX>), (int)lds);
+        range_fwd_kernel<D, EX><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
+        CHECK_LAUNCH();
+        return 0;
+    }
+    const size_t lds = 4 * 4 * 32 * 2 * D;                           // the meeting area [4][32][D + 4] fp32 is smaller
+    PF_SET_MAX_LDS_ONCE((range_split_kernel<D, EX>), (int)lds);
+    range_split_kernel<D, EX><<<(unsigned)(a.nrb * a.Hk * a.B * a.nsplit), 256, lds, stream>>>(a);
+    CHECK_LAUNCH();
+    if (a.nsplit > 1) {
+        const long long rows = (long long)a.B * a.Hk * a.Lq * a.G;
+        range_join_kernel<D><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(a);
+        CHECK_LAUNCH();
+    }
+    return 0;
+}
+
+template <int D, bool EX>
+int launch_bwd(const RArgs& a, hipStream_t stream) {
+    if (a.Lq > 0) {
+        range_prep_kernel<D><<<dim3((a.Lq + 63) / 64, a.H, a.B), 256, 0, stream>>>(a);
+        CHECK_LAUNCH();
+    }
+    if (a.Lk > 0) {
+        const size_t lds = 4 * 64 * 2 * D + 256 * 4 + 640 * 4 + (EX ? (2 * MAX_RADIUS + 1) * 4 : 0);
+        PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, EX>), (int)lds);
+        range_dkv_kernel<D, EX><<<(unsigned)(a.nkt * a.Hk * a.B), 256, lds, stream>>>(a);
+        CHECK_LAUNCH();
+    }
+    if (a.Lq > 0) {
+        const size_t lds = 4 * 64 * 2 * D + (EX ? 5 * (2 * a.R + 1) * 4 : 0);
+        PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, EX>), 4 * 64 * 2 * D + (EX ? 5 * (2 * MAX_RADIUS + 1) * 4 : 0));
+        range_dq_kernel<D, EX><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
+        CHECK_LAUNCH();
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" long long pf_attention_ranges_workspace_bytes(const pf_attn_ranges_desc* d) {
+    return check_ranges(d, false) ? -1 : fwd_bytes(d);
+}
+
+extern "C" long long pf_attention_ranges_bwd_workspace_bytes(const pf_attn_ranges_desc* d) {
+    if (check_ranges(d, true)) return -1;
+    const BwdSizes s = bwd_sizes(d);
+    return s.delta + s.tiles + s.parts;
+}
+
+extern "C" int pf_attention_ranges_which(const pf_attn_ranges_desc* d) {
+    return check_ranges(d, false) ? -1 : (few_rows(d) ? 2 : 1);
+}
+
+extern "C" int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, hipStream_t stream) {
+    if (const char* e = check_ranges(d, false)) return pf_set_err(e);
+    if (!d->B || !d->H || !d->Lq) return 0;
+    const long long need = fwd_bytes(d);
+    if (need && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need))
+        return pf_set_err("pf_attention_ranges_bf16: workspace missing, unaligned or too small");
+    RArgs a = range_args(d);
+    const bool few = few_rows(d), ex = d->bias || d->cap > 0.f;
+    const long long grid = few ? (long long)row_blocks(d) * d->Hkv * d->B * splits(d) : (long long)a.nqt * d->H * d->B;
+    if (grid > 0x7fffffffLL) return pf_set_err("pf_attention_ranges_bf16: too many workgroups");
+    a.nrb = row_blocks(d);
+    a.nsplit = few ? splits(d) : 1;
+    a.parts = (float*)d->workspace;
+    if (d->D == 64) return ex ? launch_fwd<64, true>(a, few, stream) : launch_fwd<64, false>(a, few, stream);
+    return ex ? launch_fwd<128, true>(a, few, stream) : launch_fwd<128, false>(a, few, stream);
+}
+
+extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t stream) {
+    if (const char* e = check_ranges(d, true)) return pf_set_err(e);
+    const BwdSizes s = bwd_sizes(d);
+    const long long need = s.delta + s.tiles + s.parts;
+    if (need && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need))
+        return pf_set_err("pf_attention_ranges_bwd: workspace missing, unaligned or too small");
+    if (d->B > 65535 || d->H > 65535) return pf_set_err("pf_attention_ranges_bwd: more than 65535 batch entries or heads");
+    if ((long long)((d->Lq + 127) / 128) * d->H * d->B > 0x7fffffffLL || (long long)((d->Lk + 127) / 128) * d->H * d->B > 0x7fffffffLL ||
+        (long long)(d->Lq + 63) / 64 * (d->H / (d->Hkv ? d->Hkv : 1)) > 0x7fffffffLL)
+        return pf_set_err("pf_attention_ranges_bwd: too many workgroups");
+    if (!d->H) return 0;
+    RArgs a = range_args(d);
+    a.delta = (float*)d->workspace;
+    a.tiles = (int*)((char*)d->workspace + s.delta);
+    a.dbias_parts = (float*)((char*)d->workspace + s.delta + s.tiles);
+    a.dbias = d->dbias;
+    const bool ex = d->bias || d->cap > 0.f;
+    int rc = 0;
+    if (!d->B) rc = 0;
+    else if (d->D == 64) rc = ex ? launch_bwd<64, true>(a, stream) : launch_bwd<64, false>(a, stream);
+    else rc = ex ? launch_bwd<128, true>(a, stream) : launch_bwd<128, false>(a, stream);
+    if (rc == 0 && d->dbias) {
+        range_dbias_kernel<<<dim3((2 * a.R + 1 + 63) / 64, a.H), 256, 0, stream>>>(a);
+        CHECK_LAUNCH();
+    }
+    return rc;
+}

@@ -19,6 +19,8 @@ extern "C" int pf_struct_size(int which) {
         case 1: return (int)sizeof(pf_conv_desc);
         case 2: return (int)sizeof(pf_attn_desc);
         case 3: return (int)sizeof(pf_attn_small_desc);
+        case 4: return (int)sizeof(pf_heads_desc);
+        case 5: return (int)sizeof(pf_attn_ranges_desc);
         default: return -1;
     }
 }

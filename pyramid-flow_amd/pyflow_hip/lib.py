@@ -67,6 +67,33 @@ class AttnSmallDesc(C.Structure):
                 ("bias", C.c_void_p), ("key_mask", C.c_void_p), ("causal", C.c_int), ("scale", C.c_float)]
 
 
+class RowsView(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("batch", C.c_longlong), ("row", C.c_longlong), ("head", C.c_longlong)]
+
+
+class HeadsDesc(C.Structure):
+    _fields_ = [("Q", RowsView), ("K", RowsView), ("Qo", RowsView), ("Ko", RowsView), ("dQ", RowsView), ("dK", RowsView),
+                ("wq", C.c_void_p), ("wk", C.c_void_p),
+                ("pos", C.c_void_p), ("pos_batch", C.c_longlong), ("pos_row", C.c_longlong),
+                ("freq", C.c_void_p), ("axis", C.c_void_p),
+                ("n_axes", C.c_int), ("n_pairs", C.c_int), ("halves", C.c_int),
+                ("B", C.c_int), ("L", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("D", C.c_int),
+                ("eps", C.c_float), ("q_scale", C.c_float)]
+
+
+class AttnRangesDesc(C.Structure):
+    _fields_ = [("Q", RowsView), ("K", RowsView), ("V", RowsView), ("O", RowsView),
+                ("dO", RowsView), ("dQ", RowsView), ("dK", RowsView), ("dV", RowsView),
+                ("LSE", C.c_void_p),
+                ("a_lo", C.c_void_p), ("a_hi", C.c_void_p), ("b_lo", C.c_void_p), ("b_hi", C.c_void_p),
+                ("range_batch", C.c_longlong), ("q_pos", C.c_void_p), ("q_pos_batch", C.c_longlong),
+                ("bias", C.c_void_p), ("dbias", C.c_void_p),
+                ("bias_radius", C.c_int), ("B", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("Lq", C.c_int),
+                ("Lk", C.c_int), ("D", C.c_int),
+                ("scale", C.c_float), ("cap", C.c_float),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong)]
+
+
 ABI_VERSION = 7          # PF_ABI_VERSION of include/pyflow_hip.h
 GEMM_GATE_RES = 1
 GEMM_OUT_F32 = 2
@@ -80,6 +107,9 @@ EXPORTS = [
     "pf_copy_rows", "pf_sp_relayout", "pf_renoise_upsample", "pf_avgpool2",
     "pf_gn_stats", "pf_gn_apply", "pf_softmax_rows", "pf_shift_caches", "pf_latent_to_nhwc", "pf_blend_tiles", "pf_nhwc_to_planar_f32", "pf_to_uint8",
     "pf_embed_rows", "pf_rmsnorm", "pf_glu_mul", "pf_attention_small_bf16", "pf_rgb_to_yuv420",
+    "pf_qk_norm_rope_axes", "pf_qk_norm_rope_axes_bwd", "pf_qk_norm_rope_axes_bwd_workspace_bytes",
+    "pf_attention_ranges_bf16", "pf_attention_ranges_bwd", "pf_attention_ranges_workspace_bytes",
+    "pf_attention_ranges_bwd_workspace_bytes", "pf_attention_ranges_which",
     "pf_comm_unique_id", "pf_comm_init", "pf_comm_destroy", "pf_comm_rank", "pf_comm_world", "pf_all_to_all_v",
     "pf_halo_send_recv", "pf_all_gather_v", "pf_all_reduce_sum_f32", "pf_broadcast_bytes", "pf_comm_wait",
     "pf_cmdlist_create", "pf_cmdlist_destroy", "pf_cmdlist_clear", "pf_cmdlist_size", "pf_cmdlist_is_graph", "pf_cmdlist_gemm",
@@ -117,9 +147,12 @@ def load():
     lib.pf_cmdlist_create.restype = C.c_void_p
     lib.pf_attention_workspace_bytes.restype = C.c_longlong
     lib.pf_gemm_workspace_bytes.restype = C.c_longlong
+    for name in ("pf_qk_norm_rope_axes_bwd_workspace_bytes", "pf_attention_ranges_workspace_bytes",
+                 "pf_attention_ranges_bwd_workspace_bytes"):
+        getattr(lib, name).restype = C.c_longlong
     if lib.pf_version() != ABI_VERSION:
         raise RuntimeError(f"pyflow_hip: {LIB_PATH} has ABI version {lib.pf_version()}, this host expects {ABI_VERSION}: rebuild it")
-    for which, cls in enumerate((GemmDesc, ConvDesc, AttnDesc, AttnSmallDesc)):       # struct mirrors vs the compiled layout
+    for which, cls in enumerate((GemmDesc, ConvDesc, AttnDesc, AttnSmallDesc, HeadsDesc, AttnRangesDesc)):       # struct mirrors vs the compiled layout
         if lib.pf_struct_size(C.c_int(which)) != C.sizeof(cls):
             raise RuntimeError(f"pyflow_hip: {cls.__name__} is {C.sizeof(cls)} bytes here but "
                                f"{lib.pf_struct_size(C.c_int(which))} in {LIB_PATH}: stale library? rebuild it")

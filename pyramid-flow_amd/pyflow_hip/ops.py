@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import lib as L
-from .lib import (GemmDesc, AttnDesc, AttnSmallDesc, ConvDesc, check, ptr, stream, GEMM_GATE_RES,  # noqa: F401
+from .lib import (GemmDesc, AttnDesc, AttnSmallDesc, ConvDesc, HeadsDesc, AttnRangesDesc, check, ptr, stream, GEMM_GATE_RES,  # noqa: F401
                   GEMM_OUT_F32, GEMM_ACT_QUICK_GELU, GEMM_ACT_GELU_ERF)
 
 
@@ -311,3 +311,201 @@ def attention_small(qkv, O, q_off, k_off, v_off, ld, ldo, B, H, Lseq, scale, bia
     d.scale = scale
     PROFILER.launch("attention_small", 4.0 * B * H * Lseq * Lseq * 64,
                     lambda: check(lib.pf_attention_small_bf16(C.byref(d), stream())))
+
+
+# ---------------------------------------------------------------------------------------------- attention over key ranges
+def _rows(view, t, shape, what, out=False):
+    """fills a pf_rows_view from a bf16 [B, L, H, D] tensor (any strides that are multiples of 8, channels dense)"""
+    if t.dtype != torch.bfloat16 or t.shape != shape:
+        raise ValueError(f"{what}: expected bfloat16 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if not t.numel():
+        return
+    sb, sr, sh, sc = t.stride()
+    nb, nr, nh, _ = shape
+    if sc != 1:
+        raise ValueError(f"{what}: the channels of a head must be dense")
+    # the stride of a dimension of one entry says nothing
+    sb, sr, sh = sb if nb > 1 else 0, sr if nr > 1 else 0, sh if nh > 1 else 0
+    p = t.data_ptr()
+    if (sb | sr | sh) % 8 or p % 16:
+        raise ValueError(f"{what}: data must be 16-byte aligned and strides multiples of 8 elements")
+    if out and ((nb > 1 and not sb) or (nr > 1 and not sr) or (nh > 1 and not sh)):
+        raise ValueError(f"{what}: an expanded tensor cannot be written")
+    view.p, view.batch, view.row, view.head = p, sb, sr, sh
+
+
+def _f32(t, shape, what):
+    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous float32 tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _one_device(what, *tensors):
+    """every tensor on torch's current device (whose current stream the launch goes to); nothing recordable"""
+    if RECORDER is not None:
+        raise RuntimeError(f"{what}: not available while a launch list is being recorded")
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            raise ValueError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
+
+
+def _scratch(what, need, workspace, device):
+    """`need` bytes of scratch: the caller's, or a new allocation (ordered with the current stream by torch's allocator)"""
+    if need < 0:
+        raise RuntimeError(f"{what}: invalid arguments")
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
+        raise ValueError(f"{what}: the workspace must be contiguous and hold {need} bytes")
+    return workspace
+
+
+def _heads_desc(what, q, k, q_out, k_out, wq, wk, rope, pos, eps, q_scale):
+    _one_device(what, q, k, q_out, k_out, wq, wk, rope.freq, rope.axis, pos)
+    if (q is None) != (q_out is None) or (k is None) != (k_out is None) or (q is None and k is None):
+        raise ValueError(f"{what}: q and / or k, each with its output")
+    x = q if q is not None else k
+    if x.dim() != 4:
+        raise ValueError(f"{what}: expected [B, L, heads, head_dim]")
+    B, L, _, D = x.shape
+    d = HeadsDesc()
+    d.B, d.L, d.D, d.eps, d.q_scale = B, L, D, eps, q_scale
+    if q is not None:
+        d.H = q.shape[2]
+        _rows(d.Q, q, q.shape, what)
+        _rows(d.Qo, q_out, q.shape, what, out=True)
+        if wq is not None:
+            d.wq = _f32(wq, (D,), what)
+    if k is not None:
+        d.Hkv = k.shape[2]
+        shape = (B, L, k.shape[2], D)
+        _rows(d.K, k, shape, what)
+        _rows(d.Ko, k_out, shape, what, out=True)
+        if wk is not None:
+            d.wk = _f32(wk, (D,), what)
+    d.n_pairs, d.halves = rope.n_pairs, rope.halves
+    if pos.dtype != torch.float32 or pos.dim() != 3 or pos.shape[0] not in (1, B) or pos.shape[1] != L:
+        raise ValueError(f"{what}: positions must be float32 [B or 1, L, axes]")
+    n_axes = pos.shape[2]
+    if pos.numel():
+        if n_axes > 1 and pos.stride(2) != 1:
+            raise ValueError(f"{what}: the axes of a position must be dense")
+        d.pos_batch, d.pos_row = pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1) if L > 1 else 0
+        d.pos = pos.data_ptr()
+    d.n_axes, d.freq, d.axis = n_axes, rope.freq.data_ptr(), rope.axis.data_ptr()
+    return d
+
+
+def qk_norm_rope_axes(q, k, q_out, k_out, wq, wk, rope, pos, eps=1e-6, q_scale=1.0):
+    """q_out, k_out = RMSNorm of every head (gains wq / wk fp32 [D], None = none), rotated by `rope` (plan.RopeAxes) at the
+    positions `pos` (fp32 [B or 1, L, axes]; fractions allowed), q times q_scale.  q [B, L, H, D], k [B, L, Hkv, D] bf16 views
+    (column blocks of a projection are fine), D 64 or 128; either pair may be None; an output may be its input."""
+    d = _heads_desc("qk_norm_rope_axes", q, k, q_out, k_out, wq, wk, rope, pos, eps, q_scale)
+    check(L.load().pf_qk_norm_rope_axes(C.byref(d), stream()))
+
+
+def qk_norm_rope_axes_backward(dq, dk, q, k, wq, wk, rope, pos, dq_in, dk_in, dwq=None, dwk=None, eps=1e-6, q_scale=1.0,
+                               workspace=None):
+    """Gradients of qk_norm_rope_axes: dq, dk of its results and its inputs q, k -> dq_in, dk_in (may be dq, dk) and, where given,
+    the gains' gradients dwq, dwk (fp32 [D])."""
+    what = "qk_norm_rope_axes_backward"
+    lib = L.load()
+    d = _heads_desc(what, q, k, dq_in, dk_in, wq, wk, rope, pos, eps, q_scale)
+    _one_device(what, dq, dk, dwq, dwk, workspace)
+    if (dq is None) != (q is None) or (dk is None) != (k is None):
+        raise ValueError(f"{what}: a gradient for each of q and k that is given")
+    if dq is not None:
+        _rows(d.dQ, dq, q.shape, what)
+    if dk is not None:
+        _rows(d.dK, dk, k.shape, what)
+    pwq = _f32(dwq, (d.D,), what) if dwq is not None else 0
+    pwk = _f32(dwk, (d.D,), what) if dwk is not None else 0
+    if (pwq and not d.wq) or (pwk and not d.wk):
+        raise ValueError(f"{what}: a gain gradient without its gains")
+    ws = nbytes = None
+    if pwq or pwk:
+        ws = _scratch(what, lib.pf_qk_norm_rope_axes_bwd_workspace_bytes(C.byref(d)), workspace, (q if q is not None else k).device)
+        nbytes = ws.numel() * ws.element_size() if ws is not None else 0
+    check(lib.pf_qk_norm_rope_axes_bwd(C.byref(d), C.c_void_p(pwq), C.c_void_p(pwk), ptr(ws), C.c_longlong(nbytes or 0), stream()))
+
+
+def _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap):
+    r = ranges
+    _one_device(what, q, k, v, out, lse, bias, q_pos, *((r.a_lo,) if r is not None else ()))
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"{what}: expected q [B, Lq, H, D] and k, v [B, Lk, Hkv, D]")
+    B, Lq, H, D = q.shape
+    _, Lk, Hkv, _ = k.shape
+    kv = (B, Lk, Hkv, D)
+    d = AttnRangesDesc()
+    d.B, d.H, d.Hkv, d.Lq, d.Lk, d.D = B, H, Hkv, Lq, Lk, D
+    _rows(d.Q, q, q.shape, what)
+    _rows(d.K, k, kv, what)
+    _rows(d.V, v, kv, what)
+    d.scale, d.cap = D ** -0.5 if scale is None else scale, cap
+    if lse is not None:
+        d.LSE = _f32(lse, (B, H, Lq), what)
+    if r is not None:
+        n = r.a_lo.shape[0]
+        if r.a_lo.shape[1] != Lq or n not in (1, B):
+            raise ValueError(f"{what}: key ranges of {tuple(r.a_lo.shape)} rows for q of {(B, Lq)}")
+        if Lq:
+            d.a_lo, d.a_hi = r.a_lo.data_ptr(), r.a_hi.data_ptr()
+            if r.b_lo is not None:
+                d.b_lo, d.b_hi = r.b_lo.data_ptr(), r.b_hi.data_ptr()
+            d.range_batch = Lq if n > 1 else 0
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[1] % 2 == 0:
+            raise ValueError(f"{what}: bias must be [H, 2 radius + 1]")
+        d.bias, d.bias_radius = _f32(bias, (H, bias.shape[1]), what), bias.shape[1] // 2
+    if q_pos is not None:
+        if q_pos.dtype != torch.int32 or q_pos.dim() != 2 or q_pos.shape[1] != Lq or q_pos.shape[0] not in (1, B) or not q_pos.is_contiguous():
+            raise ValueError(f"{what}: q_pos must be contiguous int32 [B or 1, Lq]")
+        if Lq:
+            d.q_pos, d.q_pos_batch = q_pos.data_ptr(), Lq if q_pos.shape[0] > 1 else 0
+    return d
+
+
+def attention_ranges(q, k, v, out, ranges=None, scale=None, bias=None, q_pos=None, cap=0.0, lse=None, workspace=None):
+    """out = softmax(t) v over the keys each row sees (plan.KeyRanges; None = all), t = cap tanh(scale q.k / cap) (cap 0: scale q.k)
+    + bias[h][clamp(j - pos, -R, R) + R].  q, out [B, Lq, H, D] and k, v [B, Lk, Hkv, D] bf16 views, D 64 or 128, H a multiple of
+    Hkv; scale defaults to D^-1/2; bias fp32 [H, 2 R + 1], R <= 512 (entries <= -1e30 hide their distance); q_pos int32 [B or 1,
+    Lq] positions of the rows among the keys (default i + Lk - Lq); lse fp32 [B, H, Lq] receives log sum exp t.  A row that sees
+    nothing gets zeros (lse -inf).  out may be q.  Few rows over many keys (single tokens over a cache) split the keys."""
+    what = "attention_ranges"
+    lib = L.load()
+    d = _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap)
+    _rows(d.O, out, q.shape, what, out=True)
+    need = lib.pf_attention_ranges_workspace_bytes(C.byref(d))
+    if need > 0:
+        _one_device(what, workspace)
+        ws = _scratch(what, need, workspace, q.device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+    PROFILER.launch("attention_ranges", 0.0, lambda: check(lib.pf_attention_ranges_bf16(C.byref(d), stream())))
+
+
+def attention_ranges_backward(dout, q, k, v, out, lse, dq, dk, dv, ranges=None, scale=None, bias=None, q_pos=None, cap=0.0,
+                              dbias=None, workspace=None):
+    """Gradients of attention_ranges from its result `out` and `lse`: dq, dk, dv (bf16, shapes of q, k, v) and, where given,
+    dbias (fp32, shape of bias).  The same bits every time."""
+    what = "attention_ranges_backward"
+    lib = L.load()
+    d = _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap)
+    _one_device(what, dout, dq, dk, dv, dbias, workspace)
+    _rows(d.O, out, q.shape, what)
+    _rows(d.dO, dout, q.shape, what)
+    _rows(d.dQ, dq, q.shape, what, out=True)
+    _rows(d.dK, dk, k.shape, what, out=True)
+    _rows(d.dV, dv, k.shape, what, out=True)
+    if dbias is not None:
+        if bias is None:
+            raise ValueError(f"{what}: a bias gradient without a bias")
+        d.dbias = _f32(dbias, bias.shape, what)
+    need = lib.pf_attention_ranges_bwd_workspace_bytes(C.byref(d))
+    if need < 0:
+        check(lib.pf_attention_ranges_bwd(C.byref(d), stream()))      # names the argument
+    ws = _scratch(what, need, workspace, q.device)
+    if ws is not None:
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+    PROFILER.launch("attention_ranges_bwd", 0.0, lambda: check(lib.pf_attention_ranges_bwd(C.byref(d), stream())))

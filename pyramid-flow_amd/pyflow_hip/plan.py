@@ -104,3 +104,101 @@ class SequencePlan:
             cache[q_row_begin] = int((h["a_hi"][:, r:] - h["a_lo"][:, r:]).astype(np.int64).sum()
                                      + (h["b_hi"][:, r:] - self.Lt).astype(np.int64).sum())
         return cache[q_row_begin]
+
+
+class RopeAxes:
+    """Rotation of head channels by several position axes, for ops.qk_norm_rope_axes: pair p turns by
+    ``pos[axis[p]] * freq[p]`` radians.  ``freq`` float64 and ``axis`` int32, both [n_pairs] device tensors; pairs are channels
+    (2 p, 2 p + 1), or (p, p + n_pairs) with ``halves``; channels behind 2 n_pairs pass through."""
+
+    def __init__(self, freq, axis, halves=False):
+        if freq.dtype != torch.float64 or axis.dtype != torch.int32 or freq.dim() != 1 or freq.shape != axis.shape:
+            raise ValueError("RopeAxes: freq must be float64 [n_pairs] and axis int32 [n_pairs]")
+        if not (freq.is_contiguous() and axis.is_contiguous()) or freq.device != axis.device:
+            raise ValueError("RopeAxes: freq and axis must be contiguous and on one device")
+        self.freq, self.axis, self.halves, self.n_pairs = freq, axis, bool(halves), freq.numel()
+
+    @classmethod
+    def build(cls, axes_dim, device, theta=10000.0, halves=False):
+        """``axes_dim`` channels per axis, each axis with its own spectrum theta^(-2 k / dim) (as rope_cos_sin)."""
+        if any(d <= 0 or d % 2 for d in axes_dim):
+            raise ValueError("RopeAxes: channels per axis must be positive and even")
+        freq = torch.cat([1.0 / (theta ** (torch.arange(0, d, 2, dtype=torch.float64) / d)) for d in axes_dim])
+        axis = torch.cat([torch.full((d // 2,), n, dtype=torch.int32) for n, d in enumerate(axes_dim)])
+        return cls(freq.to(device), axis.to(device), halves)
+
+
+class KeyRanges:
+    """The keys each row sees, for ops.attention_ranges: [a_lo, a_hi) and, if given, [b_lo, b_hi) -- int32 [B][Lq] (or [1][Lq]:
+    shared by the batch) device tensors.  A row with two empty ranges sees nothing."""
+
+    def __init__(self, a_lo, a_hi, b_lo=None, b_hi=None):
+        if (b_lo is None) != (b_hi is None):
+            raise ValueError("KeyRanges: a second range needs its start and its end")
+        for t in (a_lo, a_hi, b_lo, b_hi):
+            if t is None:
+                continue
+            if t.dtype != torch.int32 or t.dim() != 2 or t.shape != a_lo.shape or t.device != a_lo.device or not t.is_contiguous():
+                raise ValueError("KeyRanges: ranges must be contiguous int32 [B or 1][Lq] tensors of one shape on one device")
+        self.a_lo, self.a_hi, self.b_lo, self.b_hi = a_lo, a_hi, b_lo, b_hi
+
+    @classmethod
+    def _of(cls, device, *arrays):
+        return cls(*[None if a is None else torch.from_numpy(np.ascontiguousarray(np.atleast_2d(a), dtype=np.int32)).to(device)
+                     for a in arrays])
+
+    @classmethod
+    def causal(cls, Lq, Lk, device):
+        """row i is key Lk - Lq + i and sees the keys up to itself"""
+        return cls._of(device, np.zeros(Lq), np.arange(Lq) + (Lk - Lq) + 1)
+
+    @classmethod
+    def padded(cls, lengths, Lq, device):
+        """every row of batch entry b sees the first lengths[b] keys"""
+        hi = np.repeat(np.asarray(lengths)[:, None], Lq, 1)
+        return cls._of(device, np.zeros_like(hi), hi)
+
+    @classmethod
+    def documents(cls, lengths, L, device, causal=False):
+        """documents packed one behind the other into L rows; rows behind the last one see nothing"""
+        lengths = np.asarray(lengths, dtype=np.int64)
+        if (lengths < 0).any() or lengths.sum() > L:
+            raise ValueError("KeyRanges.documents: lengths must be >= 0 and fit into L")
+        end = np.cumsum(lengths)
+        lo, hi = np.zeros(L, np.int64), np.zeros(L, np.int64)
+        used = int(lengths.sum())
+        lo[:used], hi[:used] = np.repeat(end - lengths, lengths), np.repeat(end, lengths)
+        if causal:
+            hi[:used] = np.arange(used) + 1
+        return cls._of(device, lo, hi)
+
+    @classmethod
+    def prefix(cls, prefix, L, device):
+        """the first prefix[b] keys are seen by all rows, later ones by the rows from themselves on"""
+        return cls._of(device, np.zeros((len(prefix), L)), np.maximum(np.arange(L)[None] + 1, np.minimum(np.asarray(prefix), L)[:, None]))
+
+    @classmethod
+    def from_key_mask(cls, mask, Lq, device):
+        """mask [B][Lk], nonzero = visible to every row: at most two runs of visible keys per batch entry"""
+        mask = np.asarray(mask.cpu() if isinstance(mask, torch.Tensor) else mask) != 0
+        out = np.zeros((4, mask.shape[0], Lq), np.int64)
+        for b, row in enumerate(mask):
+            edges = np.flatnonzero(np.diff(np.concatenate([[0], row.astype(np.int8), [0]])))
+            if len(edges) > 4:
+                raise NotImplementedError("KeyRanges.from_key_mask: more than two runs of visible keys")
+            for n, e in enumerate(edges):
+                out[n, b] = e
+        return cls._of(device, *out)
+
+    @classmethod
+    def from_plan(cls, plan):
+        """the joint text-video mask of a SequencePlan"""
+        return cls(plan.a_lo, plan.a_hi, torch.full_like(plan.b_hi, plan.Lt), plan.b_hi)
+
+    def dense_mask(self, Lk):
+        """[B or 1, Lq, Lk] bool -- test helper: the mask the ranges stand for"""
+        j = torch.arange(Lk, device=self.a_lo.device)
+        seen = (j >= self.a_lo[..., None]) & (j < self.a_hi[..., None])
+        if self.b_lo is not None:
+            seen |= (j >= self.b_lo[..., None]) & (j < self.b_hi[..., None])
+        return seen
