@@ -42,8 +42,11 @@ struct RArgs {
     int B, H, Hk, G, Lq, Lk;
     int nqt, nkt, nrb, nsplit;
     float* parts;                      // split forward: [unit][split][32][D + 2]
-    float* delta;                      // backward: [B][H][Lq]
-    int* tiles;                        // backward: [B][ceil(Lq / 64)][8] bounds of 64-row tiles
+    float* stat;                       // backward: [B][H][nq64][4][64] lse log2 e, -delta, position, 0
+    int* vis;                          // backward: [B][nq64][4][64] the rows' ranges (Vis)
+    int* tiles;                        // backward: [B][nq64][8] bounds of 64-row tiles
+    int nq64;
+    float* kv_parts; int kv_split;     // backward: [part][B][Hk][Lk][2][D] unscaled dK, dV of a part of the rows
     float* dbias_parts; float* dbias;  // backward: [B][H][nqt][2 R + 1]
 };
 
@@ -277,10 +280,10 @@ PF_DEVICE bool exact_pair(const RArgs& p, int b, int h, int hk, int i, int j, fl
     const float z = dot_row<D>(p.q.p + b * p.q.bs + i * p.q.ld + h * p.q.hs, p.k.p + b * p.k.bs + j * p.k.ld + hk * p.k.hs);
     const float t = score2(p, z, h, j - row_pos(p, b, i), th);
     if (t == -__builtin_inff()) return false;
-    const long long at = ((long long)b * p.H + h) * p.Lq + i;
-    P = __builtin_amdgcn_exp2f(t - p.lse[at] * LOG2E);
+    const float* st = p.stat + (((long long)b * p.H + h) * p.nq64 + (i >> 6)) * 256 + (i & 63);
+    P = __builtin_amdgcn_exp2f(t - st[0]);
     const float dp = dot_row<D>(p.dO.p + b * p.dO.bs + i * p.dO.ld + h * p.dO.hs, p.v.p + b * p.v.bs + j * p.v.ld + hk * p.v.hs);
-    dz = P * (dp - p.delta[at]) * (1.f - th * th);
+    dz = P * (dp + st[64]) * (1.f - th * th);
     return true;
 }
 template <int D>
@@ -347,25 +350,23 @@ PF_DEVICE void load_table(const RArgs& p, int h, float* tab) {
 }
 
 // raw products -> base-2 scores with cap and bias; rel0 = key of register 0 minus the row's position (keys in registers)
-PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0, f32x16_t* th) {
+template <int MODE>
+PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         float t = s[r] * p.zs;
-        if (p.cap2 != 0.f) {
-            const float x = tanh_f(t);
-            if (th) (*th)[r] = x;
-            t = p.cap2 * x;
-        }
-        if (p.bias) t += tab[min(max(rel0 + reg_row(r), -p.R), p.R) + p.R];
+        if (MODE & 1) t = p.cap2 * tanh_f(t);
+        if (MODE & 2) t += tab[min(max(rel0 + reg_row(r), -p.R), p.R) + p.R];
         s[r] = t;
     }
 }
 
 // ---------------------------------------------------------------------------------------------- forward, many rows
-// One workgroup = 128 rows of one head, 4 waves x 32; key tiles of 64, two in flight.  EX: cap and / or bias (scores are formed
-// in base 2 before the maximum), else scores stay raw and the exponent's multiply-add scales them.
-template <int D, bool EX>
+// One workgroup = 128 rows of one head, 4 waves x 32; key tiles of 64, two in flight.  MODE: 1 cap, 2 bias, 3 both (scores are
+// formed in base 2 before the maximum), 0 neither (scores stay raw, the exponent's multiply-add scales them).
+template <int D, int MODE>
 __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
     constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     float* const tab = (float*)(smem + 2 * BUF);
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
     const int hi = lane >> 5, row = qt * 128 + wid * 32 + (lane & 31);
     const Vis vis = load_vis(p, b, row);
-    const int pos = EX && p.bias ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
+    const int pos = BIAS ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
 
     // ---- the workgroup's key tiles
     int* const red = (int*)smem;
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
         const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
         if (lane == 0) { red[4 * wid] = amin; red[4 * wid + 1] = amax; red[4 * wid + 2] = bmin; red[4 * wid + 3] = bmax; }
     }
-    if (EX && p.bias) load_table(p, h, tab);
+    if (BIAS) load_table(p, h, tab);
     __syncthreads();
     TileList tl;
     {
@@ -440,7 +441,7 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
         }
         if (EX) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) cap_bias(p, s[i], tab, j0 + 32 * i + 4 * hi - pos, nullptr);
+            for (int i = 0; i < 2; ++i) cap_bias<MODE>(p, s[i], tab, j0 + 32 * i + 4 * hi - pos);
         }
         if (!full) {
 #pragma unroll
@@ -506,8 +507,9 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
 // One workgroup = 32 (row, head) pairs that share a key head, one part of the keys; its 4 waves take every fourth 32-key tile of
 // the part and meet in LDS at the end.  Tiles are private to a wave: no barrier in the loop, the next tile is in flight while the
 // current one is used.  nsplit > 1: parts go to the workspace, range_join_kernel adds them.
-template <int D, bool EX>
+template <int D, int MODE>
 __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
     constexpr int TILE = 32 * 2 * D, BUF = 2 * TILE, WAVE = 2 * BUF, NP = 2 * 32 / (512 / D);
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -520,8 +522,8 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
     const int row = valid ? rho / p.G : p.Lq - 1, h = hk * p.G + (valid ? rho % p.G : 0);
     Vis vis = load_vis(p, b, row);
     if (!valid) vis.na = vis.nb = 0;
-    const int pos = EX && p.bias ? row_pos(p, b, row) : 0;
-    const float* const bias = EX && p.bias ? p.bias + (long long)h * (2 * p.R + 1) + p.R : nullptr;
+    const int pos = BIAS ? row_pos(p, b, row) : 0;
+    const float* const bias = BIAS ? p.bias + (long long)h * (2 * p.R + 1) + p.R : nullptr;
     const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
     const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
     const TileList tl = tile_list<32>(__builtin_amdgcn_readfirstlane(amin), __builtin_amdgcn_readfirstlane(amax),
@@ -566,8 +568,8 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float t = s[r] * p.zs;
-            if (EX && p.cap2 != 0.f) t = p.cap2 * tanh_f(t);
-            if (EX && bias) t += bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]);
+            if (CAP) t = p.cap2 * tanh_f(t);
+            if (BIAS) t += bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]);
             s[r] = sees(vis, k0 + reg_row(r)) ? t : -__builtin_inff();
         }
         float mt = s[0];
@@ -692,12 +694,13 @@ __global__ __launch_bounds__(256) void range_join_kernel(const RArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------- backward
-// delta[b][h][i] = sum_c dO O (four lanes per row), and for each 64-row tile the bounds of its key ranges: 0..3 the smallest start
-// and largest end of the a and b ranges that are not empty; 4..7 the largest start and smallest end over ALL its rows.
+// What both gradient kernels need of a row, in 1-KiB pieces of 64 rows that the LDS-DMA can take as they are: log-sum-exp (base 2)
+// and -delta = -sum_c dO O per head, the ranges per batch entry; and for each such tile the bounds of its ranges: 0..3 the smallest
+// start and largest end of the a and b ranges that are not empty, 4..7 the largest start and smallest end over ALL its rows.
 template <int D>
 __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
     const int qt = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-    const int row = qt * 64 + (threadIdx.x >> 2), sub = threadIdx.x & 3;
+    const int r = threadIdx.x >> 2, row = qt * 64 + r, sub = threadIdx.x & 3;
     float s = 0.f;
     if (row < p.Lq) {
         const bf16_t* x = p.dO.p + b * p.dO.bs + row * p.dO.ld + h * p.dO.hs + sub * (D / 4);
@@ -706,38 +709,46 @@ __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
     }
     s += __shfl_xor(s, 1);
     s += __shfl_xor(s, 2);
-    if (row < p.Lq && sub == 0) p.delta[((long long)b * p.H + h) * p.Lq + row] = s;
+    float* st = p.stat + (((long long)b * p.H + h) * p.nq64 + qt) * 256 + r;
+    const bool on = row < p.Lq;
+    if (sub == 0) st[0] = on ? p.lse[((long long)b * p.H + h) * p.Lq + row] * LOG2E : 0.f;
+    if (sub == 1) st[64] = on ? -s : 0.f;
+    if (sub == 2) ((int*)st)[128] = on ? row_pos(p, b, row) : 0;
+    if (sub == 3) st[192] = 0.f;
     if (h == 0 && threadIdx.x < 64) {
-        const int r = qt * 64 + threadIdx.x;
-        const Vis v = load_vis(p, b, r);
+        const Vis v = load_vis(p, b, qt * 64 + threadIdx.x);
+        const long long tile = (long long)b * p.nq64 + qt;
+        int* vp = p.vis + tile * 256 + threadIdx.x;
+        vp[0] = v.alo; vp[64] = v.na; vp[128] = v.blo; vp[192] = v.nb;
         int x[8] = {v.na ? v.alo : 0x7fffffff, v.na ? v.alo + v.na : 0, v.nb ? v.blo : 0x7fffffff, v.nb ? v.blo + v.nb : 0,
                     v.na ? v.alo : 0x7fffffff, v.na ? v.alo + v.na : 0, v.nb ? v.blo : 0x7fffffff, v.nb ? v.blo + v.nb : 0};
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (i == 0 || i == 2 || i == 5 || i == 7) ? wave_min(x[i]) : wave_max(x[i]);
         if (threadIdx.x == 0) {
-            int* t = p.tiles + ((long long)b * ((p.Lq + 63) / 64) + qt) * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = x[i];
+            for (int i = 0; i < 8; ++i) p.tiles[tile * 8 + i] = x[i];
         }
     }
 }
 
 // dK, dV of 128 keys of one key head: 4 waves x 32 keys held in registers, looping over the 64-row tiles (of every query head that
-// shares the key head) that see any of them.
-template <int D, bool EX>
-__global__ __launch_bounds__(256, 1) void range_dkv_kernel(const RArgs p) {
-    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
+// shares the key head) that see any of them.  The bounds of 64 tiles are tested at once (one lane each); the next tile is in
+// flight while one is used.  -delta enters through the C operand of the dP product.  kv_split > 1: this workgroup takes one part
+// of the (head, tile) list and leaves 32-bit sums for range_kvjoin_kernel.
+template <int D, int MODE>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void range_dkv_kernel(const RArgs p) {
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
+    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE + 2048;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    float* const rowf = (float*)(smem + 2 * BUF);                   // [2][2][64]: lse (base 2), delta
-    int* const rowi = (int*)(rowf + 256);                           // [2][5][64]: ranges, position
-    float* const tab = (float*)(rowi + 640);
+    float* const tab = (float*)(smem + 2 * BUF);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = xcd_remap(blockIdx.x, p.nkt * p.Hk * p.B);
-    const int bk = t / p.nkt, kt = t - bk * p.nkt;
+    const int t = xcd_remap(blockIdx.x, p.nkt * p.kv_split * p.Hk * p.B);
+    const int unit = t / p.kv_split, part = t - unit * p.kv_split;
+    const int bk = unit / p.nkt, kt = unit - bk * p.nkt;
     const int b = bk / p.Hk, hk = bk - b * p.Hk;
     const int hi = lane >> 5;
     const int w0 = kt * 128 + wid * 32, key = w0 + (lane & 31);
-    const int nq = (p.Lq + 63) / 64;
+    const int nq = p.nq64;
     const int* const tiles = p.tiles + (long long)b * nq * 8;
     bf16x8_t kf[D / 16], vf[D / 16];
     {
@@ -755,50 +766,71 @@ __global__ __launch_bounds__(256, 1) void range_dkv_kernel(const RArgs p) {
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = zero16();
     const int wg0 = kt * 128, wg1 = min(wg0 + 128, p.Lk);
-    // tiles are numbered g nq + qt; the next one at or behind n that sees a key of this workgroup
-    auto next = [&](int n) {
-        for (; n < p.G * nq; ++n) {
-            const int* x = tiles + (n % nq) * 8;
-            if ((x[0] < wg1 && x[1] > wg0) || (x[2] < wg1 && x[3] > wg0)) break;
+
+    // ---- the (head, tile) pairs n = g nq + tile of this part, 64 at a time: which the workgroup needs, which this wave sees at all,
+    //      which it sees whole
+    const int total = p.G * nq;
+    int base = (int)((long long)total * part / p.kv_split), group = 0;
+    const int end = (int)((long long)total * (part + 1) / p.kv_split);
+    unsigned long long need = 0, some = 0, all = 0;
+    auto refill = [&] {
+        while (need == 0 && base < end) {
+            const int n = base + lane;
+            int x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (n < end) {
+                const u32x4_t u = *(const u32x4_t*)(tiles + (n % nq) * 8), v = *(const u32x4_t*)(tiles + (n % nq) * 8 + 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { x[i] = (int)u[i]; x[4 + i] = (int)v[i]; }
+            }
+            need = __builtin_amdgcn_ballot_w64((x[0] < wg1 && x[1] > wg0) || (x[2] < wg1 && x[3] > wg0));
+            some = __builtin_amdgcn_ballot_w64((x[0] < w0 + 32 && x[1] > w0) || (x[2] < w0 + 32 && x[3] > w0));
+            all = __builtin_amdgcn_ballot_w64((x[4] <= w0 && x[5] >= w0 + 32) || (x[6] <= w0 && x[7] >= w0 + 32));
+            group = base;
+            base += 64;
         }
-        return n;
+    };
+    struct Item { int n; bool any, full; };
+    auto pop = [&]() -> Item {
+        refill();
+        if (need == 0) return {-1, false, false};
+        const int i = __builtin_ctzll(need);
+        need &= need - 1;
+        return {group + i, ((some >> i) & 1) != 0, ((all >> i) & 1) != 0};
     };
     auto issue = [&](int n, int buf) {
-        const int h = hk * p.G + n / nq, i0 = (n % nq) * 64;
-        char* base = smem + buf * BUF;
-        stage<D, 64, 4>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, i0, p.Lq - 1, base, wid, lane);
-        stage<D, 64, 4>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, i0, p.Lq - 1, base + TILE, wid, lane);
-        const int r = i0 + lane, rc = min(r, p.Lq - 1);
-        const long long at = ((long long)b * p.H + h) * p.Lq + rc;
-        if (wid == 0) rowf[buf * 128 + lane] = p.lse[at] * LOG2E;
-        if (wid == 1) rowf[buf * 128 + 64 + lane] = p.delta[at];
-        if (wid == 2) {
-            const Vis v = load_vis(p, b, r);
-            int* x = rowi + buf * 320;
-            x[lane] = v.alo; x[64 + lane] = v.na; x[128 + lane] = v.blo; x[192 + lane] = v.nb;
-        }
-        if (wid == 3 && EX && p.bias) rowi[buf * 320 + 256 + lane] = row_pos(p, b, rc);
+        const int h = hk * p.G + n / nq, qt = n % nq;
+        char* dst = smem + buf * BUF;
+        stage<D, 64, 4>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, qt * 64, p.Lq - 1, dst, wid, lane);
+        stage<D, 64, 4>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, qt * 64, p.Lq - 1, dst + TILE, wid, lane);
+        if (wid == 0) glds16(p.stat + (((long long)b * p.H + h) * nq + qt) * 256 + lane * 4, dst + 2 * TILE);
+        if (wid == 1) glds16(p.vis + ((long long)b * nq + qt) * 256 + lane * 4, dst + 2 * TILE + 1024);
     };
-    int n = next(0), buf = 0, table_of = -1;
-    if (n < p.G * nq) issue(n, 0);
-    while (n < p.G * nq) {
+    Item cur = pop();
+    int buf = 0, table_of = -1;
+    if (cur.n >= 0) issue(cur.n, 0);
+    while (cur.n >= 0) {
         drain_barrier();
-        if (EX && p.bias && n / nq != table_of) {                   // uniform: another head, another bias table
-            table_of = n / nq;
+        if (BIAS && cur.n / nq != table_of) {               // uniform: another head, another bias table
+            table_of = cur.n / nq;
             load_table(p, hk * p.G + table_of, tab);
             drain_barrier();
         }
-        const int n2 = next(n + 1);
-        if (n2 < p.G * nq) issue(n2, buf ^ 1);
-        const int* x = tiles + (n % nq) * 8;
-        const bool any = (x[0] < w0 + 32 && x[1] > w0) || (x[2] < w0 + 32 && x[3] > w0);
-        const bool full = (x[4] <= w0 && x[5] >= w0 + 32) || (x[6] <= w0 && x[7] >= w0 + 32);
-        if (any) {
+        const Item nxt = pop();
+        if (nxt.n >= 0) issue(nxt.n, buf ^ 1);
+        if (cur.any) {
             const char* sq = smem + buf * BUF;
             const char* so = sq + TILE;
+            const float* st = (const float*)(sq + 2 * TILE);
+            const int* vi = (const int*)(sq + 2 * TILE + 1024);
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
-                f32x16_t s = zero16(), dp = zero16(), th;
+                f32x16_t s = zero16(), dp;
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const f32x4_t de = *(const f32x4_t*)(st + 64 + qb * 32 + 8 * q4 + 4 * hi);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = de[e];
+                }
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
                     s = mfma(row_frag<D>(sq, roff, qb, ks), kf[ks], s);
@@ -807,27 +839,44 @@ __global__ __launch_bounds__(256, 1) void range_dkv_kernel(const RArgs p) {
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
                     const int r0 = qb * 32 + 8 * q4 + 4 * hi;
-                    const f32x4_t ls = *(const f32x4_t*)(rowf + buf * 128 + r0), de = *(const f32x4_t*)(rowf + buf * 128 + 64 + r0);
-                    const int* ri = rowi + buf * 320 + r0;
+                    const f32x4_t ls = *(const f32x4_t*)(st + r0);
+                    if (EX) {
+                        const u32x4_t pos = *(const u32x4_t*)((const int*)st + 128 + r0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * q4 + e;
-                        float z = s[r] * p.zs, fac = 1.f;
-                        bool ok = full;
-                        if (!full) ok = sees(Vis{ri[e], ri[64 + e], ri[128 + e], ri[192 + e]}, key);
-                        if (EX && p.cap2 != 0.f) {
-                            const float y = tanh_f(z);
-                            z = p.cap2 * y;
-                            fac = __builtin_fmaf(-y, y, 1.f);
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = 4 * q4 + e;
+                            float z = s[r] * p.zs, fac = 1.f;
+                            if (CAP) {
+                                const float y = tanh_f(z);
+                                z = p.cap2 * y;
+                                fac = __builtin_fmaf(-y, y, 1.f);
+                            }
+                            if (BIAS) z += tab[min(max(key - (int)pos[e], -p.R), p.R) + p.R];
+                            const bool ok = z != -__builtin_inff();
+                            const float P = __builtin_amdgcn_exp2f(z - ls[e]);
+                            s[r] = ok ? P : 0.f;
+                            dp[r] = ok ? P * dp[r] * fac : 0.f;
                         }
-                        if (EX && p.bias) {
-                            z += tab[min(max(key - ri[256 + e], -p.R), p.R) + p.R];
-                            ok = ok && z != -__builtin_inff();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = 4 * q4 + e;
+                            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls[e]));
+                            dp[r] *= s[r];
                         }
-                        const float P = __builtin_amdgcn_exp2f(z - ls[e]);
-                        const float dz = P * (dp[r] - de[e]) * fac;
-                        s[r] = ok ? P : 0.f;
-                        dp[r] = ok ? dz : 0.f;
+                    }
+                }
+                if (!cur.full) {
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        const int* v = vi + qb * 32 + 8 * q4 + 4 * hi;
+                        const u32x4_t alo = *(const u32x4_t*)v, na = *(const u32x4_t*)(v + 64), blo = *(const u32x4_t*)(v + 128), nb = *(const u32x4_t*)(v + 192);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool ok = (unsigned)key - alo[e] < na[e] || (unsigned)key - blo[e] < nb[e];
+                            s[4 * q4 + e] = ok ? s[4 * q4 + e] : 0.f;
+                            dp[4 * q4 + e] = ok ? dp[4 * q4 + e] : 0.f;
+                        }
                     }
                 }
 #pragma unroll
@@ -841,8 +890,24 @@ __global__ __launch_bounds__(256, 1) void range_dkv_kernel(const RArgs p) {
                 }
             }
         }
-        n = n2;
+        cur = nxt;
         buf ^= 1;
+    }
+    if (p.kv_split > 1) {
+        if (key < p.Lk) {
+            float* out = p.kv_parts + (((long long)part * p.B * p.Hk + bk) * p.Lk + key) * (2 * D) + 4 * hi;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    f32x4_t x, y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { x[e] = dk[c][4 * q4 + e]; y[e] = dv[c][4 * q4 + e]; }
+                    *(f32x4_t*)(out + 32 * c + 8 * q4) = x;
+                    *(f32x4_t*)(out + D + 32 * c + 8 * q4) = y;
+                }
+        }
+        return;
     }
     const bool bad = key < p.Lk && (any_nonfinite<D / 32>(dk) || any_nonfinite<D / 32>(dv));
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
@@ -858,11 +923,39 @@ __global__ __launch_bounds__(256, 1) void range_dkv_kernel(const RArgs p) {
     }
 }
 
+// one wave per key: the parts' dK and dV, added in part order
+template <int D>
+__global__ __launch_bounds__(256) void range_kvjoin_kernel(const RArgs p) {
+    const int lane = threadIdx.x & 63;
+    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), keys = (long long)p.B * p.Hk * p.Lk;
+    if (w >= keys) return;
+    const int bk = (int)(w / p.Lk), j = (int)(w - (long long)bk * p.Lk), b = bk / p.Hk, hk = bk - b * p.Hk;
+    float k[2] = {0.f, 0.f}, v[2] = {0.f, 0.f};
+    for (int s = 0; s < p.kv_split; ++s) {
+        const float* a = p.kv_parts + (s * keys + w) * (2 * D) + lane * (D / 64);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) { k[c] += a[c]; v[c] += a[D + c]; }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+        bad = bad || !(fabsf(k[c]) < __builtin_inff()) || !(fabsf(v[c]) < __builtin_inff());
+        k[c] *= p.scale;
+    }
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+        exact_dkv<D>(p, b, hk, j);
+        return;
+    }
+    store_row<D>(p.dk.p + b * p.dk.bs + j * p.dk.ld + hk * p.dk.hs, k);
+    store_row<D>(p.dv.p + b * p.dv.bs + j * p.dv.ld + hk * p.dv.hs, v);
+}
+
 // dQ of 128 rows of one head (4 waves x 32 rows held in registers) over its key tiles, and this workgroup's part of dbias: every
 // wave adds dT of its pairs into a table of its own (LDS float adds of one wave run in program order; pairs behind the table's
 // ends are summed in registers), the four tables are added in wave order.
-template <int D, bool EX>
+template <int D, int MODE>
 __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
     constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     float* const tab = (float*)(smem + 2 * BUF);
@@ -874,14 +967,14 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
     const int hi = lane >> 5, row = qt * 128 + wid * 32 + (lane & 31), rc = min(row, p.Lq - 1);
     const Vis vis = load_vis(p, b, row);
-    const int pos = EX && p.bias ? row_pos(p, b, rc) : 0;
+    const int pos = BIAS ? row_pos(p, b, rc) : 0;
     int* const red = (int*)smem;
     {
         const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
         const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
         if (lane == 0) { red[4 * wid] = amin; red[4 * wid + 1] = amax; red[4 * wid + 2] = bmin; red[4 * wid + 3] = bmax; }
     }
-    if (EX && p.bias) {
+    if (BIAS) {
         load_table(p, h, tab);
         if (p.dbias)
             for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
@@ -911,8 +1004,8 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
             of[ks] = *(const bf16x8_t*)(g + ks * 16);
         }
     }
-    const long long at = ((long long)b * p.H + h) * p.Lq + rc;
-    const float ls = p.lse[at] * LOG2E, de = p.delta[at];
+    const float* const st = p.stat + (((long long)b * p.H + h) * p.nq64 + (rc >> 6)) * 256 + (rc & 63);
+    const float ls = st[0], de = st[64];                            // log-sum-exp (base 2), -delta
     const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
     f32x16_t dq[D / 32];
 #pragma unroll
@@ -941,32 +1034,37 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            f32x16_t s = zero16(), dp = zero16();
+            f32x16_t s = zero16(), dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = de;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
                 s = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s);
                 dp = mfma(row_frag<D>(sv, roff, i, ks), of[ks], dp);
             }
             const int k0 = j0 + 32 * i + 4 * hi;
+            f32x16_t fac;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float z = s[r] * p.zs, fac = 1.f;
-                bool ok = full || sees(vis, k0 + reg_row(r));
-                if (EX && p.cap2 != 0.f) {
-                    const float y = tanh_f(z);
-                    z = p.cap2 * y;
-                    fac = __builtin_fmaf(-y, y, 1.f);
+                if (EX) {
+                    float z = s[r] * p.zs;
+                    if (CAP) {
+                        const float y = tanh_f(z);
+                        z = p.cap2 * y;
+                        fac[r] = __builtin_fmaf(-y, y, 1.f);
+                    }
+                    if (BIAS) z += tab[min(max(k0 + reg_row(r) - pos, -p.R), p.R) + p.R];
+                    const float dt = __builtin_amdgcn_exp2f(z - ls) * dp[r];
+                    s[r] = z != -__builtin_inff() ? dt : 0.f;
+                } else {
+                    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls)) * dp[r];
                 }
-                if (EX && p.bias) {
-                    z += tab[min(max(k0 + reg_row(r) - pos, -p.R), p.R) + p.R];
-                    ok = ok && z != -__builtin_inff();
-                }
-                const float P = __builtin_amdgcn_exp2f(z - ls);
-                const float dt = P * (dp[r] - de);
-                if (EX) s[r] = ok ? dt : 0.f;
-                dp[r] = ok ? dt * fac : 0.f;
             }
-            if (EX && p.bias && p.dbias) {
+            if (!full) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = sees(vis, k0 + reg_row(r)) ? s[r] : 0.f;
+            }
+            if (BIAS && p.dbias) {
                 const int lo = j0 + 32 * i - pmax, hi_ = j0 + 32 * i + 31 - pmin;     // distances of this block, wave-uniform
                 if (hi_ <= -p.R || lo >= p.R) {
                     float a = 0.f;
@@ -984,9 +1082,13 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
                     }
                 }
             }
+            if (CAP) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] *= fac[r];
+            }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const bf16x8_t zf = half_of(dp, g);
+                const bf16x8_t zf = half_of(s, g);
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) dq[c] = mfma(tr_frag<D>(sk, t0, t8, c, 2 * i + g), zf, dq[c]);
             }
@@ -1001,7 +1103,7 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
         redo &= redo - 1;
         exact_dq<D>(p, b, h, qt * 128 + wid * 32 + i);
     }
-    if (EX && p.bias && p.dbias) {
+    if (BIAS && p.dbias) {
         below = wave_add(below);
         above = wave_add(above);
         if (lane == 0) {
@@ -1055,10 +1157,12 @@ const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
     return nullptr;
 }
 
-// the form with 32 (row, head) pairs per workgroup and the keys split: where 128-row workgroups would leave compute units empty
+// the form with 32 (row, head) pairs per workgroup and the keys split: where 128-row workgroups would leave compute units empty, and
+// where one block of 32 pairs holds all rows that share a key head (each key is then read once, not once per query head)
 bool few_rows(const pf_attn_ranges_desc* d) {
-    return (long long)((d->Lq + 127) / 128) * d->H * d->B < 256;
+    return (long long)((d->Lq + 127) / 128) * d->H * d->B < 256 || (long long)d->Lq * (d->H / d->Hkv) <= 32;
 }
+int mode(const pf_attn_ranges_desc* d) { return (d->cap > 0.f ? 1 : 0) + (d->bias ? 2 : 0); }
 int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * (d->H / d->Hkv) + 31) / 32); }
 int splits(const pf_attn_ranges_desc* d) {
     const long long units = (long long)row_blocks(d) * d->Hkv * d->B, tiles = (d->Lk + 31) / 32;
@@ -1072,12 +1176,25 @@ long long fwd_bytes(const pf_attn_ranges_desc* d) {
     return s > 1 ? (long long)row_blocks(d) * d->Hkv * d->B * s * 32 * (d->D + 2) * 4 : 0;
 }
 long long up16(long long n) { return (n + 15) / 16 * 16; }
-struct BwdSizes { long long delta, tiles, parts; };
+// the (head, row tile) list of a key block in parts where the key blocks alone leave compute units empty: four tiles per part at least
+int kv_splits(const pf_attn_ranges_desc* d) {
+    if (!d->B || !d->H || !d->Lk || !d->Lq) return 1;
+    const long long units = (long long)((d->Lk + 127) / 128) * d->Hkv * d->B, tiles = (long long)((d->Lq + 63) / 64) * (d->H / d->Hkv);
+    long long n = 768 / units;
+    if (n > tiles / 4) n = tiles / 4;
+    if (n > 16) n = 16;
+    return (int)(n < 1 ? 1 : n);
+}
+struct BwdSizes { long long stat, vis, tiles, parts, kv; long long all() const { return stat + vis + tiles + parts + kv; } };
 BwdSizes bwd_sizes(const pf_attn_ranges_desc* d) {
     BwdSizes s;
-    s.delta = up16((long long)d->B * d->H * d->Lq * 4);
-    s.tiles = up16((long long)d->B * ((d->Lq + 63) / 64) * 32);
+    const long long nq = (d->Lq + 63) / 64;
+    s.stat = (long long)d->B * d->H * nq * 1024;
+    s.vis = (long long)d->B * nq * 1024;
+    s.tiles = up16((long long)d->B * nq * 32);
     s.parts = d->dbias ? up16((long long)d->B * d->H * ((d->Lq + 127) / 128) * (2 * d->bias_radius + 1) * 4) : 0;
+    const int n = kv_splits(d);
+    s.kv = n > 1 ? (long long)n * d->B * d->Hkv * d->Lk * 2 * d->D * 4 : 0;
     return s;
 }
 
@@ -1093,7 +1210,7 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
     a.cap2 = d->cap * LOG2E;
     a.zs = d->cap > 0.f ? d->scale / d->cap : d->scale * LOG2E;
     a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
-    a.nqt = (d->Lq + 127) / 128; a.nkt = (d->Lk + 127) / 128;
+    a.nqt = (d->Lq + 127) / 128; a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
     return a;
 }
 
@@ -1103,18 +1220,18 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
         if (e_ != hipSuccess) return pf_set_err(hipGetErrorString(e_)); \
     } while (0)
 
-template <int D, bool EX>
+template <int D, int MODE>
 int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
     if (!few) {
-        const size_t lds = 4 * 64 * 2 * D + (EX ? (2 * MAX_RADIUS + 1) * 4 : 0);
-        PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, EX>), (int)lds);
-        range_fwd_kernel<D, EX><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
+        const size_t lds = 4 * 64 * 2 * D + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
+        PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, MODE>), (int)lds);
+        range_fwd_kernel<D, MODE><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
         CHECK_LAUNCH();
         return 0;
     }
     const size_t lds = 4 * 4 * 32 * 2 * D;                           // the meeting area [4][32][D + 4] fp32 is smaller
-    PF_SET_MAX_LDS_ONCE((range_split_kernel<D, EX>), (int)lds);
-    range_split_kernel<D, EX><<<(unsigned)(a.nrb * a.Hk * a.B * a.nsplit), 256, lds, stream>>>(a);
+    PF_SET_MAX_LDS_ONCE((range_split_kernel<D, MODE>), (int)lds);
+    range_split_kernel<D, MODE><<<(unsigned)(a.nrb * a.Hk * a.B * a.nsplit), 256, lds, stream>>>(a);
     CHECK_LAUNCH();
     if (a.nsplit > 1) {
         const long long rows = (long long)a.B * a.Hk * a.Lq * a.G;
@@ -1124,22 +1241,26 @@ int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
     return 0;
 }
 
-template <int D, bool EX>
+template <int D, int MODE>
 int launch_bwd(const RArgs& a, hipStream_t stream) {
     if (a.Lq > 0) {
         range_prep_kernel<D><<<dim3((a.Lq + 63) / 64, a.H, a.B), 256, 0, stream>>>(a);
         CHECK_LAUNCH();
     }
     if (a.Lk > 0) {
-        const size_t lds = 4 * 64 * 2 * D + 256 * 4 + 640 * 4 + (EX ? (2 * MAX_RADIUS + 1) * 4 : 0);
-        PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, EX>), (int)lds);
-        range_dkv_kernel<D, EX><<<(unsigned)(a.nkt * a.Hk * a.B), 256, lds, stream>>>(a);
+        const size_t lds = 2 * (2 * 64 * 2 * D + 2048) + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
+        PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, MODE>), (int)lds);
+        range_dkv_kernel<D, MODE><<<(unsigned)(a.nkt * a.kv_split * a.Hk * a.B), 256, lds, stream>>>(a);
         CHECK_LAUNCH();
+        if (a.kv_split > 1) {
+            range_kvjoin_kernel<D><<<(unsigned)(((long long)a.B * a.Hk * a.Lk + 3) / 4), 256, 0, stream>>>(a);
+            CHECK_LAUNCH();
+        }
     }
     if (a.Lq > 0) {
-        const size_t lds = 4 * 64 * 2 * D + (EX ? 5 * (2 * a.R + 1) * 4 : 0);
-        PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, EX>), 4 * 64 * 2 * D + (EX ? 5 * (2 * MAX_RADIUS + 1) * 4 : 0));
-        range_dq_kernel<D, EX><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
+        const size_t lds = 4 * 64 * 2 * D + (MODE & 2 ? 5 * (2 * a.R + 1) * 4 : 0);
+        PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE>), 4 * 64 * 2 * D + (MODE & 2 ? 5 * (2 * MAX_RADIUS + 1) * 4 : 0));
+        range_dq_kernel<D, MODE><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
         CHECK_LAUNCH();
     }
     return 0;
@@ -1154,11 +1275,11 @@ extern "C" long long pf_attention_ranges_workspace_bytes(const pf_attn_ranges_de
 extern "C" long long pf_attention_ranges_bwd_workspace_bytes(const pf_attn_ranges_desc* d) {
     if (check_ranges(d, true)) return -1;
     const BwdSizes s = bwd_sizes(d);
-    return s.delta + s.tiles + s.parts;
+    return s.all();
 }
 
 extern "C" int pf_attention_ranges_which(const pf_attn_ranges_desc* d) {
-    return check_ranges(d, false) ? -1 : (few_rows(d) ? 2 : 1);
+    return check_ranges(d, false) ? -1 : (d->H == 0 || few_rows(d) ? 2 : 1);
 }
 
 extern "C" int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, hipStream_t stream) {
@@ -1168,37 +1289,55 @@ extern "C" int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, hipStream_
     if (need && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need))
         return pf_set_err("pf_attention_ranges_bf16: workspace missing, unaligned or too small");
     RArgs a = range_args(d);
-    const bool few = few_rows(d), ex = d->bias || d->cap > 0.f;
+    const bool few = few_rows(d);
     const long long grid = few ? (long long)row_blocks(d) * d->Hkv * d->B * splits(d) : (long long)a.nqt * d->H * d->B;
     if (grid > 0x7fffffffLL) return pf_set_err("pf_attention_ranges_bf16: too many workgroups");
     a.nrb = row_blocks(d);
     a.nsplit = few ? splits(d) : 1;
     a.parts = (float*)d->workspace;
-    if (d->D == 64) return ex ? launch_fwd<64, true>(a, few, stream) : launch_fwd<64, false>(a, few, stream);
-    return ex ? launch_fwd<128, true>(a, few, stream) : launch_fwd<128, false>(a, few, stream);
+    switch ((d->D == 64 ? 0 : 4) + mode(d)) {
+        case 0: return launch_fwd<64, 0>(a, few, stream);
+        case 1: return launch_fwd<64, 1>(a, few, stream);
+        case 2: return launch_fwd<64, 2>(a, few, stream);
+        case 3: return launch_fwd<64, 3>(a, few, stream);
+        case 4: return launch_fwd<128, 0>(a, few, stream);
+        case 5: return launch_fwd<128, 1>(a, few, stream);
+        case 6: return launch_fwd<128, 2>(a, few, stream);
+        default: return launch_fwd<128, 3>(a, few, stream);
+    }
 }
 
 extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t stream) {
     if (const char* e = check_ranges(d, true)) return pf_set_err(e);
     const BwdSizes s = bwd_sizes(d);
-    const long long need = s.delta + s.tiles + s.parts;
+    const long long need = s.all();
     if (need && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need))
         return pf_set_err("pf_attention_ranges_bwd: workspace missing, unaligned or too small");
     if (d->B > 65535 || d->H > 65535) return pf_set_err("pf_attention_ranges_bwd: more than 65535 batch entries or heads");
-    if ((long long)((d->Lq + 127) / 128) * d->H * d->B > 0x7fffffffLL || (long long)((d->Lk + 127) / 128) * d->H * d->B > 0x7fffffffLL ||
+    if ((long long)((d->Lq + 127) / 128) * d->H * d->B > 0x7fffffffLL || (long long)((d->Lk + 127) / 128) * d->H * d->B * 16 > 0x7fffffffLL ||
         (long long)(d->Lq + 63) / 64 * (d->H / (d->Hkv ? d->Hkv : 1)) > 0x7fffffffLL)
         return pf_set_err("pf_attention_ranges_bwd: too many workgroups");
     if (!d->H) return 0;
     RArgs a = range_args(d);
-    a.delta = (float*)d->workspace;
-    a.tiles = (int*)((char*)d->workspace + s.delta);
-    a.dbias_parts = (float*)((char*)d->workspace + s.delta + s.tiles);
+    char* w = (char*)d->workspace;
+    a.stat = (float*)w;
+    a.vis = (int*)(w += s.stat);
+    a.tiles = (int*)(w += s.vis);
+    a.dbias_parts = (float*)(w += s.tiles);
+    a.kv_parts = (float*)(w += s.parts);
+    a.kv_split = kv_splits(d);
     a.dbias = d->dbias;
-    const bool ex = d->bias || d->cap > 0.f;
     int rc = 0;
-    if (!d->B) rc = 0;
-    else if (d->D == 64) rc = ex ? launch_bwd<64, true>(a, stream) : launch_bwd<64, false>(a, stream);
-    else rc = ex ? launch_bwd<128, true>(a, stream) : launch_bwd<128, false>(a, stream);
+    if (d->B) switch ((d->D == 64 ? 0 : 4) + mode(d)) {
+        case 0: rc = launch_bwd<64, 0>(a, stream); break;
+        case 1: rc = launch_bwd<64, 1>(a, stream); break;
+        case 2: rc = launch_bwd<64, 2>(a, stream); break;
+        case 3: rc = launch_bwd<64, 3>(a, stream); break;
+        case 4: rc = launch_bwd<128, 0>(a, stream); break;
+        case 5: rc = launch_bwd<128, 1>(a, stream); break;
+        case 6: rc = launch_bwd<128, 2>(a, stream); break;
+        default: rc = launch_bwd<128, 3>(a, stream); break;
+    }
     if (rc == 0 && d->dbias) {
         range_dbias_kernel<<<dim3((2 * a.R + 1 + 63) / 64, a.H), 256, 0, stream>>>(a);
         CHECK_LAUNCH();
