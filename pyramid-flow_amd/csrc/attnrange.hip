@@ -1167,7 +1167,7 @@ int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * 
 int splits(const pf_attn_ranges_desc* d) {
     const long long units = (long long)row_blocks(d) * d->Hkv * d->B, tiles = (d->Lk + 31) / 32;
     long long n = 512 / units;
-    if (n > tiles / 8) n = tiles / 8;                     // two tiles per wave at least
+    if (n > tiles / 32) n = tiles / 32;                   // eight tiles per wave at least: the join is a launch of its own
     return (int)(n < 1 ? 1 : n);
 }
 long long fwd_bytes(const pf_attn_ranges_desc* d) {

@@ -33,37 +33,37 @@ struct HArgs {
 };
 
 // (cos, sin) of the pairs that this lane's 8 channels belong to: adjacent pairs -> 4, halves -> 8 (one per channel, the sine
-// already carrying the sign of the channel's side); pairs behind P are the identity
-template <int D>
+// already carrying the sign of the channel's side).  Lane p computes pair p once (P <= 64), the others fetch it: the 64-bit
+// product and the two series are a third of the kernel's instructions when every lane does its own pairs (131 us instead of
+// 102 us for 2 x 15488 tokens of 60 heads).
 PF_DEVICE void lane_angles(const HArgs& p, int b, int tok, int sub, float* c, float* s) {
-    const float* pos = p.pos + b * p.pos_bs + tok * p.pos_ld;
-    const int n = p.halves ? 8 : 4;
+    const int lane = threadIdx.x & 63;
+    float cs = 1.f, sn = 0.f;
+    if (lane < p.P) {
+        const float pos = p.pos[b * p.pos_bs + tok * p.pos_ld + min(max(p.axis[lane], 0), p.n_axes - 1)];
+        const double turns = (double)pos * p.freq[lane] * 0.15915494309189533577;                  // / 2 pi
+        sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+    }
+    if (p.halves) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        c[i] = 1.f;
-        s[i] = 0.f;
-        if (i >= n) continue;
-        int pr = sub * n + i;
-        float sign = 1.f;
-        if (p.halves) {
-            if (pr >= 2 * p.P) continue;
-            sign = pr < p.P ? -1.f : 1.f;
-            pr = pr < p.P ? pr : pr - p.P;
-        } else if (pr >= p.P) {
-            continue;
+        for (int i = 0; i < 8; ++i) {
+            const int ch = sub * 8 + i, pr = ch < p.P ? ch : min(ch - p.P, 63);
+            c[i] = __shfl(cs, pr);
+            s[i] = __shfl(sn, pr);
+            s[i] = ch < p.P ? -s[i] : s[i];
         }
-        const double turns = (double)pos[min(max(p.axis[pr], 0), p.n_axes - 1)] * p.freq[pr] * 0.15915494309189533577;      // / 2 pi
-        const float f = (float)(turns - rint(turns));
-        float sn, cs;
-        sincospif(2.f * f, &sn, &cs);
-        c[i] = cs;
-        s[i] = sign * sn;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int pr = min(sub * 4 + i, 63);
+            c[i] = __shfl(cs, pr);
+            s[i] = __shfl(sn, pr);
+        }
     }
 }
 
 // v <- R(+-theta) v on the lane's 8 channels (dir = -1: the inverse rotation).  halves: the partner channel of (lane, e) sits
 // at the same e of the lane P / 8 further on (channels < P) or back
-template <int D>
 PF_DEVICE void rotate8(const HArgs& p, float* v, const float* c, const float* s, int sub, float dir) {
     if (p.halves) {
         const int shift = p.P >> 3;
@@ -92,53 +92,68 @@ PF_DEVICE float unit_sum(float x) {
     return x;
 }
 
+// Wave-iterations of a token: the query heads in groups of UPW units, then the key heads (a wave-iteration is all queries or
+// all keys, so gains and strides are wave-uniform).
+struct Unit { bool isq, on; long long h; };
+template <int UPW>
+PF_DEVICE Unit unit_of(const HArgs& p, int it, int slot) {
+    const int iq = (p.H + UPW - 1) / UPW;
+    const bool isq = it < iq;
+    const int h = (isq ? it : it - iq) * UPW + slot;
+    return {isq, h < (isq ? p.H : p.Hk), h};
+}
+PF_DEVICE u32x4_t load_unit(const View& v, const Unit& u, int b, int tok, int sub) {
+    u32x4_t r = {0u, 0u, 0u, 0u};
+    if (u.on) r = *(const u32x4_t*)(v.p + b * v.bs + tok * v.ld + u.h * v.hs + sub * 8);
+    return r;
+}
+
 template <int D>
 __global__ __launch_bounds__(256) void heads_fwd_kernel(const HArgs p) {
     constexpr int LPU = D / 8, UPW = 64 / LPU;
     const int lane = threadIdx.x & 63, sub = lane % LPU;
-    const long long wave = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long wave = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long tokb = wave / p.chunks;
     if (tokb >= (long long)p.B * p.L) return;
     const int chunk = (int)(wave - tokb * p.chunks);
     const int b = (int)(tokb / p.L), tok = (int)(tokb - (long long)b * p.L);
+    const int its = (p.H + UPW - 1) / UPW + (p.Hk + UPW - 1) / UPW;
+    int it = chunk * p.per_chunk;
+    const int end = min(its, it + p.per_chunk);
+    Unit u = unit_of<UPW>(p, it, lane / LPU);
+    u32x4_t raw = load_unit(u.isq ? p.q : p.k, u, b, tok, sub);         // in flight while the angles are computed
     float c[8], s[8], wq[8], wk[8];
-    lane_angles<D>(p, b, tok, sub, c, s);
-    if (p.wq) {
+    lane_angles(p, b, tok, sub, c, s);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) wq[e] = p.wq[sub * 8 + e];
+    for (int e = 0; e < 8; ++e) {
+        wq[e] = (p.wq ? p.wq[sub * 8 + e] : 1.f) * p.q_scale;
+        wk[e] = p.wk ? p.wk[sub * 8 + e] : 1.f;
     }
-    if (p.wk) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) wk[e] = p.wk[sub * 8 + e];
-    }
-    const int total = p.H + p.Hk;
-    const int u0 = chunk * p.per_chunk * UPW, u1 = min(total, u0 + p.per_chunk * UPW);
-    for (int u = u0; u < u1; u += UPW) {
-        const int h = u + lane / LPU;
-        const bool on = h < u1, isq = h < p.H;
-        const View& in = isq ? p.q : p.k;
-        const View& out = isq ? p.qo : p.ko;
-        const int hh = isq ? h : h - p.H;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (on) unpack8(*(const u32x4_t*)(in.p + b * in.bs + tok * in.ld + hh * in.hs + sub * 8), v);
-        const bool norm = isq ? p.wq != nullptr : p.wk != nullptr;
-        if (p.wq || p.wk) {                                     // uniform: the reduction runs on all lanes
+    while (it < end) {
+        const Unit cur = u;
+        float v[8];
+        unpack8(raw, v);
+        if (++it < end) {
+            u = unit_of<UPW>(p, it, lane / LPU);
+            raw = load_unit(u.isq ? p.q : p.k, u, b, tok, sub);
+        }
+        float r = 1.f;
+        if (cur.isq ? p.wq != nullptr : p.wk != nullptr) {
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
-            const float r = rsqrtf(__builtin_fmaf(unit_sum<LPU>(ss), 1.f / D, p.eps));
-            if (norm) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = v[e] * r * (isq ? wq[e] : wk[e]);
-            }
+            r = rsqrtf(__builtin_fmaf(unit_sum<LPU>(ss), 1.f / D, p.eps));
         }
-        rotate8<D>(p, v, c, s, sub, 1.f);
-        if (on) {
-            const float f = isq ? p.q_scale : 1.f;
+        if (cur.isq) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= f;
-            *(u32x4_t*)(out.p + b * out.bs + tok * out.ld + hh * out.hs + sub * 8) = pack8(v);
+            for (int e = 0; e < 8; ++e) v[e] *= r * wq[e];
+        } else if (p.wk) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= r * wk[e];
         }
+        rotate8(p, v, c, s, sub, 1.f);
+        const View& out = cur.isq ? p.qo : p.ko;
+        if (cur.on) *(u32x4_t*)(out.p + b * out.bs + tok * out.ld + cur.h * out.hs + sub * 8) = pack8(v);
     }
 }
 
@@ -148,7 +163,7 @@ template <int D>
 __global__ __launch_bounds__(256) void heads_bwd_kernel(const HArgs p) {
     constexpr int LPU = D / 8, UPW = 64 / LPU;
     __shared__ float red[4][2][D];
-    const int lane = threadIdx.x & 63, sub = lane % LPU, wid = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, sub = lane % LPU, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float wq[8], wk[8], aq[8], ak[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -156,53 +171,59 @@ __global__ __launch_bounds__(256) void heads_bwd_kernel(const HArgs p) {
         wk[e] = p.wk ? p.wk[sub * 8 + e] : 1.f;
         aq[e] = ak[e] = 0.f;
     }
-    const int total = p.H + p.Hk;
+    const int its = (p.H + UPW - 1) / UPW + (p.Hk + UPW - 1) / UPW;
     const long long waves = (long long)p.B * p.L * p.chunks;
     for (long long wave = (long long)blockIdx.x * 4 + wid; wave < waves; wave += (long long)gridDim.x * 4) {
         const long long tokb = wave / p.chunks;
         const int chunk = (int)(wave - tokb * p.chunks);
         const int b = (int)(tokb / p.L), tok = (int)(tokb - (long long)b * p.L);
+        int it = chunk * p.per_chunk;
+        const int end = min(its, it + p.per_chunk);
+        Unit u = unit_of<UPW>(p, it, lane / LPU);
+        auto norm_of = [&](const Unit& n) { return n.isq ? p.wq != nullptr : p.wk != nullptr; };
+        u32x4_t rg = load_unit(u.isq ? p.dq : p.dk, u, b, tok, sub), rx = {0u, 0u, 0u, 0u};
+        if (norm_of(u)) rx = load_unit(u.isq ? p.q : p.k, u, b, tok, sub);
         float c[8], s[8];
-        lane_angles<D>(p, b, tok, sub, c, s);
-        const int u0 = chunk * p.per_chunk * UPW, u1 = min(total, u0 + p.per_chunk * UPW);
-        for (int u = u0; u < u1; u += UPW) {
-            const int h = u + lane / LPU;
-            const bool on = h < u1, isq = h < p.H;
-            const View& in = isq ? p.q : p.k;
-            const View& dy = isq ? p.dq : p.dk;
-            const View& out = isq ? p.qo : p.ko;
-            const int hh = isq ? h : h - p.H;
-            const bool norm = isq ? p.wq != nullptr : p.wk != nullptr;
-            float g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (on) {
-                unpack8(*(const u32x4_t*)(dy.p + b * dy.bs + tok * dy.ld + hh * dy.hs + sub * 8), g);
-                if (norm) unpack8(*(const u32x4_t*)(in.p + b * in.bs + tok * in.ld + hh * in.hs + sub * 8), x);
-                const float f = isq ? p.q_scale : 1.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= f;
+        lane_angles(p, b, tok, sub, c, s);
+        while (it < end) {
+            const Unit cur = u;
+            float g[8], x[8];
+            unpack8(rg, g);
+            unpack8(rx, x);
+            if (++it < end) {
+                u = unit_of<UPW>(p, it, lane / LPU);
+                rg = load_unit(u.isq ? p.dq : p.dk, u, b, tok, sub);
+                if (norm_of(u)) rx = load_unit(u.isq ? p.q : p.k, u, b, tok, sub);
             }
-            rotate8<D>(p, g, c, s, sub, -1.f);
-            if (p.wq || p.wk) {
-                float ss = 0.f, st = 0.f, w[8];
+            if (cur.isq) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] *= p.q_scale;
+            }
+            rotate8(p, g, c, s, sub, -1.f);
+            if (norm_of(cur)) {
+                float ss = 0.f, st = 0.f, wg[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    w[e] = isq ? wq[e] : wk[e];
+                    wg[e] = (cur.isq ? wq[e] : wk[e]) * g[e];
                     ss = __builtin_fmaf(x[e], x[e], ss);
-                    st = __builtin_fmaf(w[e] * g[e], x[e], st);
+                    st = __builtin_fmaf(wg[e], x[e], st);
                 }
                 const float r = rsqrtf(__builtin_fmaf(unit_sum<LPU>(ss), 1.f / D, p.eps));
                 const float k = unit_sum<LPU>(st) * (1.f / D) * r * r * r;
-                if (on && norm) {
+                if (cur.on) {                                          // a row of zeros and eps 0 would leave 0 x inf
+                    if (cur.isq) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float gx = g[e] * x[e] * r;
-                        aq[e] += isq ? gx : 0.f;
-                        ak[e] += isq ? 0.f : gx;
-                        g[e] = __builtin_fmaf(r, w[e] * g[e], -(x[e] * k));
+                        for (int e = 0; e < 8; ++e) aq[e] = __builtin_fmaf(g[e], x[e] * r, aq[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) ak[e] = __builtin_fmaf(g[e], x[e] * r, ak[e]);
                     }
                 }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] = __builtin_fmaf(r, wg[e], -(x[e] * k));
             }
-            if (on) *(u32x4_t*)(out.p + b * out.bs + tok * out.ld + hh * out.hs + sub * 8) = pack8(g);
+            const View& out = cur.isq ? p.qo : p.ko;
+            if (cur.on) *(u32x4_t*)(out.p + b * out.bs + tok * out.ld + cur.h * out.hs + sub * 8) = pack8(g);
         }
     }
     if (!p.parts) return;                                       // uniform over the launch
@@ -225,18 +246,20 @@ __global__ __launch_bounds__(256) void heads_bwd_kernel(const HArgs p) {
     }
 }
 
-// dw[i] = sum over workgroups of parts[wg][i], i < 2 D (queries, then keys): 32 columns per workgroup, 8 row groups
-__global__ __launch_bounds__(256) void heads_dw_kernel(const float* parts, float* dwq, float* dwk, int nwg, int D) {
-    __shared__ float red[8][32];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), grp = threadIdx.x >> 5;
+// dw[i] = sum over workgroups of parts[wg][i], i < 2 D (queries, then keys): 32 columns per workgroup, 32 row groups (with 8 of
+// them the launch took 32 us of loads in a row, more than half of the gradient kernel itself)
+__global__ __launch_bounds__(1024) void heads_dw_kernel(const float* parts, float* dwq, float* dwk, int nwg, int D) {
+    __shared__ float red[32][33];
+    const int x = threadIdx.x & 31, grp = threadIdx.x >> 5, col = blockIdx.x * 32 + x;
     float a = 0.f;
-    for (int w = grp; w < nwg; w += 8) a += parts[(long long)w * 2 * D + col];
-    red[grp][threadIdx.x & 31] = a;
+#pragma unroll 8
+    for (int w = grp; w < nwg; w += 32) a += parts[(long long)w * 2 * D + col];
+    red[grp][x] = a;
     __syncthreads();
     if (grp == 0) {
         float t = 0.f;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) t += red[g][threadIdx.x];
+        for (int g = 0; g < 32; ++g) t += red[g][x];
         if (col < D) {
             if (dwq) dwq[col] = t;
         } else if (dwk) {
@@ -252,7 +275,7 @@ int bwd_grid(long long waves) { return (int)((waves + 3) / 4 < BWD_GRID ? (waves
 // wave-iterations of one token over `chunks` waves: one wave per token amortises the angles over all of its heads; with few
 // tokens every iteration gets a wave of its own (the call is latency then, not bandwidth)
 void split_heads(const pf_heads_desc* d, int* chunks, int* per_chunk) {
-    const int upw = 64 / (d->D / 8), its = (d->H + d->Hkv + upw - 1) / upw;
+    const int upw = 64 / (d->D / 8), its = (d->H + upw - 1) / upw + (d->Hkv + upw - 1) / upw;
     *per_chunk = (long long)d->B * d->L * its <= 8192 ? 1 : its;
     *chunks = (its + *per_chunk - 1) / *per_chunk;
 }
@@ -338,7 +361,7 @@ extern "C" int pf_qk_norm_rope_axes_bwd(const pf_heads_desc* d, float* dwq, floa
         CHECK_LAUNCH();
     }
     if (gains) {                                                // no tokens: the sums are zero
-        heads_dw_kernel<<<2 * d->D / 32, 256, 0, stream>>>((const float*)workspace, dwq, dwk, grid, d->D);
+        heads_dw_kernel<<<2 * d->D / 32, 1024, 0, stream>>>((const float*)workspace, dwq, dwk, grid, d->D);
         CHECK_LAUNCH();
     }
     return 0;

@@ -147,9 +147,15 @@ def load():
     lib.pf_cmdlist_create.restype = C.c_void_p
     lib.pf_attention_workspace_bytes.restype = C.c_longlong
     lib.pf_gemm_workspace_bytes.restype = C.c_longlong
+    # declared argument types: the single-token calls of these are a few microseconds of GPU time, and building ctypes objects per
+    # argument would cost as much again on the host
     for name in ("pf_qk_norm_rope_axes_bwd_workspace_bytes", "pf_attention_ranges_workspace_bytes",
                  "pf_attention_ranges_bwd_workspace_bytes"):
         getattr(lib, name).restype = C.c_longlong
+        getattr(lib, name).argtypes = [C.c_void_p]
+    for name in ("pf_qk_norm_rope_axes", "pf_attention_ranges_bf16", "pf_attention_ranges_bwd"):
+        getattr(lib, name).argtypes = [C.c_void_p, C.c_void_p]
+    lib.pf_qk_norm_rope_axes_bwd.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p]
     if lib.pf_version() != ABI_VERSION:
         raise RuntimeError(f"pyflow_hip: {LIB_PATH} has ABI version {lib.pf_version()}, this host expects {ABI_VERSION}: rebuild it")
     for which, cls in enumerate((GemmDesc, ConvDesc, AttnDesc, AttnSmallDesc, HeadsDesc, AttnRangesDesc)):       # struct mirrors vs the compiled layout
@@ -167,6 +173,11 @@ def check(rc):
 
 def stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def raw_stream():
+    """the current stream of the current device as an integer (no Stream object is built)"""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def ptr(t):

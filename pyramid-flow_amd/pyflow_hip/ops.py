@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import lib as L
-from .lib import (GemmDesc, AttnDesc, AttnSmallDesc, ConvDesc, HeadsDesc, AttnRangesDesc, check, ptr, stream, GEMM_GATE_RES,  # noqa: F401
+from .lib import (GemmDesc, AttnDesc, AttnSmallDesc, ConvDesc, HeadsDesc, AttnRangesDesc, check, ptr, stream, raw_stream, GEMM_GATE_RES,  # noqa: F401
                   GEMM_OUT_F32, GEMM_ACT_QUICK_GELU, GEMM_ACT_GELU_ERF)
 
 
@@ -316,26 +316,26 @@ def attention_small(qkv, O, q_off, k_off, v_off, ld, ldo, B, H, Lseq, scale, bia
 # ---------------------------------------------------------------------------------------------- attention over key ranges
 def _rows(view, t, shape, what, out=False):
     """fills a pf_rows_view from a bf16 [B, L, H, D] tensor (any strides that are multiples of 8, channels dense)"""
-    if t.dtype != torch.bfloat16 or t.shape != shape:
+    if t.dtype is not torch.bfloat16 or t.shape != shape:
         raise ValueError(f"{what}: expected bfloat16 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if not t.numel():
-        return
     sb, sr, sh, sc = t.stride()
-    nb, nr, nh, _ = shape
-    if sc != 1:
-        raise ValueError(f"{what}: the channels of a head must be dense")
-    # the stride of a dimension of one entry says nothing
-    sb, sr, sh = sb if nb > 1 else 0, sr if nr > 1 else 0, sh if nh > 1 else 0
     p = t.data_ptr()
-    if (sb | sr | sh) % 8 or p % 16:
-        raise ValueError(f"{what}: data must be 16-byte aligned and strides multiples of 8 elements")
-    if out and ((nb > 1 and not sb) or (nr > 1 and not sr) or (nh > 1 and not sh)):
-        raise ValueError(f"{what}: an expanded tensor cannot be written")
+    if sc != 1 or (sb | sr | sh) & 7 or p & 15 or (out and not (sb and sr and sh)):
+        if not t.numel():
+            return
+        if sc != 1:
+            raise ValueError(f"{what}: the channels of a head must be dense")
+        # the stride of a dimension of one entry says nothing
+        sb, sr, sh = (s if n > 1 else 0 for s, n in zip((sb, sr, sh), shape))
+        if (sb | sr | sh) & 7 or p & 15:
+            raise ValueError(f"{what}: data must be 16-byte aligned and strides multiples of 8 elements")
+        if out and any(n > 1 and not s for s, n in zip((sb, sr, sh), shape)):
+            raise ValueError(f"{what}: an expanded tensor cannot be written")
     view.p, view.batch, view.row, view.head = p, sb, sr, sh
 
 
 def _f32(t, shape, what):
-    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous float32 tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -346,7 +346,7 @@ def _one_device(what, *tensors):
         raise RuntimeError(f"{what}: not available while a launch list is being recorded")
     dev = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"{what}: a tensor is on {t.device}, the current device is cuda:{dev}")
 
 
@@ -402,7 +402,7 @@ def qk_norm_rope_axes(q, k, q_out, k_out, wq, wk, rope, pos, eps=1e-6, q_scale=1
     positions `pos` (fp32 [B or 1, L, axes]; fractions allowed), q times q_scale.  q [B, L, H, D], k [B, L, Hkv, D] bf16 views
     (column blocks of a projection are fine), D 64 or 128; either pair may be None; an output may be its input."""
     d = _heads_desc("qk_norm_rope_axes", q, k, q_out, k_out, wq, wk, rope, pos, eps, q_scale)
-    check(L.load().pf_qk_norm_rope_axes(C.byref(d), stream()))
+    check(L.load().pf_qk_norm_rope_axes(C.byref(d), raw_stream()))
 
 
 def qk_norm_rope_axes_backward(dq, dk, q, k, wq, wk, rope, pos, dq_in, dk_in, dwq=None, dwk=None, eps=1e-6, q_scale=1.0,
@@ -423,11 +423,11 @@ def qk_norm_rope_axes_backward(dq, dk, q, k, wq, wk, rope, pos, dq_in, dk_in, dw
     pwk = _f32(dwk, (d.D,), what) if dwk is not None else 0
     if (pwq and not d.wq) or (pwk and not d.wk):
         raise ValueError(f"{what}: a gain gradient without its gains")
-    ws = nbytes = None
+    ws, nbytes = None, 0
     if pwq or pwk:
         ws = _scratch(what, lib.pf_qk_norm_rope_axes_bwd_workspace_bytes(C.byref(d)), workspace, (q if q is not None else k).device)
         nbytes = ws.numel() * ws.element_size() if ws is not None else 0
-    check(lib.pf_qk_norm_rope_axes_bwd(C.byref(d), C.c_void_p(pwq), C.c_void_p(pwk), ptr(ws), C.c_longlong(nbytes or 0), stream()))
+    check(lib.pf_qk_norm_rope_axes_bwd(C.byref(d), pwq, pwk, ws.data_ptr() if ws is not None else 0, nbytes, raw_stream()))
 
 
 def _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap):
@@ -482,7 +482,7 @@ def attention_ranges(q, k, v, out, ranges=None, scale=None, bias=None, q_pos=Non
         _one_device(what, workspace)
         ws = _scratch(what, need, workspace, q.device)
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    PROFILER.launch("attention_ranges", 0.0, lambda: check(lib.pf_attention_ranges_bf16(C.byref(d), stream())))
+    PROFILER.launch("attention_ranges", 0.0, lambda: check(lib.pf_attention_ranges_bf16(C.byref(d), raw_stream())))
 
 
 def attention_ranges_backward(dout, q, k, v, out, lse, dq, dk, dv, ranges=None, scale=None, bias=None, q_pos=None, cap=0.0,
@@ -504,8 +504,8 @@ def attention_ranges_backward(dout, q, k, v, out, lse, dq, dk, dv, ranges=None, 
         d.dbias = _f32(dbias, bias.shape, what)
     need = lib.pf_attention_ranges_bwd_workspace_bytes(C.byref(d))
     if need < 0:
-        check(lib.pf_attention_ranges_bwd(C.byref(d), stream()))      # names the argument
+        check(lib.pf_attention_ranges_bwd(C.byref(d), raw_stream()))      # names the argument
     ws = _scratch(what, need, workspace, q.device)
     if ws is not None:
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    PROFILER.launch("attention_ranges_bwd", 0.0, lambda: check(lib.pf_attention_ranges_bwd(C.byref(d), stream())))
+    PROFILER.launch("attention_ranges_bwd", 0.0, lambda: check(lib.pf_attention_ranges_bwd(C.byref(d), raw_stream())))

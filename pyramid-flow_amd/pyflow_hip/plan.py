@@ -112,9 +112,9 @@ class RopeAxes:
     (2 p, 2 p + 1), or (p, p + n_pairs) with ``halves``; channels behind 2 n_pairs pass through."""
 
     def __init__(self, freq, axis, halves=False):
-        if freq.dtype != torch.float64 or axis.dtype != torch.int32 or freq.dim() != 1 or freq.shape != axis.shape:
+        if freq.dtype is not torch.float64 or axis.dtype is not torch.int32 or freq.dim() != 1 or freq.shape != axis.shape:
             raise ValueError("RopeAxes: freq must be float64 [n_pairs] and axis int32 [n_pairs]")
-        if not (freq.is_contiguous() and axis.is_contiguous()) or freq.device != axis.device:
+        if not (freq.is_contiguous() and axis.is_contiguous()) or freq.get_device() != axis.get_device():
             raise ValueError("RopeAxes: freq and axis must be contiguous and on one device")
         self.freq, self.axis, self.halves, self.n_pairs = freq, axis, bool(halves), freq.numel()
 
@@ -135,10 +135,9 @@ class KeyRanges:
     def __init__(self, a_lo, a_hi, b_lo=None, b_hi=None):
         if (b_lo is None) != (b_hi is None):
             raise ValueError("KeyRanges: a second range needs its start and its end")
-        for t in (a_lo, a_hi, b_lo, b_hi):
-            if t is None:
-                continue
-            if t.dtype != torch.int32 or t.dim() != 2 or t.shape != a_lo.shape or t.device != a_lo.device or not t.is_contiguous():
+        shape, device = a_lo.shape, a_lo.get_device()
+        for t in (a_lo, a_hi) if b_lo is None else (a_lo, a_hi, b_lo, b_hi):
+            if t.dtype is not torch.int32 or t.shape != shape or len(shape) != 2 or t.get_device() != device or not t.is_contiguous():
                 raise ValueError("KeyRanges: ranges must be contiguous int32 [B or 1][Lq] tensors of one shape on one device")
         self.a_lo, self.a_hi, self.b_lo, self.b_hi = a_lo, a_hi, b_lo, b_hi
 
