@@ -38,7 +38,8 @@ struct RArgs {
     const int* a_lo; const int* a_hi; const int* b_lo; const int* b_hi; long long range_bs;
     const int* q_pos; long long pos_bs;
     const float* bias; int R;
-    float zs, cap2, scale;             // z zs = base-2 score (uncapped) or the tanh's argument; cap log2 e, 0 = uncapped
+    float zs, cap2, scale;             // z zs = base-2 score (uncapped), tanh's argument (series) or 2 log2 e times it; cap log2 e, 0 = uncapped
+    int series;
     int B, H, Hk, G, Lq, Lk;
     int nqt, nkt, nrb, nsplit;
     float* parts;                      // split forward: [unit][split][32][D + 2]
@@ -192,23 +193,34 @@ PF_DEVICE float other_half(float x) {
 }
 
 // ---------------------------------------------------------------------------------------------- scores
-// odd series below 0.3 (next term 0.0089 x^10: 5e-8), else 1 - 2 / (1 + e^2x): no cancellation of the 1 where x is small
+// cap tanh(z / cap) in base 2 from the raw product.  1 - 2 / (1 + e^2x) leaves 2^-23 of the CAP in the score, nothing for caps up
+// to 64 (8e-6); SERIES (larger caps) takes the odd series below |x| = 0.3 (next term 0.0089 x^10: 5e-8), where a score is a small
+// part of its cap.  The series in every call cost 19 us of 165 at 16 heads of 128 channels and 8000 packed rows.  slope = 1 - tanh^2.
 PF_DEVICE float tanh_f(float x) {
     const float y = x * x;
     const float near = x * __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
     const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x));
     return fabsf(x) < 0.3f ? near : far;
 }
+template <bool SERIES>
+PF_DEVICE float capped(const RArgs& p, float z, float& slope) {
+    if constexpr (SERIES) {
+        const float y = tanh_f(z * p.zs);
+        slope = __builtin_fmaf(-y, y, 1.f);
+        return p.cap2 * y;
+    } else {
+        const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * p.zs));
+        slope = 4.f * __builtin_fmaf(-r, r, r);
+        return __builtin_fmaf(-2.f * p.cap2, r, p.cap2);
+    }
+}
 PF_DEVICE float bias2(float b) { return b <= HIDDEN ? -__builtin_inff() : b * LOG2E; }
 
-// base-2 score of one pair from global memory (exact_* and nothing else); th = the capped score's tanh
-PF_DEVICE float score2(const RArgs& p, float z, int h, int dist, float& th) {
+// base-2 score of one pair from global memory (exact_* and nothing else)
+PF_DEVICE float score2(const RArgs& p, float z, int h, int dist, float& slope) {
     float t = z * p.zs;
-    th = 0.f;
-    if (p.cap2 != 0.f) {
-        th = tanh_f(t);
-        t = p.cap2 * th;
-    }
+    slope = 1.f;
+    if (p.cap2 != 0.f) t = p.series ? capped<true>(p, z, slope) : capped<false>(p, z, slope);
     if (p.bias) t += bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(dist, -p.R), p.R) + p.R]);
     return t;
 }
@@ -262,9 +274,9 @@ PF_DEVICE void exact_o(const RArgs& p, int b, int h, int i, float m, float l) {
         const int j = j0 + lane;
         bool use = j < p.Lk && sees(v, j);
         if (__builtin_amdgcn_ballot_w64(use) == 0) continue;
-        float w = 0.f, th;
+        float w = 0.f, slope;
         if (use) {
-            const float t = score2(p, dot_row<D>(q, K + j * p.k.ld), h, j - pos, th);
+            const float t = score2(p, dot_row<D>(q, K + j * p.k.ld), h, j - pos, slope);
             use = t != -__builtin_inff();
             w = __builtin_amdgcn_exp2f(t - m) / l;
         }
@@ -276,14 +288,14 @@ PF_DEVICE void exact_o(const RArgs& p, int b, int h, int i, float m, float l) {
 // P and dZ of one visible pair, from global memory
 template <int D>
 PF_DEVICE bool exact_pair(const RArgs& p, int b, int h, int hk, int i, int j, float& P, float& dz) {
-    float th;
+    float slope;
     const float z = dot_row<D>(p.q.p + b * p.q.bs + i * p.q.ld + h * p.q.hs, p.k.p + b * p.k.bs + j * p.k.ld + hk * p.k.hs);
-    const float t = score2(p, z, h, j - row_pos(p, b, i), th);
+    const float t = score2(p, z, h, j - row_pos(p, b, i), slope);
     if (t == -__builtin_inff()) return false;
     const float* st = p.stat + (((long long)b * p.H + h) * p.nq64 + (i >> 6)) * 256 + (i & 63);
     P = __builtin_amdgcn_exp2f(t - st[0]);
     const float dp = dot_row<D>(p.dO.p + b * p.dO.bs + i * p.dO.ld + h * p.dO.hs, p.v.p + b * p.v.bs + j * p.v.ld + hk * p.v.hs);
-    dz = P * (dp + st[64]) * (1.f - th * th);
+    dz = P * (dp + st[64]) * slope;
     return true;
 }
 template <int D>
@@ -354,16 +366,17 @@ template <int MODE>
 PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        float t = s[r] * p.zs;
-        if (MODE & 1) t = p.cap2 * tanh_f(t);
+        float slope, t;
+        if (MODE & 1) t = capped<(MODE & 4) != 0>(p, s[r], slope);
+        else t = s[r] * p.zs;
         if (MODE & 2) t += tab[min(max(rel0 + reg_row(r), -p.R), p.R) + p.R];
         s[r] = t;
     }
 }
 
 // ---------------------------------------------------------------------------------------------- forward, many rows
-// One workgroup = 128 rows of one head, 4 waves x 32; key tiles of 64, two in flight.  MODE: 1 cap, 2 bias, 3 both (scores are
-// formed in base 2 before the maximum), 0 neither (scores stay raw, the exponent's multiply-add scales them).
+// One workgroup = 128 rows of one head, 4 waves x 32; key tiles of 64, two in flight.  MODE bits: 1 cap, 2 bias (scores are
+// formed in base 2 before the maximum; neither: they stay raw and the exponent's multiply-add scales them), 4 SERIES.
 template <int D, int MODE>
 __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
@@ -567,8 +580,9 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
         const int k0 = j0 + 4 * hi;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            float t = s[r] * p.zs;
-            if (CAP) t = p.cap2 * tanh_f(t);
+            float slope, t;
+            if (CAP) t = capped<(MODE & 4) != 0>(p, s[r], slope);
+            else t = s[r] * p.zs;
             if (BIAS) t += bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]);
             s[r] = sees(vis, k0 + reg_row(r)) ? t : -__builtin_inff();
         }
@@ -845,12 +859,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void range_dkv_kernel(const R
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = 4 * q4 + e;
-                            float z = s[r] * p.zs, fac = 1.f;
-                            if (CAP) {
-                                const float y = tanh_f(z);
-                                z = p.cap2 * y;
-                                fac = __builtin_fmaf(-y, y, 1.f);
-                            }
+                            float z, fac = 1.f;
+                            if (CAP) z = capped<(MODE & 4) != 0>(p, s[r], fac);
+                            else z = s[r] * p.zs;
                             if (BIAS) z += tab[min(max(key - (int)pos[e], -p.R), p.R) + p.R];
                             const bool ok = z != -__builtin_inff();
                             const float P = __builtin_amdgcn_exp2f(z - ls[e]);
@@ -950,9 +961,44 @@ __global__ __launch_bounds__(256) void range_kvjoin_kernel(const RArgs p) {
     store_row<D>(p.dv.p + b * p.dv.bs + j * p.dv.ld + hk * p.dv.hs, v);
 }
 
+// Adds the 32 x 32 block dT (lane: row lane % 32, keys in registers) to the wave's table of distances.  Rows that follow one another
+// make every distance a diagonal: 16 rows at a time go to LDS with 32 columns of zeros between them, and lane l sums diagonal
+// l - 15 without a test.  d0 = distance of key 0 of the block from row 0.  (One LDS float add per pair instead: about 200 cycles per
+// instruction, 57 us for the query gradients of 2 x 12 heads x 301 rows instead of 30.)
+constexpr int SKEW = 16 * 64 + 64;                          // floats per wave
+PF_DEVICE void add_diagonals(const f32x16_t& dt, float* skew, float* hist, int R, int d0, float& below, float& above) {
+    const int lane = threadIdx.x & 63, hi = lane >> 5, r = lane & 15;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        if (((lane >> 4) & 1) == half) {
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                f32x4_t w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = dt[4 * q4 + e];
+                *(f32x4_t*)(skew + 32 + 64 * r + 8 * q4 + 4 * hi) = w;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (lane < 47) {
+            float a = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) a += skew[32 + 65 * i + lane - 15];
+            const int d = d0 - 16 * half + lane - 15;
+            if (d <= -R) below += a;
+            else if (d >= R) above += a;
+            else hist[d + R] += a;
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
 // dQ of 128 rows of one head (4 waves x 32 rows held in registers) over its key tiles, and this workgroup's part of dbias: every
-// wave adds dT of its pairs into a table of its own (LDS float adds of one wave run in program order; pairs behind the table's
-// ends are summed in registers), the four tables are added in wave order.
+// wave adds dT of its pairs into a table of its own (by diagonals, or pair by pair where positions are not consecutive: LDS adds
+// of one wave run in program order; pairs behind the table's ends are summed in registers), the four tables are added in wave
+// order.
 template <int D, int MODE>
 __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
@@ -962,6 +1008,7 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     const int NB = 2 * p.R + 1;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* const hist = tab + NB + wid * NB;
+    float* const skew = tab + (5 * NB + 3) / 4 * 4 + wid * SKEW;
     const int t = xcd_remap(blockIdx.x, p.nqt * p.H * p.B);
     const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
@@ -976,8 +1023,10 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     }
     if (BIAS) {
         load_table(p, h, tab);
-        if (p.dbias)
+        if (p.dbias) {
             for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
+            for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
+        }
     }
     __syncthreads();
     TileList tl;
@@ -1012,6 +1061,8 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     for (int c = 0; c < D / 32; ++c) dq[c] = zero16();
     float below = 0.f, above = 0.f;                 // dbias of distances <= -R and >= R
     const int pmin = wave_min(row < p.Lq ? pos : 0x7fffffff), pmax = wave_max(row < p.Lq ? pos : -0x7fffffff);
+    const int pos0 = __builtin_amdgcn_readfirstlane(pos);
+    const bool in_line = __builtin_amdgcn_ballot_w64(row < p.Lq && pos != pos0 + (lane & 31)) == 0;
     bool whole = true;
     drain_barrier();
     auto issue = [&](int n) {
@@ -1047,11 +1098,12 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 if (EX) {
-                    float z = s[r] * p.zs;
+                    float z, slope;
                     if (CAP) {
-                        const float y = tanh_f(z);
-                        z = p.cap2 * y;
-                        fac[r] = __builtin_fmaf(-y, y, 1.f);
+                        z = capped<(MODE & 4) != 0>(p, s[r], slope);
+                        fac[r] = slope;
+                    } else {
+                        z = s[r] * p.zs;
                     }
                     if (BIAS) z += tab[min(max(k0 + reg_row(r) - pos, -p.R), p.R) + p.R];
                     const float dt = __builtin_amdgcn_exp2f(z - ls) * dp[r];
@@ -1072,6 +1124,8 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
                     for (int r = 0; r < 16; ++r) a += s[r];
                     if (lo >= p.R) above += a;
                     else below += a;
+                } else if (in_line) {
+                    add_diagonals(s, skew, hist, p.R, j0 + 32 * i - pos0, below, above);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
@@ -1162,7 +1216,7 @@ const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
 bool few_rows(const pf_attn_ranges_desc* d) {
     return (long long)((d->Lq + 127) / 128) * d->H * d->B < 256 || (long long)d->Lq * (d->H / d->Hkv) <= 32;
 }
-int mode(const pf_attn_ranges_desc* d) { return (d->cap > 0.f ? 1 : 0) + (d->bias ? 2 : 0); }
+int mode(const pf_attn_ranges_desc* d) { return (d->cap > 64.f ? 5 : (d->cap > 0.f ? 1 : 0)) + (d->bias ? 2 : 0); }
 int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * (d->H / d->Hkv) + 31) / 32); }
 int splits(const pf_attn_ranges_desc* d) {
     const long long units = (long long)row_blocks(d) * d->Hkv * d->B, tiles = (d->Lk + 31) / 32;
@@ -1208,7 +1262,8 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
     a.bias = d->bias; a.R = d->bias ? d->bias_radius : 0;
     a.scale = d->scale;
     a.cap2 = d->cap * LOG2E;
-    a.zs = d->cap > 0.f ? d->scale / d->cap : d->scale * LOG2E;
+    a.series = d->cap > 64.f;
+    a.zs = d->cap > 0.f ? d->scale / d->cap * (a.series ? 1.f : 2.f * LOG2E) : d->scale * LOG2E;
     a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
     a.nqt = (d->Lq + 127) / 128; a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
     return a;
@@ -1258,8 +1313,8 @@ int launch_bwd(const RArgs& a, hipStream_t stream) {
         }
     }
     if (a.Lq > 0) {
-        const size_t lds = 4 * 64 * 2 * D + (MODE & 2 ? 5 * (2 * a.R + 1) * 4 : 0);
-        PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE>), 4 * 64 * 2 * D + (MODE & 2 ? 5 * (2 * MAX_RADIUS + 1) * 4 : 0));
+        const size_t lds = 4 * 64 * 2 * D + (MODE & 2 ? 5 * (2 * a.R + 1) * 4 + 12 + 4 * SKEW * 4 : 0);
+        PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE>), 4 * 64 * 2 * D + (MODE & 2 ? 5 * (2 * MAX_RADIUS + 1) * 4 + 12 + 4 * SKEW * 4 : 0));
         range_dq_kernel<D, MODE><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
         CHECK_LAUNCH();
     }
@@ -1295,15 +1350,19 @@ extern "C" int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, hipStream_
     a.nrb = row_blocks(d);
     a.nsplit = few ? splits(d) : 1;
     a.parts = (float*)d->workspace;
-    switch ((d->D == 64 ? 0 : 4) + mode(d)) {
+    switch ((d->D == 64 ? 0 : 8) + mode(d)) {
         case 0: return launch_fwd<64, 0>(a, few, stream);
         case 1: return launch_fwd<64, 1>(a, few, stream);
         case 2: return launch_fwd<64, 2>(a, few, stream);
         case 3: return launch_fwd<64, 3>(a, few, stream);
-        case 4: return launch_fwd<128, 0>(a, few, stream);
-        case 5: return launch_fwd<128, 1>(a, few, stream);
-        case 6: return launch_fwd<128, 2>(a, few, stream);
-        default: return launch_fwd<128, 3>(a, few, stream);
+        case 5: return launch_fwd<64, 5>(a, few, stream);
+        case 7: return launch_fwd<64, 7>(a, few, stream);
+        case 8: return launch_fwd<128, 0>(a, few, stream);
+        case 9: return launch_fwd<128, 1>(a, few, stream);
+        case 10: return launch_fwd<128, 2>(a, few, stream);
+        case 11: return launch_fwd<128, 3>(a, few, stream);
+        case 13: return launch_fwd<128, 5>(a, few, stream);
+        default: return launch_fwd<128, 7>(a, few, stream);
     }
 }
 
@@ -1328,15 +1387,19 @@ extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t
     a.kv_split = kv_splits(d);
     a.dbias = d->dbias;
     int rc = 0;
-    if (d->B) switch ((d->D == 64 ? 0 : 4) + mode(d)) {
+    if (d->B) switch ((d->D == 64 ? 0 : 8) + mode(d)) {
         case 0: rc = launch_bwd<64, 0>(a, stream); break;
         case 1: rc = launch_bwd<64, 1>(a, stream); break;
         case 2: rc = launch_bwd<64, 2>(a, stream); break;
         case 3: rc = launch_bwd<64, 3>(a, stream); break;
-        case 4: rc = launch_bwd<128, 0>(a, stream); break;
-        case 5: rc = launch_bwd<128, 1>(a, stream); break;
-        case 6: rc = launch_bwd<128, 2>(a, stream); break;
-        default: rc = launch_bwd<128, 3>(a, stream); break;
+        case 5: rc = launch_bwd<64, 5>(a, stream); break;
+        case 7: rc = launch_bwd<64, 7>(a, stream); break;
+        case 8: rc = launch_bwd<128, 0>(a, stream); break;
+        case 9: rc = launch_bwd<128, 1>(a, stream); break;
+        case 10: rc = launch_bwd<128, 2>(a, stream); break;
+        case 11: rc = launch_bwd<128, 3>(a, stream); break;
+        case 13: rc = launch_bwd<128, 5>(a, stream); break;
+        default: rc = launch_bwd<128, 7>(a, stream); break;
     }
     if (rc == 0 && d->dbias) {
         range_dbias_kernel<<<dim3((2 * a.R + 1 + 63) / 64, a.H), 256, 0, stream>>>(a);

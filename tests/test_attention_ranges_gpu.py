@@ -91,6 +91,8 @@ CASES = [  # B, Lq, Lk, H, Hkv, D, kind, radius, cap
     (1, 257, 257, 4, 1, 128, "documents causal", 512, 0.0),
     (2, 31, 1000, 2, 1, 64, "random", 40, 9.0),
     (1, 2, 5000, 4, 2, 128, "padded", None, 30.0),
+    (2, 90, 90, 4, 2, 64, "causal", 20, 64.5),
+    (1, 3, 700, 4, 2, 128, "random", None, 5000.0),
 ]
 MANY = [  # enough workgroups of 128 rows for the first form
     (4, 70, 70, 64, 64, 64, "causal", None, 0.0),
@@ -99,6 +101,8 @@ MANY = [  # enough workgroups of 128 rows for the first form
     (3, 200, 200, 48, 12, 64, "documents", 9, 25.0),
     (8, 128, 64, 32, 32, 128, "padded", 64, 0.0),
     (2, 385, 385, 40, 8, 64, "prefix", None, 0.0),
+    (4, 130, 130, 32, 8, 128, "random", 100, 300.0),
+    (4, 150, 150, 32, 32, 64, "causal", 30, 0.0),
 ]
 
 
