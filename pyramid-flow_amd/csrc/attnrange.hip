@@ -16,6 +16,7 @@
 //
 // A hidden key must not reach a row's result even as 0 x inf: the matrix products cannot tell, so a result row that came out
 // non-finite although some of the row's keys were hidden is recomputed by a plain loop over its visible keys (exact_*).
+#include <type_traits>
 #include "common.h"
 #include "pyflow_hip.h"
 
@@ -75,12 +76,6 @@ PF_DEVICE Vis load_vis(const RArgs& p, int b, int row) {
 PF_DEVICE bool sees(const Vis& v, int key) {
     return (unsigned)(key - v.alo) < (unsigned)v.na || (unsigned)(key - v.blo) < (unsigned)v.nb;
 }
-PF_DEVICE bool sees_any(const Vis& v, int j0, int j1) {
-    return (v.na && v.alo < j1 && v.alo + v.na > j0) || (v.nb && v.blo < j1 && v.blo + v.nb > j0);
-}
-PF_DEVICE bool sees_all(const Vis& v, int j0, int j1) {
-    return (v.alo <= j0 && v.alo + v.na >= j1) || (v.blo <= j0 && v.blo + v.nb >= j1);
-}
 
 PF_DEVICE int wave_min(int x) {
 #pragma unroll
@@ -117,6 +112,9 @@ PF_DEVICE TileList tile_list(int amin, int amax, int bmin, int bmax) {
     return {as, ae - as, bs, (ae - as) + (be - bs)};
 }
 
+template <int D>
+constexpr int FWD_KB = D == 64 ? 64 : 32;     // keys of a forward tile
+
 // ---------------------------------------------------------------------------------------------- LDS tiles
 // Row-major bf16 rows of D channels, 16-byte chunk c of row r at c ^ swz(r).  A row read (ds_read_b128, one chunk of 16
 // consecutive rows per 256 bytes) needs swz to differ over 16 rows modulo the row pitch; a transposed read
@@ -127,16 +125,66 @@ PF_DEVICE int swz(int r) {
     else return ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
-// rows [row0, row0 + ROWS) of a head -> LDS, by the NW waves that share the tile.  Rows behind `last` repeat it (hidden later).
+// Rows [row0, row0 + ROWS) of a head -> LDS, by the NW waves that share the tile.  A lane's 32-bit byte offsets inside a tile are
+// fixed, the tile's base is wave-uniform: no vector arithmetic per tile (64-bit addresses per piece were a sixth of the forward
+// kernel's vector instructions).  Rows behind `last` repeat it (hidden later).  Row strides are below 2^25 elements (host check).
 template <int D, int ROWS, int NW>
-PF_DEVICE void stage(const bf16_t* base, long long ld, int row0, int last, char* lds, int wid, int lane) {
-    constexpr int LPR = D / 8, RPP = 64 / LPR, N = ROWS / RPP / NW;            // lanes per row, rows per 1-KiB piece
+struct Stager {
+    static constexpr int LPR = D / 8, RPP = 64 / LPR, N = ROWS / RPP / NW;     // lanes per row, rows per 1-KiB piece
     static_assert(N >= 1 && N * RPP * NW == ROWS, "the tile is a whole number of pieces per wave");
+    unsigned off[N];
+    PF_DEVICE Stager(long long ld, int wid, int lane) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const int i = wid * N + j, r = i * RPP + lane / LPR, c = (lane % LPR) ^ swz<D>(r);
-        glds16(base + (long long)min(row0 + r, last) * ld + c * 8, lds + i * 1024);
+        for (int j = 0; j < N; ++j) {
+            const int r = (wid * N + j) * RPP + lane / LPR;
+            off[j] = (unsigned)r * (unsigned)(2 * ld) + (unsigned)(((lane % LPR) ^ swz<D>(r)) * 16);
+        }
     }
+    PF_DEVICE void issue(const bf16_t* head, long long ld, int row0, int last, char* lds, int wid, int lane) const {
+        const char* base = (const char*)(head + row0 * ld);
+        if (row0 + ROWS - 1 <= last) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) glds16(base + off[j], lds + (wid * N + j) * 1024);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int r = (wid * N + j) * RPP + lane / LPR;
+                const unsigned o = (unsigned)min(r, last - row0) * (unsigned)(2 * ld) + (unsigned)(((lane % LPR) ^ swz<D>(r)) * 16);
+                glds16(base + o, lds + (wid * N + j) * 1024);
+            }
+        }
+    }
+};
+
+// Wave-uniform bounds of the ranges of a wave's rows: any key of [j0, j1) seen by some row; all of them by every row (a
+// sufficient test: rows that cover it by different ranges count as partial)
+struct Bounds {
+    int amin, amax, bmin, bmax;                // over the ranges that are not empty
+    int alo, ahi, blo, bhi;                    // largest start, smallest end over all rows (an empty range: none)
+    PF_DEVICE bool any(int j0, int j1) const { return (amin < j1 && amax > j0) || (bmin < j1 && bmax > j0); }
+    PF_DEVICE bool full(int j0, int j1) const { return (alo <= j0 && ahi >= j1) || (blo <= j0 && bhi >= j1); }
+};
+PF_DEVICE Bounds wave_bounds(const Vis& v) {
+    auto lo = [](int x) { return __builtin_amdgcn_readfirstlane(wave_min(x)); };
+    auto hi = [](int x) { return __builtin_amdgcn_readfirstlane(wave_max(x)); };
+    constexpr int BIG = 0x7fffffff;
+    return {lo(v.na ? v.alo : BIG), hi(v.na ? v.alo + v.na : 0), lo(v.nb ? v.blo : BIG), hi(v.nb ? v.blo + v.nb : 0),
+            hi(v.na ? v.alo : BIG), lo(v.na ? v.alo + v.na : 0), hi(v.nb ? v.blo : BIG), lo(v.nb ? v.blo + v.nb : 0)};
+}
+// the key tiles of a workgroup of 4 waves (`red`: 16 ints of LDS, read behind a barrier)
+template <int KB>
+PF_DEVICE TileList workgroup_tiles(const Bounds& w, int* red, int wid, int lane) {
+    if (lane == 0) { red[4 * wid] = w.amin; red[4 * wid + 1] = w.amax; red[4 * wid + 2] = w.bmin; red[4 * wid + 3] = w.bmax; }
+    __syncthreads();
+    int x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[i] = red[i];
+#pragma unroll
+        for (int u = 1; u < 4; ++u) x[i] = (i & 1) ? max(x[i], red[4 * u + i]) : min(x[i], red[4 * u + i]);
+        x[i] = __builtin_amdgcn_readfirstlane(x[i]);
+    }
+    return tile_list<KB>(x[0], x[1], x[2], x[3]);
 }
 
 // A operand of a product over channels: row lane % 32 (+ 32 i), channels 16 ks + 8 (lane / 32) ..
@@ -375,14 +423,21 @@ PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0)
 }
 
 // ---------------------------------------------------------------------------------------------- forward, many rows
-// One workgroup = 128 rows of one head, 4 waves x 32; key tiles of 64, two in flight.  MODE bits: 1 cap, 2 bias (scores are
+// One workgroup = 128 rows of one head, 4 waves x 32; key tiles of KB, two in flight.  MODE bits: 1 cap, 2 bias (scores are
 // formed in base 2 before the maximum; neither: they stay raw and the exponent's multiply-add scales them), 4 SERIES.
+//
+// Bound: vector issue (per 32 rows x 64 keys 512 cycles of matrix pipe at D = 64 against 32 multiply-adds, 32 exponentials at
+// 8 cycles, 32 adds, 16 conversions).  So the first pass keeps no running maximum: a row's reference is the maximum of the first
+// tile in which it sees a key; a weight may then grow to 2^127 before anything overflows and its rounding to bf16 is relative,
+// so the result is the same.  If a sum or a result of the workgroup came out non-finite, it runs again with the running maximum
+// (CAREFUL), and rows that are still non-finite and had hidden keys are recomputed from their visible keys (exact_o).
 template <int D, int MODE>
 __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
-    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
-    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
+    constexpr bool BIAS = MODE & 2, EX = MODE != 0;
+    constexpr int KB = FWD_KB<D>, NI = KB / 32, TILE = KB * 2 * D, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    float* const tab = (float*)(smem + 2 * BUF);
+    int* const redo_flag = (int*)(smem + 2 * BUF);
+    float* const tab = (float*)(smem + 2 * BUF + 16);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = xcd_remap(blockIdx.x, p.nqt * p.H * p.B);
     const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
@@ -390,30 +445,13 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
     const int hi = lane >> 5, row = qt * 128 + wid * 32 + (lane & 31);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
-
-    // ---- the workgroup's key tiles
-    int* const red = (int*)smem;
-    {
-        const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
-        const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
-        if (lane == 0) { red[4 * wid] = amin; red[4 * wid + 1] = amax; red[4 * wid + 2] = bmin; red[4 * wid + 3] = bmax; }
-    }
+    const Bounds wb = wave_bounds(vis);
     if (BIAS) load_table(p, h, tab);
-    __syncthreads();
-    TileList tl;
-    {
-        int x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = red[i];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) x[i] = (i & 1) ? max(x[i], red[4 * w + i]) : min(x[i], red[4 * w + i]);
-            x[i] = __builtin_amdgcn_readfirstlane(x[i]);
-        }
-        tl = tile_list<64>(x[0], x[1], x[2], x[3]);
-    }
+    if (threadIdx.x == 0) *redo_flag = 0;
+    const TileList tl = workgroup_tiles<KB>(wb, (int*)smem, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
+    const Stager<D, KB, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
     bf16x8_t qf[D / 16];
     {
         const bf16_t* q = p.q.p + b * p.q.bs + (long long)min(row, p.Lq - 1) * p.q.ld + h * p.q.hs + hi * 8;
@@ -422,83 +460,100 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
     }
     const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
     f32x16_t o[D / 32];
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) o[c] = zero16();
-    float m = -__builtin_inff(), l = 0.f;
-    bool whole = true;                             // wave-uniform: no row of the wave had a hidden key in any tile
-    drain_barrier();                               // `red` is read: its memory becomes tile memory
+    float m, l;
+    bool whole;                                    // wave-uniform: no row of the wave had a hidden key in any tile
     auto issue = [&](int n) {
-        const int j0 = tl.at(n) * 64;
+        const int j0 = tl.at(n) * KB;
         char* buf = smem + (n & 1) * BUF;
-        stage<D, 64, 4>(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
-        stage<D, 64, 4>(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
+        sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
+        sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
     };
-    if (tl.n > 0) issue(0);
-    for (int n = 0; n < tl.n; ++n) {
-        drain_barrier();
-        if (n + 1 < tl.n) issue(n + 1);
-        const int j0 = tl.at(n) * 64;
-        const char* sk = smem + (n & 1) * BUF;
-        const char* sv = sk + TILE;
-        const bool full = __builtin_amdgcn_ballot_w64(!sees_all(vis, j0, j0 + 64)) == 0;
-        if (!full) {
-            whole = false;
-            if (__builtin_amdgcn_ballot_w64(sees_any(vis, j0, j0 + 64)) == 0) continue;
-        }
-        f32x16_t s[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            s[i] = zero16();
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) s[i] = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s[i]);
-        }
-        if (EX) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) cap_bias<MODE>(p, s[i], tab, j0 + 32 * i + 4 * hi - pos);
-        }
-        if (!full) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] = sees(vis, j0 + 32 * i + 4 * hi + reg_row(r)) ? s[i][r] : -__builtin_inff();
-        }
-        float mt = s[0][0];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[i][r]);
-        mt = fmaxf(mt, other_half(mt));
+    auto pass = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
         const float zs = EX ? 1.f : p.zs;
-        mt *= zs;
-        if (__builtin_amdgcn_ballot_w64(mt > m + DEFER) != 0) {
-            const float mn = fmaxf(m, mt);
-            const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= alpha;
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[c][r] *= alpha;
-        }
-        const float ms = m == -__builtin_inff() ? 0.f : m;
-        float ps = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], zs, -ms));
-                s[i][r] = e;
-                ps += e;
+        for (int c = 0; c < D / 32; ++c) o[c] = zero16();
+        m = -__builtin_inff();
+        l = 0.f;
+        whole = true;
+        unsigned long long fresh = __builtin_amdgcn_ballot_w64(vis.na + vis.nb > 0);     // rows without a reference yet
+        drain_barrier();                           // nobody reads what lay in the tiles' memory any more
+        if (tl.n > 0) issue(0);
+        for (int n = 0; n < tl.n; ++n) {
+            drain_barrier();
+            if (n + 1 < tl.n) issue(n + 1);
+            const int j0 = tl.at(n) * KB;
+            const char* sk = smem + (n & 1) * BUF;
+            const char* sv = sk + TILE;
+            const bool full = wb.full(j0, j0 + KB);
+            if (!full) {
+                whole = false;
+                if (!wb.any(j0, j0 + KB)) continue;
             }
-        l += ps;
+            f32x16_t s[NI];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const bf16x8_t pf = half_of(s[g >> 1], g & 1);
+            for (int i = 0; i < NI; ++i) {
+                s[i] = zero16();
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) o[c] = mfma(tr_frag<D>(sv, t0, t8, c, g), pf, o[c]);
+                for (int ks = 0; ks < D / 16; ++ks) s[i] = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s[i]);
+            }
+            if (EX) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i) cap_bias<MODE>(p, s[i], tab, j0 + 32 * i + 4 * hi - pos);
+            }
+            if (!full) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = sees(vis, j0 + 32 * i + 4 * hi + reg_row(r)) ? s[i][r] : -__builtin_inff();
+            }
+            if (CAREFUL || fresh != 0) {           // wave-uniform
+                float mt = s[0][0];
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[i][r]);
+                mt = fmaxf(mt, other_half(mt)) * zs;
+                if (CAREFUL) {
+                    if (__builtin_amdgcn_ballot_w64(mt > m + DEFER) != 0) {
+                        const float mn = fmaxf(m, mt);
+                        const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                        m = mn;
+                        l *= alpha;
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[c][r] *= alpha;
+                    }
+                } else {
+                    m = m == -__builtin_inff() ? mt : m;
+                    fresh &= __builtin_amdgcn_ballot_w64(m == -__builtin_inff());
+                }
+            }
+            const float ms = m == -__builtin_inff() ? 0.f : m;
+            float ps[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], zs, -ms));
+                    s[i][r] = e;
+                    ps[r & 1] += e;
+                }
+            l += ps[0] + ps[1];
+#pragma unroll
+            for (int g = 0; g < 2 * NI; ++g) {
+                const bf16x8_t pf = half_of(s[g >> 1], g & 1);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) o[c] = mfma(tr_frag<D>(sv, t0, t8, c, g), pf, o[c]);
+            }
         }
-    }
-    l += other_half(l);
+        l += other_half(l);
+    };
+    pass(std::false_type{});
+    if (__builtin_amdgcn_ballot_w64(!(l < __builtin_inff()) || any_nonfinite<D / 32>(o)) != 0 && lane == 0) *redo_flag = 1;
+    __syncthreads();
+    if (*redo_flag != 0) pass(std::true_type{});   // workgroup-uniform: the passes share tiles and barriers
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const bool bad = any_nonfinite<D / 32>(o) && !whole && l == l && row < p.Lq;
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
@@ -557,10 +612,11 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
     float m = -__builtin_inff(), l = 0.f;
     char* const mem = smem + wid * WAVE;
     drain();                                                        // the counted waits below see tile pieces only
+    const Stager<D, 32, 1> sk_(p.k.ld, 0, lane), sv_(p.v.ld, 0, lane);
     auto issue = [&](int n, int buf) {
         const int j0 = tl.at(n) * 32;
-        stage<D, 32, 1>(K, p.k.ld, j0, p.Lk - 1, mem + buf * BUF, 0, lane);
-        stage<D, 32, 1>(V, p.v.ld, j0, p.Lk - 1, mem + buf * BUF + TILE, 0, lane);
+        sk_.issue(K, p.k.ld, j0, p.Lk - 1, mem + buf * BUF, 0, lane);
+        sv_.issue(V, p.v.ld, j0, p.Lk - 1, mem + buf * BUF + TILE, 0, lane);
     };
     if (n0 + wid < n1) issue(n0 + wid, 0);
     int buf = 0;
@@ -780,6 +836,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void range_dkv_kernel(const R
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = zero16();
     const int wg0 = kt * 128, wg1 = min(wg0 + 128, p.Lk);
+    const Stager<D, 64, 4> sq_(p.q.ld, wid, lane), so_(p.dO.ld, wid, lane);
 
     // ---- the (head, tile) pairs n = g nq + tile of this part, 64 at a time: which the workgroup needs, which this wave sees at all,
     //      which it sees whole
@@ -814,8 +871,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void range_dkv_kernel(const R
     auto issue = [&](int n, int buf) {
         const int h = hk * p.G + n / nq, qt = n % nq;
         char* dst = smem + buf * BUF;
-        stage<D, 64, 4>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, qt * 64, p.Lq - 1, dst, wid, lane);
-        stage<D, 64, 4>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, qt * 64, p.Lq - 1, dst + TILE, wid, lane);
+        sq_.issue(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, qt * 64, p.Lq - 1, dst, wid, lane);
+        so_.issue(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, qt * 64, p.Lq - 1, dst + TILE, wid, lane);
         if (wid == 0) glds16(p.stat + (((long long)b * p.H + h) * nq + qt) * 256 + lane * 4, dst + 2 * TILE);
         if (wid == 1) glds16(p.vis + ((long long)b * nq + qt) * 256 + lane * 4, dst + 2 * TILE + 1024);
     };
@@ -1015,12 +1072,7 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     const int hi = lane >> 5, row = qt * 128 + wid * 32 + (lane & 31), rc = min(row, p.Lq - 1);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, rc) : 0;
-    int* const red = (int*)smem;
-    {
-        const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
-        const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
-        if (lane == 0) { red[4 * wid] = amin; red[4 * wid + 1] = amax; red[4 * wid + 2] = bmin; red[4 * wid + 3] = bmax; }
-    }
+    const Bounds wb = wave_bounds(vis);
     if (BIAS) {
         load_table(p, h, tab);
         if (p.dbias) {
@@ -1028,19 +1080,8 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
             for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
         }
     }
-    __syncthreads();
-    TileList tl;
-    {
-        int x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = red[i];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) x[i] = (i & 1) ? max(x[i], red[4 * w + i]) : min(x[i], red[4 * w + i]);
-            x[i] = __builtin_amdgcn_readfirstlane(x[i]);
-        }
-        tl = tile_list<64>(x[0], x[1], x[2], x[3]);
-    }
+    const TileList tl = workgroup_tiles<64>(wb, (int*)smem, wid, lane);
+    const Stager<D, 64, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
     bf16x8_t qf[D / 16], of[D / 16];
@@ -1068,8 +1109,8 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     auto issue = [&](int n) {
         const int j0 = tl.at(n) * 64;
         char* buf = smem + (n & 1) * BUF;
-        stage<D, 64, 4>(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
-        stage<D, 64, 4>(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
+        sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
+        sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
     };
     if (tl.n > 0) issue(0);
     for (int n = 0; n < tl.n; ++n) {
@@ -1078,10 +1119,10 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
         const int j0 = tl.at(n) * 64;
         const char* sk = smem + (n & 1) * BUF;
         const char* sv = sk + TILE;
-        const bool full = __builtin_amdgcn_ballot_w64(!sees_all(vis, j0, j0 + 64)) == 0;
+        const bool full = wb.full(j0, j0 + 64);
         if (!full) {
             whole = false;
-            if (__builtin_amdgcn_ballot_w64(sees_any(vis, j0, j0 + 64)) == 0) continue;
+            if (!wb.any(j0, j0 + 64)) continue;
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -1184,7 +1225,7 @@ __global__ __launch_bounds__(256) void range_dbias_kernel(const RArgs p) {
 
 // ---------------------------------------------------------------------------------------------- host side
 bool bad_view(const pf_rows_view& v) {
-    return !v.p || ((uintptr_t)v.p & 15) || v.batch < 0 || v.row < 0 || v.head < 0 || ((v.batch | v.row | v.head) & 7);
+    return !v.p || ((uintptr_t)v.p & 15) || v.batch < 0 || v.row < 0 || v.head < 0 || ((v.batch | v.row | v.head) & 7) || v.row >= (1 << 25);
 }
 View view(const pf_rows_view& v) { return {(bf16_t*)v.p, v.batch, v.row, v.head}; }
 
@@ -1202,7 +1243,7 @@ const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
     if (d->bias && (d->bias_radius < 0 || d->bias_radius > MAX_RADIUS)) return "pf_attention_ranges: bias_radius must be in 0..512";
     if (d->dbias && !d->bias) return "pf_attention_ranges: a bias gradient without a bias";
     const bool rows = d->B && d->H && d->Lq, keys = d->B && d->H && d->Lk;
-    const char* const bad = "pf_attention_ranges: tensors must be 16-byte aligned with strides that are multiples of 8 elements";
+    const char* const bad = "pf_attention_ranges: tensors must be 16-byte aligned with strides that are multiples of 8 elements, rows less than 2^25 elements apart";
     if ((rows && (bad_view(d->Q) || bad_view(d->O))) || (keys && (bad_view(d->K) || bad_view(d->V)))) return bad;
     if (grad) {
         if ((rows && (bad_view(d->dO) || bad_view(d->dQ))) || (keys && (bad_view(d->dK) || bad_view(d->dV)))) return bad;
@@ -1278,7 +1319,7 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
 template <int D, int MODE>
 int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
     if (!few) {
-        const size_t lds = 4 * 64 * 2 * D + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
+        const size_t lds = 4 * FWD_KB<D> * 2 * D + 16 + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
         PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, MODE>), (int)lds);
         range_fwd_kernel<D, MODE><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
         CHECK_LAUNCH();
