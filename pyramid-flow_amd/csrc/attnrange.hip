@@ -801,17 +801,22 @@ __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
     }
 }
 
-// dK, dV of 128 keys of one key head: 4 waves x 32 keys held in registers, looping over the 64-row tiles (of every query head that
-// shares the key head) that see any of them.  The bounds of 64 tiles are tested at once (one lane each); the next tile is in
-// flight while one is used.  -delta enters through the C operand of the dP product.  kv_split > 1: this workgroup takes one part
-// of the (head, tile) list and leaves 32-bit sums for range_kvjoin_kernel.
+// dK, dV of 128 keys of one key head: 4 waves x 32 keys, looping over the row tiles (of every query head that shares the key head)
+// that see any of them.  The bounds of 64 tiles are tested at once (one lane each); the next tile is in flight while one is used.
+// -delta enters through the C operand of the dP product.  kv_split > 1: this workgroup takes an even part of the (head, tile)
+// pairs that the keys need and leaves 32-bit sums for range_kvjoin_kernel.
+//
+// D = 64: 64-row tiles, K and V fragments and both results in registers (two workgroups per compute unit).  D = 128 has twice
+// the results (128 registers): 32-row tiles and V read from LDS leave room for the second workgroup (with V in registers and
+// 64-row tiles one wave per SIMD ran everything in series, 8400 cycles per tile, 800 of its instructions register moves).
 template <int D, int MODE>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void range_dkv_kernel(const RArgs p) {
-    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
-    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE + 2048;
+__global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0, VLDS = D == 128;
+    constexpr int RT = D == 64 ? 64 : 32, HALVES = 64 / RT, TILE = RT * 2 * D, BUF = 2 * TILE + 2048, VTILE = VLDS ? 32 * 2 * D : 0;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    float* const tab = (float*)(smem + 2 * BUF);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    char* const vtile = smem + 2 * BUF + wid * VTILE;
+    float* const tab = (float*)(smem + 2 * BUF + 4 * VTILE);
     const int t = xcd_remap(blockIdx.x, p.nkt * p.kv_split * p.Hk * p.B);
     const int unit = t / p.kv_split, part = t - unit * p.kv_split;
     const int bk = unit / p.nkt, kt = unit - bk * p.nkt;
@@ -820,15 +825,19 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void range_dkv_kernel(const R
     const int w0 = kt * 128 + wid * 32, key = w0 + (lane & 31);
     const int nq = p.nq64;
     const int* const tiles = p.tiles + (long long)b * nq * 8;
-    bf16x8_t kf[D / 16], vf[D / 16];
+    bf16x8_t kf[D / 16], vf[VLDS ? 1 : D / 16];
     {
         const long long kr = min(key, p.Lk - 1);
         const bf16_t* k = p.k.p + b * p.k.bs + kr * p.k.ld + hk * p.k.hs + hi * 8;
-        const bf16_t* v = p.v.p + b * p.v.bs + kr * p.v.ld + hk * p.v.hs + hi * 8;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            kf[ks] = *(const bf16x8_t*)(k + ks * 16);
-            vf[ks] = *(const bf16x8_t*)(v + ks * 16);
+        for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *(const bf16x8_t*)(k + ks * 16);
+        if constexpr (VLDS) {
+            const Stager<D, 32, 1> s(p.v.ld, 0, lane);
+            s.issue(p.v.p + b * p.v.bs + hk * p.v.hs, p.v.ld, min(w0, p.Lk - 1), p.Lk - 1, vtile, 0, lane);
+        } else {
+            const bf16_t* v = p.v.p + b * p.v.bs + kr * p.v.ld + hk * p.v.hs + hi * 8;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) vf[ks] = *(const bf16x8_t*)(v + ks * 16);
         }
     }
     const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
@@ -836,65 +845,84 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void range_dkv_kernel(const R
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dk[c] = dv[c] = zero16();
     const int wg0 = kt * 128, wg1 = min(wg0 + 128, p.Lk);
-    const Stager<D, 64, 4> sq_(p.q.ld, wid, lane), so_(p.dO.ld, wid, lane);
+    const Stager<D, RT, 4> sq_(p.q.ld, wid, lane), so_(p.dO.ld, wid, lane);
 
-    // ---- the (head, tile) pairs n = g nq + tile of this part, 64 at a time: which the workgroup needs, which this wave sees at all,
+    // ---- the (head g, 64-row tile) pairs of this part, 64 tiles at a time: which the workgroup needs, which this wave sees at all,
     //      which it sees whole
-    const int total = p.G * nq;
-    int base = (int)((long long)total * part / p.kv_split), group = 0;
-    const int end = (int)((long long)total * (part + 1) / p.kv_split);
     unsigned long long need = 0, some = 0, all = 0;
-    auto refill = [&] {
-        while (need == 0 && base < end) {
-            const int n = base + lane;
-            int x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (n < end) {
-                const u32x4_t u = *(const u32x4_t*)(tiles + (n % nq) * 8), v = *(const u32x4_t*)(tiles + (n % nq) * 8 + 4);
+    auto test = [&](int base) {
+        const int n = base + lane;
+        int x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (n < nq) {
+            const u32x4_t u = *(const u32x4_t*)(tiles + n * 8LL), v = *(const u32x4_t*)(tiles + n * 8LL + 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { x[i] = (int)u[i]; x[4 + i] = (int)v[i]; }
-            }
-            need = __builtin_amdgcn_ballot_w64((x[0] < wg1 && x[1] > wg0) || (x[2] < wg1 && x[3] > wg0));
-            some = __builtin_amdgcn_ballot_w64((x[0] < w0 + 32 && x[1] > w0) || (x[2] < w0 + 32 && x[3] > w0));
-            all = __builtin_amdgcn_ballot_w64((x[4] <= w0 && x[5] >= w0 + 32) || (x[6] <= w0 && x[7] >= w0 + 32));
-            group = base;
-            base += 64;
+            for (int i = 0; i < 4; ++i) { x[i] = (int)u[i]; x[4 + i] = (int)v[i]; }
         }
+        need = __builtin_amdgcn_ballot_w64((x[0] < wg1 && x[1] > wg0) || (x[2] < wg1 && x[3] > wg0));
+        some = __builtin_amdgcn_ballot_w64((x[0] < w0 + 32 && x[1] > w0) || (x[2] < w0 + 32 && x[3] > w0));
+        all = __builtin_amdgcn_ballot_w64((x[4] <= w0 && x[5] >= w0 + 32) || (x[6] <= w0 && x[7] >= w0 + 32));
     };
-    struct Item { int n; bool any, full; };
+    int g = 0, base = 0, skip = 0, left = 0x7fffffff, group_g = 0, group_base = 0;
+    if (p.kv_split > 1) {
+        int per_head = 0;
+        for (int n = 0; n < nq; n += 64) {
+            test(n);
+            per_head += __builtin_popcountll(need);
+        }
+        need = 0;
+        const long long pairs = (long long)per_head * p.G, from = pairs * part / p.kv_split;
+        left = (int)(pairs * (part + 1) / p.kv_split - from);
+        g = per_head ? (int)(from / per_head) : p.G;
+        skip = (int)(from - (long long)g * per_head);
+    }
+    struct Item { int g, qt, half; bool any, full; };
     auto pop = [&]() -> Item {
-        refill();
-        if (need == 0) return {-1, false, false};
+        while (need == 0) {
+            if (left == 0 || g >= p.G || nq == 0) return {-1, 0, 0, false, false};
+            test(base);
+            group_g = g;
+            group_base = base;
+            base += 64;
+            if (base >= nq) { base = 0; ++g; }
+            while (skip > 0 && need != 0) { need &= need - 1; --skip; }
+        }
+        if (left == 0) return {-1, 0, 0, false, false};
         const int i = __builtin_ctzll(need);
         need &= need - 1;
-        return {group + i, ((some >> i) & 1) != 0, ((all >> i) & 1) != 0};
+        --left;
+        return {group_g, group_base + i, 0, ((some >> i) & 1) != 0, ((all >> i) & 1) != 0};
     };
-    auto issue = [&](int n, int buf) {
-        const int h = hk * p.G + n / nq, qt = n % nq;
+    auto follow = [&](const Item& c) -> Item {                      // the other half of a tile, if it has rows, or the next tile
+        if (HALVES == 2 && c.half == 0 && c.qt * 64 + RT < p.Lq) return {c.g, c.qt, 1, c.any, c.full};
+        return pop();
+    };
+    auto issue = [&](const Item& n, int buf) {
+        const int h = hk * p.G + n.g, r0 = n.qt * 64 + n.half * RT;
         char* dst = smem + buf * BUF;
-        sq_.issue(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, qt * 64, p.Lq - 1, dst, wid, lane);
-        so_.issue(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, qt * 64, p.Lq - 1, dst + TILE, wid, lane);
-        if (wid == 0) glds16(p.stat + (((long long)b * p.H + h) * nq + qt) * 256 + lane * 4, dst + 2 * TILE);
-        if (wid == 1) glds16(p.vis + ((long long)b * nq + qt) * 256 + lane * 4, dst + 2 * TILE + 1024);
+        sq_.issue(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, r0, p.Lq - 1, dst, wid, lane);
+        so_.issue(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, r0, p.Lq - 1, dst + TILE, wid, lane);
+        if (wid == 0) glds16(p.stat + (((long long)b * p.H + h) * nq + n.qt) * 256 + lane * 4, dst + 2 * TILE);
+        if (wid == 1) glds16(p.vis + ((long long)b * nq + n.qt) * 256 + lane * 4, dst + 2 * TILE + 1024);
     };
     Item cur = pop();
     int buf = 0, table_of = -1;
-    if (cur.n >= 0) issue(cur.n, 0);
-    while (cur.n >= 0) {
+    if (cur.g >= 0) issue(cur, 0);
+    while (cur.g >= 0) {
         drain_barrier();
-        if (BIAS && cur.n / nq != table_of) {               // uniform: another head, another bias table
-            table_of = cur.n / nq;
+        if (BIAS && cur.g != table_of) {                            // uniform: another head, another bias table
+            table_of = cur.g;
             load_table(p, hk * p.G + table_of, tab);
             drain_barrier();
         }
-        const Item nxt = pop();
-        if (nxt.n >= 0) issue(nxt.n, buf ^ 1);
+        const Item nxt = follow(cur);
+        if (nxt.g >= 0) issue(nxt, buf ^ 1);
         if (cur.any) {
             const char* sq = smem + buf * BUF;
             const char* so = sq + TILE;
-            const float* st = (const float*)(sq + 2 * TILE);
-            const int* vi = (const int*)(sq + 2 * TILE + 1024);
+            const float* st = (const float*)(sq + 2 * TILE) + cur.half * RT;
+            const int* vi = (const int*)(sq + 2 * TILE + 1024) + cur.half * RT;
 #pragma unroll
-            for (int qb = 0; qb < 2; ++qb) {
+            for (int qb = 0; qb < RT / 32; ++qb) {
                 f32x16_t s = zero16(), dp;
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
@@ -905,7 +933,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void range_dkv_kernel(const R
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
                     s = mfma(row_frag<D>(sq, roff, qb, ks), kf[ks], s);
-                    dp = mfma(row_frag<D>(so, roff, qb, ks), vf[ks], dp);
+                    dp = mfma(row_frag<D>(so, roff, qb, ks), VLDS ? row_frag<D>(vtile, roff, 0, ks) : vf[VLDS ? 0 : ks], dp);
                 }
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
@@ -1344,7 +1372,8 @@ int launch_bwd(const RArgs& a, hipStream_t stream) {
         CHECK_LAUNCH();
     }
     if (a.Lk > 0) {
-        const size_t lds = 2 * (2 * 64 * 2 * D + 2048) + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
+        const int rt = D == 64 ? 64 : 32;
+        const size_t lds = 2 * (2 * rt * 2 * D + 2048) + (D == 128 ? 4 * 32 * 2 * D : 0) + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
         PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, MODE>), (int)lds);
         range_dkv_kernel<D, MODE><<<(unsigned)(a.nkt * a.kv_split * a.Hk * a.B), 256, lds, stream>>>(a);
         CHECK_LAUNCH();
