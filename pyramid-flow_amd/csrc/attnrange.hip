@@ -39,7 +39,10 @@ struct RArgs {
     const int* a_lo; const int* a_hi; const int* b_lo; const int* b_hi; long long range_bs;
     const int* q_pos; long long pos_bs;
     const float* bias; int R;
-    float zs, cap2, scale;             // z zs = base-2 score (uncapped), tanh's argument (series) or 2 log2 e times it; cap log2 e, 0 = uncapped
+    // z = q.k.  Scores in base 2 are x zs + shift with x = z (uncapped), x = cap_u(z zc) (cap) or x = cap log2 e tanh(z zc) (SERIES);
+    // the shift is left out wherever only differences of scores count
+    float zs, zc, shift, cap2;
+    float scale, dscale;               // dQ, dK = dscale times the products of dZ (4 scale with cap_u's slope)
     int series;
     int B, H, Hk, G, Lq, Lk;
     int nqt, nkt, nrb, nsplit;
@@ -241,36 +244,40 @@ PF_DEVICE float other_half(float x) {
 }
 
 // ---------------------------------------------------------------------------------------------- scores
-// cap tanh(z / cap) in base 2 from the raw product.  1 - 2 / (1 + e^2x) leaves 2^-23 of the CAP in the score, nothing for caps up
-// to 64 (8e-6); SERIES (larger caps) takes the odd series below |x| = 0.3 (next term 0.0089 x^10: 5e-8), where a score is a small
-// part of its cap.  The series in every call cost 19 us of 165 at 16 heads of 128 channels and 8000 packed rows.  slope = 1 - tanh^2.
+// cap tanh(z / cap) = cap (1 + 2 u) with u = -1 / (1 + 2^(z zc)), zc = 2 scale log2 e / cap: the kernels keep u where an uncapped
+// score would be (its factor is 2 cap log2 e), and the slope 1 - tanh^2 = -4 (u + u^2).  That leaves 2^-23 of the CAP in the
+// score, nothing for caps up to 64 (8e-6); SERIES (larger caps) takes tanh itself, below |x| = 0.3 by its odd series (next term
+// 0.0089 x^10: 5e-8).  The series in every call cost 19 us of 165 at 16 heads of 128 channels and 8000 packed rows.
+PF_DEVICE float cap_u(float x) { return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x)); }
 PF_DEVICE float tanh_f(float x) {
     const float y = x * x;
     const float near = x * __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
     const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x));
     return fabsf(x) < 0.3f ? near : far;
 }
-template <bool SERIES>
+// x of one product and the slope of the cap (a quarter of it with cap_u)
+template <int MODE>
 PF_DEVICE float capped(const RArgs& p, float z, float& slope) {
-    if constexpr (SERIES) {
-        const float y = tanh_f(z * p.zs);
+    if constexpr ((MODE & 1) == 0) {
+        return z;
+    } else if constexpr ((MODE & 4) != 0) {
+        const float y = tanh_f(z * p.zc);
         slope = __builtin_fmaf(-y, y, 1.f);
         return p.cap2 * y;
     } else {
-        const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * p.zs));
-        slope = 4.f * __builtin_fmaf(-r, r, r);
-        return __builtin_fmaf(-2.f * p.cap2, r, p.cap2);
+        const float u = cap_u(z * p.zc);
+        slope = __builtin_fmaf(-u, u, -u);
+        return u;
     }
 }
 PF_DEVICE float bias2(float b) { return b <= HIDDEN ? -__builtin_inff() : b * LOG2E; }
 
 // base-2 score of one pair from global memory (exact_* and nothing else)
 PF_DEVICE float score2(const RArgs& p, float z, int h, int dist, float& slope) {
-    float t = z * p.zs;
     slope = 1.f;
-    if (p.cap2 != 0.f) t = p.series ? capped<true>(p, z, slope) : capped<false>(p, z, slope);
-    if (p.bias) t += bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(dist, -p.R), p.R) + p.R]);
-    return t;
+    const float x = p.cap2 == 0.f ? z : p.series ? capped<5>(p, z, slope) : capped<1>(p, z, slope);
+    const float t = __builtin_fmaf(x, p.zs, p.shift);
+    return p.bias ? t + bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(dist, -p.R), p.R) + p.R]) : t;
 }
 PF_DEVICE int row_pos(const RArgs& p, int b, int row) { return p.q_pos ? p.q_pos[b * p.pos_bs + row] : row + p.Lk - p.Lq; }
 
@@ -341,7 +348,7 @@ PF_DEVICE bool exact_pair(const RArgs& p, int b, int h, int hk, int i, int j, fl
     const float t = score2(p, z, h, j - row_pos(p, b, i), slope);
     if (t == -__builtin_inff()) return false;
     const float* st = p.stat + (((long long)b * p.H + h) * p.nq64 + (i >> 6)) * 256 + (i & 63);
-    P = __builtin_amdgcn_exp2f(t - st[0]);
+    P = __builtin_amdgcn_exp2f(t - p.shift - st[0]);
     const float dp = dot_row<D>(p.dO.p + b * p.dO.bs + i * p.dO.ld + h * p.dO.hs, p.v.p + b * p.v.bs + j * p.v.ld + hk * p.v.hs);
     dz = P * (dp + st[64]) * slope;
     return true;
@@ -357,7 +364,7 @@ PF_DEVICE void exact_dq(const RArgs& p, int b, int h, int i) {
         if (__builtin_amdgcn_ballot_w64(use) == 0) continue;
         float P = 0.f, dz = 0.f;
         if (use) use = exact_pair<D>(p, b, h, hk, i, j, P, dz);
-        add_rows<D>(p.k.p + b * p.k.bs + hk * p.k.hs, p.k.ld, j0, __builtin_amdgcn_ballot_w64(use), dz * p.scale, acc);
+        add_rows<D>(p.k.p + b * p.k.bs + hk * p.k.hs, p.k.ld, j0, __builtin_amdgcn_ballot_w64(use), dz * p.dscale, acc);
     }
     store_row<D>(p.dq.p + b * p.dq.bs + i * p.dq.ld + h * p.dq.hs, acc);
 }
@@ -373,7 +380,7 @@ PF_DEVICE void exact_dkv(const RArgs& p, int b, int hk, int j) {
             float P = 0.f, dz = 0.f;
             if (use) use = exact_pair<D>(p, b, h, hk, i, j, P, dz);
             const unsigned long long m = __builtin_amdgcn_ballot_w64(use);
-            add_rows<D>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, i0, m, dz * p.scale, ak);
+            add_rows<D>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, i0, m, dz * p.dscale, ak);
             add_rows<D>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, i0, m, P, av);
         }
     store_row<D>(p.dk.p + b * p.dk.bs + j * p.dk.ld + hk * p.dk.hs, ak);
@@ -409,22 +416,20 @@ PF_DEVICE void load_table(const RArgs& p, int h, float* tab) {
     for (int i = threadIdx.x; i < 2 * p.R + 1; i += 256) tab[i] = bias2(p.bias[(long long)h * (2 * p.R + 1) + i]);
 }
 
-// raw products -> base-2 scores with cap and bias; rel0 = key of register 0 minus the row's position (keys in registers)
+// products -> x (see RArgs), or with a bias -> scores; rel0 = key of register 0 minus the row's position (keys in registers)
 template <int MODE>
 PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        float slope, t;
-        if (MODE & 1) t = capped<(MODE & 4) != 0>(p, s[r], slope);
-        else t = s[r] * p.zs;
-        if (MODE & 2) t += tab[min(max(rel0 + reg_row(r), -p.R), p.R) + p.R];
-        s[r] = t;
+        float slope;
+        s[r] = capped<MODE>(p, s[r], slope);
+        if (MODE & 2) s[r] = __builtin_fmaf(s[r], p.zs, tab[min(max(rel0 + reg_row(r), -p.R), p.R) + p.R]);
     }
 }
 
 // ---------------------------------------------------------------------------------------------- forward, many rows
 // One workgroup = 128 rows of one head, 4 waves x 32; key tiles of KB, two in flight.  MODE bits: 1 cap, 2 bias (scores are
-// formed in base 2 before the maximum; neither: they stay raw and the exponent's multiply-add scales them), 4 SERIES.
+// formed before the maximum; without one the exponent's multiply-add scales them), 4 SERIES.
 //
 // Bound: vector issue (per 32 rows x 64 keys 512 cycles of matrix pipe at D = 64 against 32 multiply-adds, 32 exponentials at
 // 8 cycles, 32 adds, 16 conversions).  So the first pass keeps no running maximum: a row's reference is the maximum of the first
@@ -433,7 +438,7 @@ PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0)
 // (CAREFUL), and rows that are still non-finite and had hidden keys are recomputed from their visible keys (exact_o).
 template <int D, int MODE>
 __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
-    constexpr bool BIAS = MODE & 2, EX = MODE != 0;
+    constexpr bool BIAS = MODE & 2;
     constexpr int KB = FWD_KB<D>, NI = KB / 32, TILE = KB * 2 * D, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     int* const redo_flag = (int*)(smem + 2 * BUF);
@@ -470,7 +475,7 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
     };
     auto pass = [&](auto careful) {
         constexpr bool CAREFUL = decltype(careful)::value;
-        const float zs = EX ? 1.f : p.zs;
+        const float zs = BIAS ? 1.f : p.zs;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) o[c] = zero16();
         m = -__builtin_inff();
@@ -497,7 +502,7 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) s[i] = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s[i]);
             }
-            if (EX) {
+            if (MODE != 0) {
 #pragma unroll
                 for (int i = 0; i < NI; ++i) cap_bias<MODE>(p, s[i], tab, j0 + 32 * i + 4 * hi - pos);
             }
@@ -561,12 +566,12 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
     const bool mine = (redo >> (lane & 31)) & 1;
     if (row < p.Lq) {
         if (!mine) store_cols<D>(p.o.p + b * p.o.bs + row * p.o.ld + h * p.o.hs, o, inv);
-        if (p.lse && hi == 0) p.lse[((long long)b * p.H + h) * p.Lq + row] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+        if (p.lse && hi == 0) p.lse[((long long)b * p.H + h) * p.Lq + row] = l == 0.f ? -__builtin_inff() : (m + p.shift + __builtin_amdgcn_logf(l)) * LN2;
     }
     while (redo) {
         const int i = __builtin_ctzll(redo);
         redo &= redo - 1;
-        exact_o<D>(p, b, h, qt * 128 + wid * 32 + i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), i)),
+        exact_o<D>(p, b, h, qt * 128 + wid * 32 + i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), i)) + p.shift,
                    __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), i)));
     }
 }
@@ -577,7 +582,7 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
 // current one is used.  nsplit > 1: parts go to the workspace, range_join_kernel adds them.
 template <int D, int MODE>
 __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
-    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
     constexpr int TILE = 32 * 2 * D, BUF = 2 * TILE, WAVE = 2 * BUF, NP = 2 * 32 / (512 / D);
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -636,9 +641,8 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
         const int k0 = j0 + 4 * hi;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            float slope, t;
-            if (CAP) t = capped<(MODE & 4) != 0>(p, s[r], slope);
-            else t = s[r] * p.zs;
+            float slope;
+            float t = capped<MODE>(p, s[r], slope) * p.zs;
             if (BIAS) t += bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]);
             s[r] = sees(vis, k0 + reg_row(r)) ? t : -__builtin_inff();
         }
@@ -713,14 +717,14 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) bad = bad || !(fabsf(v[c]) < __builtin_inff());
         if (__builtin_amdgcn_ballot_w64(bad) != 0 && ll == ll) {
-            exact_o<D>(p, b, hh, i, mm, ll);
+            exact_o<D>(p, b, hh, i, mm + p.shift, ll);
         } else {
             const float inv = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) v[c] *= inv;
             store_row<D>(p.o.p + b * p.o.bs + i * p.o.ld + hh * p.o.hs, v);
         }
-        if (p.lse && lane == 0) p.lse[((long long)b * p.H + hh) * p.Lq + i] = ll == 0.f ? -__builtin_inff() : (mm + __builtin_amdgcn_logf(ll)) * LN2;
+        if (p.lse && lane == 0) p.lse[((long long)b * p.H + hh) * p.Lq + i] = ll == 0.f ? -__builtin_inff() : (mm + p.shift + __builtin_amdgcn_logf(ll)) * LN2;
     }
 }
 
@@ -753,19 +757,19 @@ __global__ __launch_bounds__(256) void range_join_kernel(const RArgs p) {
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) bad = bad || !(fabsf(v[c]) < __builtin_inff());
     if (__builtin_amdgcn_ballot_w64(bad) != 0 && l == l) {
-        exact_o<D>(p, b, h, i, m, l);
+        exact_o<D>(p, b, h, i, m + p.shift, l);
     } else {
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) v[c] *= inv;
         store_row<D>(p.o.p + b * p.o.bs + i * p.o.ld + h * p.o.hs, v);
     }
-    if (p.lse && lane == 0) p.lse[((long long)b * p.H + h) * p.Lq + i] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (p.lse && lane == 0) p.lse[((long long)b * p.H + h) * p.Lq + i] = l == 0.f ? -__builtin_inff() : (m + p.shift + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 // ---------------------------------------------------------------------------------------------- backward
-// What both gradient kernels need of a row, in 1-KiB pieces of 64 rows that the LDS-DMA can take as they are: log-sum-exp (base 2)
-// and -delta = -sum_c dO O per head, the ranges per batch entry; and for each such tile the bounds of its ranges: 0..3 the smallest
+// What both gradient kernels need of a row, in 1-KiB pieces of 64 rows that the LDS-DMA can take as they are: log-sum-exp (base 2,
+// less the scores' shift) and -delta = -sum_c dO O per head, the ranges per batch entry; and for each such tile the bounds of its ranges: 0..3 the smallest
 // start and largest end of the a and b ranges that are not empty, 4..7 the largest start and smallest end over ALL its rows.
 template <int D>
 __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
@@ -781,7 +785,7 @@ __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
     s += __shfl_xor(s, 2);
     float* st = p.stat + (((long long)b * p.H + h) * p.nq64 + qt) * 256 + r;
     const bool on = row < p.Lq;
-    if (sub == 0) st[0] = on ? p.lse[((long long)b * p.H + h) * p.Lq + row] * LOG2E : 0.f;
+    if (sub == 0) st[0] = on ? p.lse[((long long)b * p.H + h) * p.Lq + row] * LOG2E - p.shift : 0.f;
     if (sub == 1) st[64] = on ? -s : 0.f;
     if (sub == 2) ((int*)st)[128] = on ? row_pos(p, b, row) : 0;
     if (sub == 3) st[192] = 0.f;
@@ -811,7 +815,7 @@ __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
 // 64-row tiles one wave per SIMD ran everything in series, 8400 cycles per tile, 800 of its instructions register moves).
 template <int D, int MODE>
 __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
-    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0, VLDS = D == 128;
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, VLDS = D == 128;
     constexpr int RT = D == 64 ? 64 : 32, HALVES = 64 / RT, TILE = RT * 2 * D, BUF = 2 * TILE + 2048, VTILE = VLDS ? 32 * 2 * D : 0;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -939,27 +943,21 @@ __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
                 for (int q4 = 0; q4 < 4; ++q4) {
                     const int r0 = qb * 32 + 8 * q4 + 4 * hi;
                     const f32x4_t ls = *(const f32x4_t*)(st + r0);
-                    if (EX) {
-                        const u32x4_t pos = *(const u32x4_t*)((const int*)st + 128 + r0);
+                    u32x4_t pos;
+                    if (BIAS) pos = *(const u32x4_t*)((const int*)st + 128 + r0);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int r = 4 * q4 + e;
-                            float z, fac = 1.f;
-                            if (CAP) z = capped<(MODE & 4) != 0>(p, s[r], fac);
-                            else z = s[r] * p.zs;
-                            if (BIAS) z += tab[min(max(key - (int)pos[e], -p.R), p.R) + p.R];
-                            const bool ok = z != -__builtin_inff();
-                            const float P = __builtin_amdgcn_exp2f(z - ls[e]);
-                            s[r] = ok ? P : 0.f;
-                            dp[r] = ok ? P * dp[r] * fac : 0.f;
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * q4 + e;
+                        float slope;
+                        float x = capped<MODE>(p, s[r], slope);
+                        if (BIAS) {
+                            x = __builtin_fmaf(x, p.zs, tab[min(max(key - (int)pos[e], -p.R), p.R) + p.R]);
+                            s[r] = x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - ls[e]);
+                        } else {
+                            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.zs, -ls[e]));
                         }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int r = 4 * q4 + e;
-                            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls[e]));
-                            dp[r] *= s[r];
-                        }
+                        dp[r] *= s[r];
+                        if (CAP) dp[r] *= slope;
                     }
                 }
                 if (!cur.full) {
@@ -1009,7 +1007,7 @@ __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
     redo = (redo | (redo >> 32)) & 0xffffffffull;
     if (key < p.Lk && !((redo >> (lane & 31)) & 1)) {
-        store_cols<D>(p.dk.p + b * p.dk.bs + key * p.dk.ld + hk * p.dk.hs, dk, p.scale);
+        store_cols<D>(p.dk.p + b * p.dk.bs + key * p.dk.ld + hk * p.dk.hs, dk, p.dscale);
         store_cols<D>(p.dv.p + b * p.dv.bs + key * p.dv.ld + hk * p.dv.hs, dv, 1.f);
     }
     while (redo) {
@@ -1036,7 +1034,7 @@ __global__ __launch_bounds__(256) void range_kvjoin_kernel(const RArgs p) {
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
         bad = bad || !(fabsf(k[c]) < __builtin_inff()) || !(fabsf(v[c]) < __builtin_inff());
-        k[c] *= p.scale;
+        k[c] *= p.dscale;
     }
     if (__builtin_amdgcn_ballot_w64(bad) != 0) {
         exact_dkv<D>(p, b, hk, j);
@@ -1086,7 +1084,7 @@ PF_DEVICE void add_diagonals(const f32x16_t& dt, float* skew, float* hist, int R
 // order.
 template <int D, int MODE>
 __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
-    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, EX = MODE != 0;
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
     constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     float* const tab = (float*)(smem + 2 * BUF);
@@ -1166,19 +1164,14 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
             f32x16_t fac;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                if (EX) {
-                    float z, slope;
-                    if (CAP) {
-                        z = capped<(MODE & 4) != 0>(p, s[r], slope);
-                        fac[r] = slope;
-                    } else {
-                        z = s[r] * p.zs;
-                    }
-                    if (BIAS) z += tab[min(max(k0 + reg_row(r) - pos, -p.R), p.R) + p.R];
-                    const float dt = __builtin_amdgcn_exp2f(z - ls) * dp[r];
-                    s[r] = z != -__builtin_inff() ? dt : 0.f;
+                float slope;
+                float x = capped<MODE>(p, s[r], slope);
+                if (CAP) fac[r] = slope;
+                if (BIAS) {
+                    x = __builtin_fmaf(x, p.zs, tab[min(max(k0 + reg_row(r) - pos, -p.R), p.R) + p.R]);
+                    s[r] = x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - ls) * dp[r];
                 } else {
-                    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls)) * dp[r];
+                    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.zs, -ls)) * dp[r];
                 }
             }
             if (!full) {
@@ -1220,7 +1213,7 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     const bool bad = any_nonfinite<D / 32>(dq) && !whole && row < p.Lq;
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
     redo = (redo | (redo >> 32)) & 0xffffffffull;
-    if (row < p.Lq && !((redo >> (lane & 31)) & 1)) store_cols<D>(p.dq.p + b * p.dq.bs + row * p.dq.ld + h * p.dq.hs, dq, p.scale);
+    if (row < p.Lq && !((redo >> (lane & 31)) & 1)) store_cols<D>(p.dq.p + b * p.dq.bs + row * p.dq.ld + h * p.dq.hs, dq, p.dscale);
     while (redo) {
         const int i = __builtin_ctzll(redo);
         redo &= redo - 1;
@@ -1303,7 +1296,7 @@ long long up16(long long n) { return (n + 15) / 16 * 16; }
 int kv_splits(const pf_attn_ranges_desc* d) {
     if (!d->B || !d->H || !d->Lk || !d->Lq) return 1;
     const long long units = (long long)((d->Lk + 127) / 128) * d->Hkv * d->B, tiles = (long long)((d->Lq + 63) / 64) * (d->H / d->Hkv);
-    long long n = 768 / units;
+    long long n = 1024 / units;
     if (n > tiles / 4) n = tiles / 4;
     if (n > 16) n = 16;
     return (int)(n < 1 ? 1 : n);
@@ -1332,7 +1325,11 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
     a.scale = d->scale;
     a.cap2 = d->cap * LOG2E;
     a.series = d->cap > 64.f;
-    a.zs = d->cap > 0.f ? d->scale / d->cap * (a.series ? 1.f : 2.f * LOG2E) : d->scale * LOG2E;
+    const bool fast = d->cap > 0.f && !a.series;
+    a.zc = d->cap > 0.f ? d->scale / d->cap * (fast ? 2.f * LOG2E : 1.f) : 0.f;
+    a.zs = fast ? 2.f * a.cap2 : a.series ? 1.f : d->scale * LOG2E;
+    a.shift = fast ? a.cap2 : 0.f;
+    a.dscale = fast ? 4.f * d->scale : d->scale;
     a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
     a.nqt = (d->Lq + 127) / 128; a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
     return a;
