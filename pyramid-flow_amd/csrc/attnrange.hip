@@ -174,8 +174,8 @@ PF_DEVICE Bounds wave_bounds(const Vis& v) {
     return {lo(v.na ? v.alo : BIG), hi(v.na ? v.alo + v.na : 0), lo(v.nb ? v.blo : BIG), hi(v.nb ? v.blo + v.nb : 0),
             hi(v.na ? v.alo : BIG), lo(v.na ? v.alo + v.na : 0), hi(v.nb ? v.blo : BIG), lo(v.nb ? v.blo + v.nb : 0)};
 }
-// the key tiles of a workgroup of 4 waves (`red`: 16 ints of LDS, read behind a barrier)
-template <int KB>
+// the key tiles of a workgroup of NW waves (`red`: 4 NW ints of LDS, read behind a barrier)
+template <int KB, int NW>
 PF_DEVICE TileList workgroup_tiles(const Bounds& w, int* red, int wid, int lane) {
     if (lane == 0) { red[4 * wid] = w.amin; red[4 * wid + 1] = w.amax; red[4 * wid + 2] = w.bmin; red[4 * wid + 3] = w.bmax; }
     __syncthreads();
@@ -184,7 +184,7 @@ PF_DEVICE TileList workgroup_tiles(const Bounds& w, int* red, int wid, int lane)
     for (int i = 0; i < 4; ++i) {
         x[i] = red[i];
 #pragma unroll
-        for (int u = 1; u < 4; ++u) x[i] = (i & 1) ? max(x[i], red[4 * u + i]) : min(x[i], red[4 * u + i]);
+        for (int u = 1; u < NW; ++u) x[i] = (i & 1) ? max(x[i], red[4 * u + i]) : min(x[i], red[4 * u + i]);
         x[i] = __builtin_amdgcn_readfirstlane(x[i]);
     }
     return tile_list<KB>(x[0], x[1], x[2], x[3]);
@@ -412,8 +412,9 @@ PF_DEVICE bool any_nonfinite(const f32x16_t* o) {
 }
 
 // the bias table of head h in LDS, base 2
+template <int NW>
 PF_DEVICE void load_table(const RArgs& p, int h, float* tab) {
-    for (int i = threadIdx.x; i < 2 * p.R + 1; i += 256) tab[i] = bias2(p.bias[(long long)h * (2 * p.R + 1) + i]);
+    for (int i = threadIdx.x; i < 2 * p.R + 1; i += 64 * NW) tab[i] = bias2(p.bias[(long long)h * (2 * p.R + 1) + i]);
 }
 
 // products -> x (see RArgs), or with a bias -> scores; rel0 = key of register 0 minus the row's position (keys in registers)
@@ -427,8 +428,23 @@ PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0)
     }
 }
 
+// Which (head, tile) a workgroup takes.  Every XCD has a contiguous run of heads (their K and V stay in its L2), walks the first
+// half of each head's tiles -- the ones that causal and frame-wise masks make long -- for all of its heads and then the second
+// halves: the launch ends on short workgroups.  Tile numbers here count from the heavy end.  (Head after head instead: 1415, now
+// 1308 us for 30 heads of the 15488-row video sequence; 1500, now 1333 us for the gradients at 7808 rows.)
+PF_DEVICE int heavy_first(int block, int n, int nwg) {
+    const int q = nwg >> 3, r = nwg & 7, xcd = block & 7, i = block >> 3;
+    const int c0 = xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q, c1 = c0 + q + (xcd < r ? 1 : 0);
+    const int nh = (n + 1) / 2, nl = n - nh;
+    auto heavy_below = [&](int c) { return c / n * nh + min(c % n, nh); };
+    const int h0 = heavy_below(c0), hn = heavy_below(c1) - h0;
+    if (i < hn) return (h0 + i) / nh * n + (h0 + i) % nh;
+    const int k = (c0 - h0) + (i - hn);
+    return k / nl * n + nh + k % nl;
+}
+
 // ---------------------------------------------------------------------------------------------- forward, many rows
-// One workgroup = 128 rows of one head, 4 waves x 32; key tiles of KB, two in flight.  MODE bits: 1 cap, 2 bias (scores are
+// One workgroup = NW waves x 32 rows of one head; key tiles of KB, two in flight.  MODE bits: 1 cap, 2 bias (scores are
 // formed before the maximum; without one the exponent's multiply-add scales them), 4 SERIES.
 //
 // Bound: vector issue (per 32 rows x 64 keys 512 cycles of matrix pipe at D = 64 against 32 multiply-adds, 32 exponentials at
@@ -436,27 +452,27 @@ PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0)
 // tile in which it sees a key; a weight may then grow to 2^127 before anything overflows and its rounding to bf16 is relative,
 // so the result is the same.  If a sum or a result of the workgroup came out non-finite, it runs again with the running maximum
 // (CAREFUL), and rows that are still non-finite and had hidden keys are recomputed from their visible keys (exact_o).
-template <int D, int MODE>
-__global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
+template <int D, int MODE, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void range_fwd_kernel(const RArgs p) {
     constexpr bool BIAS = MODE & 2;
     constexpr int KB = FWD_KB<D>, NI = KB / 32, TILE = KB * 2 * D, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     int* const redo_flag = (int*)(smem + 2 * BUF);
     float* const tab = (float*)(smem + 2 * BUF + 16);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = xcd_remap(blockIdx.x, p.nqt * p.H * p.B);
+    const int t = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
     const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
-    const int hi = lane >> 5, row = qt * 128 + wid * 32 + (lane & 31);
+    const int hi = lane >> 5, row0 = (qt * NW + wid) * 32, row = row0 + (lane & 31);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
     const Bounds wb = wave_bounds(vis);
-    if (BIAS) load_table(p, h, tab);
+    if (BIAS) load_table<NW>(p, h, tab);
     if (threadIdx.x == 0) *redo_flag = 0;
-    const TileList tl = workgroup_tiles<KB>(wb, (int*)smem, wid, lane);
+    const TileList tl = workgroup_tiles<KB, NW>(wb, (int*)smem, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
-    const Stager<D, KB, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
+    const Stager<D, KB, NW> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
     bf16x8_t qf[D / 16];
     {
         const bf16_t* q = p.q.p + b * p.q.bs + (long long)min(row, p.Lq - 1) * p.q.ld + h * p.q.hs + hi * 8;
@@ -571,7 +587,7 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
     while (redo) {
         const int i = __builtin_ctzll(redo);
         redo &= redo - 1;
-        exact_o<D>(p, b, h, qt * 128 + wid * 32 + i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), i)) + p.shift,
+        exact_o<D>(p, b, h, row0 + i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), i)) + p.shift,
                    __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), i)));
     }
 }
@@ -821,7 +837,7 @@ __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     char* const vtile = smem + 2 * BUF + wid * VTILE;
     float* const tab = (float*)(smem + 2 * BUF + 4 * VTILE);
-    const int t = xcd_remap(blockIdx.x, p.nkt * p.kv_split * p.Hk * p.B);
+    const int t = heavy_first(blockIdx.x, p.nkt * p.kv_split, p.nkt * p.kv_split * p.Hk * p.B);
     const int unit = t / p.kv_split, part = t - unit * p.kv_split;
     const int bk = unit / p.nkt, kt = unit - bk * p.nkt;
     const int b = bk / p.Hk, hk = bk - b * p.Hk;
@@ -915,7 +931,7 @@ __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
         drain_barrier();
         if (BIAS && cur.g != table_of) {                            // uniform: another head, another bias table
             table_of = cur.g;
-            load_table(p, hk * p.G + table_of, tab);
+            load_table<4>(p, hk * p.G + table_of, tab);
             drain_barrier();
         }
         const Item nxt = follow(cur);
@@ -1078,12 +1094,11 @@ PF_DEVICE void add_diagonals(const f32x16_t& dt, float* skew, float* hist, int R
     }
 }
 
-// dQ of 128 rows of one head (4 waves x 32 rows held in registers) over its key tiles, and this workgroup's part of dbias: every
+// dQ of NW x 32 rows of one head (a wave's 32 rows held in registers) over its key tiles, and this workgroup's part of dbias: every
 // wave adds dT of its pairs into a table of its own (by diagonals, or pair by pair where positions are not consecutive: LDS adds
-// of one wave run in program order; pairs behind the table's ends are summed in registers), the four tables are added in wave
-// order.
-template <int D, int MODE>
-__global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
+// of one wave run in program order; pairs behind the table's ends are summed in registers), the tables are added in wave order.
+template <int D, int MODE, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void range_dq_kernel(const RArgs p) {
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
     constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -1091,23 +1106,23 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     const int NB = 2 * p.R + 1;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* const hist = tab + NB + wid * NB;
-    float* const skew = tab + (5 * NB + 3) / 4 * 4 + wid * SKEW;
-    const int t = xcd_remap(blockIdx.x, p.nqt * p.H * p.B);
+    float* const skew = tab + ((NW + 1) * NB + 3) / 4 * 4 + wid * SKEW;
+    const int t = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
     const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
-    const int hi = lane >> 5, row = qt * 128 + wid * 32 + (lane & 31), rc = min(row, p.Lq - 1);
+    const int hi = lane >> 5, row0 = (qt * NW + wid) * 32, row = row0 + (lane & 31), rc = min(row, p.Lq - 1);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, rc) : 0;
     const Bounds wb = wave_bounds(vis);
     if (BIAS) {
-        load_table(p, h, tab);
+        load_table<NW>(p, h, tab);
         if (p.dbias) {
             for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
             for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
         }
     }
-    const TileList tl = workgroup_tiles<64>(wb, (int*)smem, wid, lane);
-    const Stager<D, 64, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
+    const TileList tl = workgroup_tiles<64, NW>(wb, (int*)smem, wid, lane);
+    const Stager<D, 64, NW> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
     bf16x8_t qf[D / 16], of[D / 16];
@@ -1217,7 +1232,7 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     while (redo) {
         const int i = __builtin_ctzll(redo);
         redo &= redo - 1;
-        exact_dq<D>(p, b, h, qt * 128 + wid * 32 + i);
+        exact_dq<D>(p, b, h, row0 + i);
     }
     if (BIAS && p.dbias) {
         below = wave_add(below);
@@ -1228,7 +1243,12 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
         }
         __syncthreads();
         float* out = p.dbias_parts + ((long long)bh * p.nqt + qt) * NB;
-        for (int i = threadIdx.x; i < NB; i += 256) out[i] = (tab[NB + i] + tab[2 * NB + i]) + (tab[3 * NB + i] + tab[4 * NB + i]);
+        for (int i = threadIdx.x; i < NB; i += 64 * NW) {
+            float a = tab[NB + i];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) a += tab[(w + 1) * NB + i];
+            out[i] = a;
+        }
     }
 }
 
@@ -1278,6 +1298,11 @@ const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
 bool few_rows(const pf_attn_ranges_desc* d) {
     return (long long)((d->Lq + 127) / 128) * d->H * d->B < 256 || (long long)d->Lq * (d->H / d->Hkv) <= 32;
 }
+// 64-row instead of 128-row workgroups where a head_dim-64 problem has fewer than four of the latter per compute unit: 24.4 instead
+// of 27.6 us for 2 x 64 heads of 512 rows; 1670 instead of 1415 us for 30 heads of 15488.  At head_dim 128 the tiles of the
+// smaller workgroups take the LDS that a third one needs: slower at every size measured.
+bool small_groups(int D, long long Lq, long long H, long long B) { return D == 64 && (Lq + 127) / 128 * H * B < 1024; }
+int row_groups(const pf_attn_ranges_desc* d) { return small_groups(d->D, d->Lq, d->H, d->B) ? (d->Lq + 63) / 64 : (d->Lq + 127) / 128; }
 int mode(const pf_attn_ranges_desc* d) { return (d->cap > 64.f ? 5 : (d->cap > 0.f ? 1 : 0)) + (d->bias ? 2 : 0); }
 int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * (d->H / d->Hkv) + 31) / 32); }
 int splits(const pf_attn_ranges_desc* d) {
@@ -1308,7 +1333,7 @@ BwdSizes bwd_sizes(const pf_attn_ranges_desc* d) {
     s.stat = (long long)d->B * d->H * nq * 1024;
     s.vis = (long long)d->B * nq * 1024;
     s.tiles = up16((long long)d->B * nq * 32);
-    s.parts = d->dbias ? up16((long long)d->B * d->H * ((d->Lq + 127) / 128) * (2 * d->bias_radius + 1) * 4) : 0;
+    s.parts = d->dbias ? up16((long long)d->B * d->H * row_groups(d) * (2 * d->bias_radius + 1) * 4) : 0;
     const int n = kv_splits(d);
     s.kv = n > 1 ? (long long)n * d->B * d->Hkv * d->Lk * 2 * d->D * 4 : 0;
     return s;
@@ -1331,7 +1356,7 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
     a.shift = fast ? a.cap2 : 0.f;
     a.dscale = fast ? 4.f * d->scale : d->scale;
     a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
-    a.nqt = (d->Lq + 127) / 128; a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
+    a.nqt = row_groups(d); a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
     return a;
 }
 
@@ -1341,14 +1366,21 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
         if (e_ != hipSuccess) return pf_set_err(hipGetErrorString(e_)); \
     } while (0)
 
+template <int D, int MODE, int NW>
+int launch_fwd_rows(const RArgs& a, hipStream_t stream) {
+    const size_t lds = 4 * FWD_KB<D> * 2 * D + 16 + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
+    PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, MODE, NW>), (int)lds);
+    range_fwd_kernel<D, MODE, NW><<<(unsigned)(a.nqt * a.H * a.B), 64 * NW, lds, stream>>>(a);
+    CHECK_LAUNCH();
+    return 0;
+}
+
 template <int D, int MODE>
 int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
     if (!few) {
-        const size_t lds = 4 * FWD_KB<D> * 2 * D + 16 + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
-        PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, MODE>), (int)lds);
-        range_fwd_kernel<D, MODE><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
-        CHECK_LAUNCH();
-        return 0;
+        if constexpr (D == 64)
+            if (small_groups(D, a.Lq, a.H, a.B)) return launch_fwd_rows<D, MODE, 2>(a, stream);
+        return launch_fwd_rows<D, MODE, 4>(a, stream);
     }
     const size_t lds = 4 * 4 * 32 * 2 * D;                           // the meeting area [4][32][D + 4] fp32 is smaller
     PF_SET_MAX_LDS_ONCE((range_split_kernel<D, MODE>), (int)lds);
@@ -1359,6 +1391,15 @@ int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
         range_join_kernel<D><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(a);
         CHECK_LAUNCH();
     }
+    return 0;
+}
+
+template <int D, int MODE, int NW>
+int launch_dq(const RArgs& a, hipStream_t stream) {
+    auto lds = [](int R) { return 4 * 64 * 2 * D + (MODE & 2 ? (NW + 1) * (2 * R + 1) * 4 + 12 + NW * SKEW * 4 : 0); };
+    PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE, NW>), lds(MAX_RADIUS));
+    range_dq_kernel<D, MODE, NW><<<(unsigned)(a.nqt * a.H * a.B), 64 * NW, (size_t)lds(a.R), stream>>>(a);
+    CHECK_LAUNCH();
     return 0;
 }
 
@@ -1380,10 +1421,9 @@ int launch_bwd(const RArgs& a, hipStream_t stream) {
         }
     }
     if (a.Lq > 0) {
-        const size_t lds = 4 * 64 * 2 * D + (MODE & 2 ? 5 * (2 * a.R + 1) * 4 + 12 + 4 * SKEW * 4 : 0);
-        PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE>), 4 * 64 * 2 * D + (MODE & 2 ? 5 * (2 * MAX_RADIUS + 1) * 4 + 12 + 4 * SKEW * 4 : 0));
-        range_dq_kernel<D, MODE><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
-        CHECK_LAUNCH();
+        if constexpr (D == 64)
+            if (small_groups(D, a.Lq, a.H, a.B)) return launch_dq<D, MODE, 2>(a, stream);
+        return launch_dq<D, MODE, 4>(a, stream);
     }
     return 0;
 }
