@@ -44,10 +44,10 @@ struct RArgs {
     float zs, zc, shift, cap2;
     float scale, dscale;               // dQ, dK = dscale times the products of dZ (4 scale with cap_u's slope)
     int series;
-    int B, H, Hk, G, Lq, Lk;
+    int D, B, H, Hk, G, Lq, Lk;
     int nqt, nkt, nrb, nsplit;
     float* parts;                      // split forward: [unit][split][32][D + 2]
-    float* stat;                       // backward: [B][H][nq64][4][64] lse log2 e, -delta, position, 0
+    float* stat;                       // backward: [B][H][nq64][4][64] lse log2 e - shift, -delta, position, the tile's positions
     int* vis;                          // backward: [B][nq64][4][64] the rows' ranges (Vis)
     int* tiles;                        // backward: [B][nq64][8] bounds of 64-row tiles
     int nq64;
@@ -115,8 +115,8 @@ PF_DEVICE TileList tile_list(int amin, int amax, int bmin, int bmax) {
     return {as, ae - as, bs, (ae - as) + (be - bs)};
 }
 
-template <int D>
-constexpr int FWD_KB = D == 64 ? 64 : 32;     // keys of a forward tile
+template <int D, int KS>
+constexpr int FWD_KB = D == 64 || KS == 2 ? 64 : 32;     // keys of a forward tile
 
 // ---------------------------------------------------------------------------------------------- LDS tiles
 // Row-major bf16 rows of D channels, 16-byte chunk c of row r at c ^ swz(r).  A row read (ds_read_b128, one chunk of 16
@@ -174,8 +174,8 @@ PF_DEVICE Bounds wave_bounds(const Vis& v) {
     return {lo(v.na ? v.alo : BIG), hi(v.na ? v.alo + v.na : 0), lo(v.nb ? v.blo : BIG), hi(v.nb ? v.blo + v.nb : 0),
             hi(v.na ? v.alo : BIG), lo(v.na ? v.alo + v.na : 0), hi(v.nb ? v.blo : BIG), lo(v.nb ? v.blo + v.nb : 0)};
 }
-// the key tiles of a workgroup of NW waves (`red`: 4 NW ints of LDS, read behind a barrier)
-template <int KB, int NW>
+// the key tiles of a workgroup of 4 waves (`red`: 16 ints of LDS, read behind a barrier)
+template <int KB>
 PF_DEVICE TileList workgroup_tiles(const Bounds& w, int* red, int wid, int lane) {
     if (lane == 0) { red[4 * wid] = w.amin; red[4 * wid + 1] = w.amax; red[4 * wid + 2] = w.bmin; red[4 * wid + 3] = w.bmax; }
     __syncthreads();
@@ -184,7 +184,7 @@ PF_DEVICE TileList workgroup_tiles(const Bounds& w, int* red, int wid, int lane)
     for (int i = 0; i < 4; ++i) {
         x[i] = red[i];
 #pragma unroll
-        for (int u = 1; u < NW; ++u) x[i] = (i & 1) ? max(x[i], red[4 * u + i]) : min(x[i], red[4 * u + i]);
+        for (int u = 1; u < 4; ++u) x[i] = (i & 1) ? max(x[i], red[4 * u + i]) : min(x[i], red[4 * u + i]);
         x[i] = __builtin_amdgcn_readfirstlane(x[i]);
     }
     return tile_list<KB>(x[0], x[1], x[2], x[3]);
@@ -279,7 +279,8 @@ PF_DEVICE float score2(const RArgs& p, float z, int h, int dist, float& slope) {
     const float t = __builtin_fmaf(x, p.zs, p.shift);
     return p.bias ? t + bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(dist, -p.R), p.R) + p.R]) : t;
 }
-PF_DEVICE int row_pos(const RArgs& p, int b, int row) { return p.q_pos ? p.q_pos[b * p.pos_bs + row] : row + p.Lk - p.Lq; }
+// positions in front of every key by more than any radius count alike: differences stay inside 32 bits
+PF_DEVICE int row_pos(const RArgs& p, int b, int row) { return p.q_pos ? max(p.q_pos[b * p.pos_bs + row], 4096 - (1 << 30)) : row + p.Lk - p.Lq; }
 
 template <int D>
 PF_DEVICE float dot_row(const bf16_t* a, const bf16_t* b) {
@@ -411,20 +412,48 @@ PF_DEVICE bool any_nonfinite(const f32x16_t* o) {
     return t != t;
 }
 
-// the bias table of head h in LDS, base 2
-template <int NW>
-PF_DEVICE void load_table(const RArgs& p, int h, float* tab) {
-    for (int i = threadIdx.x; i < 2 * p.R + 1; i += 64 * NW) tab[i] = bias2(p.bias[(long long)h * (2 * p.R + 1) + i]);
+// The bias table of head h in LDS, base 2, continued by PAD entries of its end values on both sides: a 32 x 64 block of consecutive
+// rows whose distances are not all behind an end stays inside it, so its entries lie at fixed offsets from one address per
+// lane (a subtraction, a clamp and an address per score otherwise).  Returned: the entry of distance 0.
+constexpr int PAD = 96;
+constexpr int table_floats(int R) { return 2 * R + 1 + 2 * PAD; }
+PF_DEVICE const float* load_table(const RArgs& p, int h, float* tab) {
+    for (int i = threadIdx.x; i < table_floats(p.R); i += 256)
+        tab[i] = bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(i - PAD, 0), 2 * p.R)]);
+    return tab + PAD + p.R;
+}
+// how a block with distances lo .. hi (wave-uniform) reads it
+enum Reach { NEAR, FAR, MIXED };
+PF_DEVICE Reach reach(int R, int lo, int hi) {
+    return (hi <= -R || lo >= R) ? FAR : (lo >= -R - PAD && hi <= R + PAD) ? NEAR : MIXED;
 }
 
-// products -> x (see RArgs), or with a bias -> scores; rel0 = key of register 0 minus the row's position (keys in registers)
+// products -> x (see RArgs)
 template <int MODE>
-PF_DEVICE void cap_bias(const RArgs& p, f32x16_t& s, const float* tab, int rel0) {
+PF_DEVICE void cap_only(const RArgs& p, f32x16_t& s) {
+    if constexpr ((MODE & 1) != 0) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        float slope;
-        s[r] = capped<MODE>(p, s[r], slope);
-        if (MODE & 2) s[r] = __builtin_fmaf(s[r], p.zs, tab[min(max(rel0 + reg_row(r), -p.R), p.R) + p.R]);
+        for (int r = 0; r < 16; ++r) {
+            float slope;
+            s[r] = capped<MODE>(p, s[r], slope);
+        }
+    }
+}
+// x -> score with the bias; d0 = distance of this lane's register 0 (SIGN 1: registers are keys, -1: rows), lo, hi = of the block
+template <int SIGN>
+PF_DEVICE void add_bias(const RArgs& p, f32x16_t& s, const float* tab, int d0, int lo, int hi) {
+    const Reach how = reach(p.R, lo, hi);
+    if (how == NEAR) {
+        const float* at = tab + d0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.zs, at[SIGN * reg_row(r)]);
+    } else if (how == FAR) {
+        const float c = tab[hi <= -p.R ? -p.R : p.R];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.zs, c);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.zs, tab[min(max(d0 + SIGN * reg_row(r), -p.R), p.R)]);
     }
 }
 
@@ -444,35 +473,38 @@ PF_DEVICE int heavy_first(int block, int n, int nwg) {
 }
 
 // ---------------------------------------------------------------------------------------------- forward, many rows
-// One workgroup = NW waves x 32 rows of one head; key tiles of KB, two in flight.  MODE bits: 1 cap, 2 bias (scores are
-// formed before the maximum; without one the exponent's multiply-add scales them), 4 SERIES.
+// One workgroup of 4 waves = 128 rows of one head, or with KS = 2 64 rows whose two halves of every key tile go to different waves
+// (their results meet in LDS at the end): the shorter chain for problems with few row tiles.  Key tiles of KB, two in flight.
+// MODE bits: 1 cap, 2 bias (scores are formed before the maximum; without one the exponent's multiply-add scales them), 4 SERIES.
 //
 // Bound: vector issue (per 32 rows x 64 keys 512 cycles of matrix pipe at D = 64 against 32 multiply-adds, 32 exponentials at
 // 8 cycles, 32 adds, 16 conversions).  So the first pass keeps no running maximum: a row's reference is the maximum of the first
 // tile in which it sees a key; a weight may then grow to 2^127 before anything overflows and its rounding to bf16 is relative,
 // so the result is the same.  If a sum or a result of the workgroup came out non-finite, it runs again with the running maximum
 // (CAREFUL), and rows that are still non-finite and had hidden keys are recomputed from their visible keys (exact_o).
-template <int D, int MODE, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void range_fwd_kernel(const RArgs p) {
+template <int D, int MODE, int KS>
+__global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
     constexpr bool BIAS = MODE & 2;
-    constexpr int KB = FWD_KB<D>, NI = KB / 32, TILE = KB * 2 * D, BUF = 2 * TILE;
+    constexpr int KB = FWD_KB<D, KS>, NI = KB / 32 / KS, TILE = KB * 2 * D, BUF = 2 * TILE, RW = 4 / KS;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     int* const redo_flag = (int*)(smem + 2 * BUF);
-    float* const tab = (float*)(smem + 2 * BUF + 16);
-    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float* const meet = (float*)(smem + 2 * BUF + 16);              // KS = 2: [row wave][3][64] maximum, sum, whole
+    float* const tab_ = meet + (KS == 2 ? RW * 192 : 0);
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
     const int t = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
     const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
-    const int hi = lane >> 5, row0 = (qt * NW + wid) * 32, row = row0 + (lane & 31);
+    const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
+    const int pmin = BIAS ? __builtin_amdgcn_readfirstlane(wave_min(pos)) : 0, pmax = BIAS ? __builtin_amdgcn_readfirstlane(wave_max(pos)) : 0;
     const Bounds wb = wave_bounds(vis);
-    if (BIAS) load_table<NW>(p, h, tab);
+    const float* const tab = BIAS ? load_table(p, h, tab_) : nullptr;
     if (threadIdx.x == 0) *redo_flag = 0;
-    const TileList tl = workgroup_tiles<KB, NW>(wb, (int*)smem, wid, lane);
+    const TileList tl = workgroup_tiles<KB>(wb, (int*)smem, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
-    const Stager<D, KB, NW> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
+    const Stager<D, KB, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
     bf16x8_t qf[D / 16];
     {
         const bf16_t* q = p.q.p + b * p.q.bs + (long long)min(row, p.Lq - 1) * p.q.ld + h * p.q.hs + hi * 8;
@@ -503,13 +535,13 @@ __global__ __launch_bounds__(64 * NW, 2) void range_fwd_kernel(const RArgs p) {
         for (int n = 0; n < tl.n; ++n) {
             drain_barrier();
             if (n + 1 < tl.n) issue(n + 1);
-            const int j0 = tl.at(n) * KB;
-            const char* sk = smem + (n & 1) * BUF;
+            const int j0 = tl.at(n) * KB + kw * 32 * NI;             // this wave's keys of the tile
+            const char* sk = smem + (n & 1) * BUF + kw * NI * 64 * D;
             const char* sv = sk + TILE;
-            const bool full = wb.full(j0, j0 + KB);
+            const bool full = wb.full(j0, j0 + 32 * NI);
             if (!full) {
                 whole = false;
-                if (!wb.any(j0, j0 + KB)) continue;
+                if (!wb.any(j0, j0 + 32 * NI)) continue;
             }
             f32x16_t s[NI];
 #pragma unroll
@@ -518,9 +550,10 @@ __global__ __launch_bounds__(64 * NW, 2) void range_fwd_kernel(const RArgs p) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) s[i] = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s[i]);
             }
-            if (MODE != 0) {
 #pragma unroll
-                for (int i = 0; i < NI; ++i) cap_bias<MODE>(p, s[i], tab, j0 + 32 * i + 4 * hi - pos);
+            for (int i = 0; i < NI; ++i) {
+                cap_only<MODE>(p, s[i]);
+                if (BIAS) add_bias<1>(p, s[i], tab, j0 + 32 * i + 4 * hi - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
             }
             if (!full) {
 #pragma unroll
@@ -575,6 +608,32 @@ __global__ __launch_bounds__(64 * NW, 2) void range_fwd_kernel(const RArgs p) {
     if (__builtin_amdgcn_ballot_w64(!(l < __builtin_inff()) || any_nonfinite<D / 32>(o)) != 0 && lane == 0) *redo_flag = 1;
     __syncthreads();
     if (*redo_flag != 0) pass(std::true_type{});   // workgroup-uniform: the passes share tiles and barriers
+    if constexpr (KS == 2) {
+        float* const acc = (float*)smem + rw * (D / 32) * 16 * 64;   // the tiles' memory: [row wave][register][lane]
+        __syncthreads();
+        if (kw == 1) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[(c * 16 + r) * 64 + lane] = o[c][r];
+            meet[rw * 192 + lane] = m;
+            meet[rw * 192 + 64 + lane] = l;
+            meet[rw * 192 + 128 + lane] = whole ? 1.f : 0.f;
+        }
+        __syncthreads();
+        if (kw == 1) return;
+        const float m2 = meet[rw * 192 + lane], l2 = meet[rw * 192 + 64 + lane], mm = fmaxf(m, m2);
+        whole = whole && meet[rw * 192 + 128] != 0.f;
+        const bool one = m2 == -__builtin_inff(), two = m == -__builtin_inff();       // only one half saw a key
+        const float f = two ? 0.f : m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm), f2 = one ? 0.f : m2 == mm ? 1.f : __builtin_amdgcn_exp2f(m2 - mm);
+        // a half without a key holds zeros (or 0 x inf of hidden keys, which exact_o sees); a NaN sum has its maximum at -inf
+        l = (two && l == 0.f ? 0.f : two ? l : f * l) + (one ? l2 : f2 * l2);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[c][r] = f * o[c][r] + f2 * acc[(c * 16 + r) * 64 + lane];
+        m = mm;
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const bool bad = any_nonfinite<D / 32>(o) && !whole && l == l && row < p.Lq;
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
@@ -613,6 +672,8 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
     if (!valid) vis.na = vis.nb = 0;
     const int pos = BIAS ? row_pos(p, b, row) : 0;
     const float* const bias = BIAS ? p.bias + (long long)h * (2 * p.R + 1) + p.R : nullptr;
+    const float far_below = BIAS ? bias2(bias[-p.R]) : 0.f, far_above = BIAS ? bias2(bias[p.R]) : 0.f;
+    const int pmin = BIAS ? __builtin_amdgcn_readfirstlane(wave_min(pos)) : 0, pmax = BIAS ? __builtin_amdgcn_readfirstlane(wave_max(pos)) : 0;
     const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
     const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
     const TileList tl = tile_list<32>(__builtin_amdgcn_readfirstlane(amin), __builtin_amdgcn_readfirstlane(amax),
@@ -655,11 +716,13 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) s = mfma(row_frag<D>(sk, roff, 0, ks), qf[ks], s);
         const int k0 = j0 + 4 * hi;
+        // the gather from global memory waits for the tile in flight too: only where the distances are inside the table
+        const bool far = BIAS && reach(p.R, j0 - pmax, j0 + 31 - pmin) == FAR;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float slope;
             float t = capped<MODE>(p, s[r], slope) * p.zs;
-            if (BIAS) t += bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]);
+            if (BIAS) t += far ? (j0 + 31 - pmin <= -p.R ? far_below : far_above) : bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]);
             s[r] = sees(vis, k0 + reg_row(r)) ? t : -__builtin_inff();
         }
         float mt = s[0];
@@ -804,7 +867,13 @@ __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
     if (sub == 0) st[0] = on ? p.lse[((long long)b * p.H + h) * p.Lq + row] * LOG2E - p.shift : 0.f;
     if (sub == 1) st[64] = on ? -s : 0.f;
     if (sub == 2) ((int*)st)[128] = on ? row_pos(p, b, row) : 0;
-    if (sub == 3) st[192] = 0.f;
+    if (threadIdx.x < 64) {                                         // the tile's positions: smallest, largest, whether they follow one another
+        const int at = row_pos(p, b, min(qt * 64 + (int)threadIdx.x, p.Lq - 1)), first = __builtin_amdgcn_readfirstlane(at);
+        const bool line = __builtin_amdgcn_ballot_w64(qt * 64 + (int)threadIdx.x < p.Lq && at != first + (int)threadIdx.x) == 0;
+        const int lo = line ? first : wave_min(at), hi = line ? first + 63 : wave_max(at);
+        int* x = (int*)(p.stat + (((long long)b * p.H + h) * p.nq64 + qt) * 256) + 192;
+        x[threadIdx.x] = threadIdx.x == 0 ? lo : threadIdx.x == 1 ? hi : threadIdx.x == 2 ? (int)line : 0;
+    }
     if (h == 0 && threadIdx.x < 64) {
         const Vis v = load_vis(p, b, qt * 64 + threadIdx.x);
         const long long tile = (long long)b * p.nq64 + qt;
@@ -836,7 +905,8 @@ __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     char* const vtile = smem + 2 * BUF + wid * VTILE;
-    float* const tab = (float*)(smem + 2 * BUF + 4 * VTILE);
+    float* const tab_ = (float*)(smem + 2 * BUF + 4 * VTILE);
+    const float* tab = nullptr;
     const int t = heavy_first(blockIdx.x, p.nkt * p.kv_split, p.nkt * p.kv_split * p.Hk * p.B);
     const int unit = t / p.kv_split, part = t - unit * p.kv_split;
     const int bk = unit / p.nkt, kt = unit - bk * p.nkt;
@@ -931,7 +1001,7 @@ __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
         drain_barrier();
         if (BIAS && cur.g != table_of) {                            // uniform: another head, another bias table
             table_of = cur.g;
-            load_table<4>(p, hk * p.G + table_of, tab);
+            tab = load_table(p, hk * p.G + table_of, tab_);
             drain_barrier();
         }
         const Item nxt = follow(cur);
@@ -955,25 +1025,44 @@ __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
                     s = mfma(row_frag<D>(sq, roff, qb, ks), kf[ks], s);
                     dp = mfma(row_frag<D>(so, roff, qb, ks), VLDS ? row_frag<D>(vtile, roff, 0, ks) : vf[VLDS ? 0 : ks], dp);
                 }
+                if (CAP) {                                          // the slope goes to dP at once: P dP slope is all that follows
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float slope;
+                        s[r] = capped<MODE>(p, s[r], slope);
+                        dp[r] *= slope;
+                    }
+                }
+                if (BIAS) {
+                    const int* at = (const int*)(sq + 2 * TILE) + 192;
+                    const int lo = __builtin_amdgcn_readfirstlane(at[0]), hi_ = __builtin_amdgcn_readfirstlane(at[1]);
+                    if (__builtin_amdgcn_readfirstlane(at[2]) != 0) {        // consecutive rows
+                        const int p0 = lo + cur.half * RT + qb * 32;
+                        add_bias<-1>(p, s, tab, key - p0 - 4 * hi, w0 - p0 - 31, w0 + 31 - p0);
+                    } else if (reach(p.R, w0 - hi_, w0 + 31 - lo) == FAR) {
+                        add_bias<-1>(p, s, tab, 0, w0 - hi_, w0 + 31 - lo);
+                    } else {
+#pragma unroll
+                        for (int q4 = 0; q4 < 4; ++q4) {
+                            const u32x4_t pos = *(const u32x4_t*)((const int*)st + 128 + qb * 32 + 8 * q4 + 4 * hi);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int r = 4 * q4 + e;
+                                s[r] = __builtin_fmaf(s[r], p.zs, tab[min(max(key - (int)pos[e], -p.R), p.R)]);
+                            }
+                        }
+                    }
+                }
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
                     const int r0 = qb * 32 + 8 * q4 + 4 * hi;
                     const f32x4_t ls = *(const f32x4_t*)(st + r0);
-                    u32x4_t pos;
-                    if (BIAS) pos = *(const u32x4_t*)((const int*)st + 128 + r0);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = 4 * q4 + e;
-                        float slope;
-                        float x = capped<MODE>(p, s[r], slope);
-                        if (BIAS) {
-                            x = __builtin_fmaf(x, p.zs, tab[min(max(key - (int)pos[e], -p.R), p.R) + p.R]);
-                            s[r] = x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - ls[e]);
-                        } else {
-                            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.zs, -ls[e]));
-                        }
+                        if (BIAS) s[r] = s[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s[r] - ls[e]);
+                        else s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls[e]));
                         dp[r] *= s[r];
-                        if (CAP) dp[r] *= slope;
                     }
                 }
                 if (!cur.full) {
@@ -1094,35 +1183,35 @@ PF_DEVICE void add_diagonals(const f32x16_t& dt, float* skew, float* hist, int R
     }
 }
 
-// dQ of NW x 32 rows of one head (a wave's 32 rows held in registers) over its key tiles, and this workgroup's part of dbias: every
+// dQ of 128 rows of one head (a wave's 32 rows held in registers; KS = 2: 64 rows, as in the forward kernel) over its key tiles, and this workgroup's part of dbias: every
 // wave adds dT of its pairs into a table of its own (by diagonals, or pair by pair where positions are not consecutive: LDS adds
 // of one wave run in program order; pairs behind the table's ends are summed in registers), the tables are added in wave order.
-template <int D, int MODE, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void range_dq_kernel(const RArgs p) {
+template <int D, int MODE, int KS>
+__global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
-    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE;
+    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE, RW = 4 / KS, NI = 2 / KS;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    float* const tab = (float*)(smem + 2 * BUF);
-    const int NB = 2 * p.R + 1;
-    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    float* const hist = tab + NB + wid * NB;
-    float* const skew = tab + ((NW + 1) * NB + 3) / 4 * 4 + wid * SKEW;
+    float* const meet = (float*)(smem + 2 * BUF);                   // KS = 2: [row wave] whole
+    float* const tab_ = meet + 4;
+    const int NB = 2 * p.R + 1, TS = (table_floats(p.R) + 3) / 4 * 4;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
+    float* const hists = tab_ + TS;
+    float* const hist = hists + wid * NB;
+    float* const skew = hists + (4 * NB + 3) / 4 * 4 + wid * SKEW;
     const int t = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
     const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
-    const int hi = lane >> 5, row0 = (qt * NW + wid) * 32, row = row0 + (lane & 31), rc = min(row, p.Lq - 1);
+    const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31), rc = min(row, p.Lq - 1);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, rc) : 0;
     const Bounds wb = wave_bounds(vis);
-    if (BIAS) {
-        load_table<NW>(p, h, tab);
-        if (p.dbias) {
-            for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
-            for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
-        }
+    const float* const tab = BIAS ? load_table(p, h, tab_) : nullptr;
+    if (BIAS && p.dbias) {
+        for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
+        for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
     }
-    const TileList tl = workgroup_tiles<64, NW>(wb, (int*)smem, wid, lane);
-    const Stager<D, 64, NW> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
+    const TileList tl = workgroup_tiles<64>(wb, (int*)smem, wid, lane);
+    const Stager<D, 64, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
     bf16x8_t qf[D / 16], of[D / 16];
@@ -1142,7 +1231,7 @@ __global__ __launch_bounds__(64 * NW, 2) void range_dq_kernel(const RArgs p) {
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = zero16();
     float below = 0.f, above = 0.f;                 // dbias of distances <= -R and >= R
-    const int pmin = wave_min(row < p.Lq ? pos : 0x7fffffff), pmax = wave_max(row < p.Lq ? pos : -0x7fffffff);
+    const int pmin = BIAS ? __builtin_amdgcn_readfirstlane(wave_min(pos)) : 0, pmax = BIAS ? __builtin_amdgcn_readfirstlane(wave_max(pos)) : 0;
     const int pos0 = __builtin_amdgcn_readfirstlane(pos);
     const bool in_line = __builtin_amdgcn_ballot_w64(row < p.Lq && pos != pos0 + (lane & 31)) == 0;
     bool whole = true;
@@ -1157,16 +1246,16 @@ __global__ __launch_bounds__(64 * NW, 2) void range_dq_kernel(const RArgs p) {
     for (int n = 0; n < tl.n; ++n) {
         drain_barrier();
         if (n + 1 < tl.n) issue(n + 1);
-        const int j0 = tl.at(n) * 64;
-        const char* sk = smem + (n & 1) * BUF;
+        const int j0 = tl.at(n) * 64 + kw * 32 * NI;                // this wave's keys of the tile
+        const char* sk = smem + (n & 1) * BUF + kw * NI * 64 * D;
         const char* sv = sk + TILE;
-        const bool full = wb.full(j0, j0 + 64);
+        const bool full = wb.full(j0, j0 + 32 * NI);
         if (!full) {
             whole = false;
-            if (!wb.any(j0, j0 + 64)) continue;
+            if (!wb.any(j0, j0 + 32 * NI)) continue;
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NI; ++i) {
             f32x16_t s = zero16(), dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) dp[r] = de;
@@ -1176,18 +1265,21 @@ __global__ __launch_bounds__(64 * NW, 2) void range_dq_kernel(const RArgs p) {
                 dp = mfma(row_frag<D>(sv, roff, i, ks), of[ks], dp);
             }
             const int k0 = j0 + 32 * i + 4 * hi;
-            f32x16_t fac;
+            f32x16_t fac;                                           // dbias wants dT without the slope
+            if (CAP) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float slope;
+                    s[r] = capped<MODE>(p, s[r], slope);
+                    if (BIAS) fac[r] = slope;
+                    else dp[r] *= slope;
+                }
+            }
+            if (BIAS) add_bias<1>(p, s, tab, k0 - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float slope;
-                float x = capped<MODE>(p, s[r], slope);
-                if (CAP) fac[r] = slope;
-                if (BIAS) {
-                    x = __builtin_fmaf(x, p.zs, tab[min(max(k0 + reg_row(r) - pos, -p.R), p.R) + p.R]);
-                    s[r] = x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - ls) * dp[r];
-                } else {
-                    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.zs, -ls)) * dp[r];
-                }
+                if (BIAS) s[r] = s[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s[r] - ls) * dp[r];
+                else s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls)) * dp[r];
             }
             if (!full) {
 #pragma unroll
@@ -1213,7 +1305,7 @@ __global__ __launch_bounds__(64 * NW, 2) void range_dq_kernel(const RArgs p) {
                     }
                 }
             }
-            if (CAP) {
+            if (CAP && BIAS) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] *= fac[r];
             }
@@ -1225,10 +1317,30 @@ __global__ __launch_bounds__(64 * NW, 2) void range_dq_kernel(const RArgs p) {
             }
         }
     }
-    const bool bad = any_nonfinite<D / 32>(dq) && !whole && row < p.Lq;
+    if constexpr (KS == 2) {
+        float* const acc = (float*)smem + rw * (D / 32) * 16 * 64;
+        __syncthreads();
+        if (kw == 1) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[(c * 16 + r) * 64 + lane] = dq[c][r];
+            if (lane == 0) meet[rw] = whole ? 1.f : 0.f;
+        }
+        __syncthreads();
+        if (kw == 0) {
+            whole = whole && meet[rw] != 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dq[c][r] += acc[(c * 16 + r) * 64 + lane];
+        }
+    }
+    const bool store = row < p.Lq && kw == 0;
+    const bool bad = any_nonfinite<D / 32>(dq) && !whole && store;
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
     redo = (redo | (redo >> 32)) & 0xffffffffull;
-    if (row < p.Lq && !((redo >> (lane & 31)) & 1)) store_cols<D>(p.dq.p + b * p.dq.bs + row * p.dq.ld + h * p.dq.hs, dq, p.dscale);
+    if (store && !((redo >> (lane & 31)) & 1)) store_cols<D>(p.dq.p + b * p.dq.bs + row * p.dq.ld + h * p.dq.hs, dq, p.dscale);
     while (redo) {
         const int i = __builtin_ctzll(redo);
         redo &= redo - 1;
@@ -1243,12 +1355,7 @@ __global__ __launch_bounds__(64 * NW, 2) void range_dq_kernel(const RArgs p) {
         }
         __syncthreads();
         float* out = p.dbias_parts + ((long long)bh * p.nqt + qt) * NB;
-        for (int i = threadIdx.x; i < NB; i += 64 * NW) {
-            float a = tab[NB + i];
-#pragma unroll
-            for (int w = 1; w < NW; ++w) a += tab[(w + 1) * NB + i];
-            out[i] = a;
-        }
+        for (int i = threadIdx.x; i < NB; i += 256) out[i] = (hists[i] + hists[NB + i]) + (hists[2 * NB + i] + hists[3 * NB + i]);
     }
 }
 
@@ -1301,7 +1408,7 @@ bool few_rows(const pf_attn_ranges_desc* d) {
 // 64-row instead of 128-row workgroups where a head_dim-64 problem has fewer than four of the latter per compute unit: 24.4 instead
 // of 27.6 us for 2 x 64 heads of 512 rows; 1670 instead of 1415 us for 30 heads of 15488.  At head_dim 128 the tiles of the
 // smaller workgroups take the LDS that a third one needs: slower at every size measured.
-bool small_groups(int D, long long Lq, long long H, long long B) { return D == 64 && (Lq + 127) / 128 * H * B < 1024; }
+bool small_groups(int D, long long Lq, long long H, long long B) { return (Lq + 127) / 128 * H * B < (D == 64 ? 1024 : 2048); }
 int row_groups(const pf_attn_ranges_desc* d) { return small_groups(d->D, d->Lq, d->H, d->B) ? (d->Lq + 63) / 64 : (d->Lq + 127) / 128; }
 int mode(const pf_attn_ranges_desc* d) { return (d->cap > 64.f ? 5 : (d->cap > 0.f ? 1 : 0)) + (d->bias ? 2 : 0); }
 int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * (d->H / d->Hkv) + 31) / 32); }
@@ -1355,7 +1462,7 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
     a.zs = fast ? 2.f * a.cap2 : a.series ? 1.f : d->scale * LOG2E;
     a.shift = fast ? a.cap2 : 0.f;
     a.dscale = fast ? 4.f * d->scale : d->scale;
-    a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
+    a.D = d->D; a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
     a.nqt = row_groups(d); a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
     return a;
 }
@@ -1366,22 +1473,18 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
         if (e_ != hipSuccess) return pf_set_err(hipGetErrorString(e_)); \
     } while (0)
 
-template <int D, int MODE, int NW>
+template <int D, int MODE, int KS>
 int launch_fwd_rows(const RArgs& a, hipStream_t stream) {
-    const size_t lds = 4 * FWD_KB<D> * 2 * D + 16 + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
-    PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, MODE, NW>), (int)lds);
-    range_fwd_kernel<D, MODE, NW><<<(unsigned)(a.nqt * a.H * a.B), 64 * NW, lds, stream>>>(a);
+    const size_t lds = 4 * FWD_KB<D, KS> * 2 * D + 16 + (KS == 2 ? 2 * 192 * 4 : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
+    PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, MODE, KS>), (int)lds);
+    range_fwd_kernel<D, MODE, KS><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
     CHECK_LAUNCH();
     return 0;
 }
 
 template <int D, int MODE>
 int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
-    if (!few) {
-        if constexpr (D == 64)
-            if (small_groups(D, a.Lq, a.H, a.B)) return launch_fwd_rows<D, MODE, 2>(a, stream);
-        return launch_fwd_rows<D, MODE, 4>(a, stream);
-    }
+    if (!few) return small_groups(a.D, a.Lq, a.H, a.B) ? launch_fwd_rows<D, MODE, 2>(a, stream) : launch_fwd_rows<D, MODE, 1>(a, stream);
     const size_t lds = 4 * 4 * 32 * 2 * D;                           // the meeting area [4][32][D + 4] fp32 is smaller
     PF_SET_MAX_LDS_ONCE((range_split_kernel<D, MODE>), (int)lds);
     range_split_kernel<D, MODE><<<(unsigned)(a.nrb * a.Hk * a.B * a.nsplit), 256, lds, stream>>>(a);
@@ -1394,11 +1497,11 @@ int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
     return 0;
 }
 
-template <int D, int MODE, int NW>
+template <int D, int MODE, int KS>
 int launch_dq(const RArgs& a, hipStream_t stream) {
-    auto lds = [](int R) { return 4 * 64 * 2 * D + (MODE & 2 ? (NW + 1) * (2 * R + 1) * 4 + 12 + NW * SKEW * 4 : 0); };
-    PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE, NW>), lds(MAX_RADIUS));
-    range_dq_kernel<D, MODE, NW><<<(unsigned)(a.nqt * a.H * a.B), 64 * NW, (size_t)lds(a.R), stream>>>(a);
+    auto lds = [](int R) { return 4 * 64 * 2 * D + 16 + (MODE & 2 ? (table_floats(R) + 3 + 4 * (2 * R + 1) + 3 + 4 * SKEW) * 4 : 0); };
+    PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE, KS>), lds(MAX_RADIUS));
+    range_dq_kernel<D, MODE, KS><<<(unsigned)(a.nqt * a.H * a.B), 256, (size_t)lds(a.R), stream>>>(a);
     CHECK_LAUNCH();
     return 0;
 }
@@ -1411,7 +1514,7 @@ int launch_bwd(const RArgs& a, hipStream_t stream) {
     }
     if (a.Lk > 0) {
         const int rt = D == 64 ? 64 : 32;
-        const size_t lds = 2 * (2 * rt * 2 * D + 2048) + (D == 128 ? 4 * 32 * 2 * D : 0) + (MODE & 2 ? (2 * MAX_RADIUS + 1) * 4 : 0);
+        const size_t lds = 2 * (2 * rt * 2 * D + 2048) + (D == 128 ? 4 * 32 * 2 * D : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
         PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, MODE>), (int)lds);
         range_dkv_kernel<D, MODE><<<(unsigned)(a.nkt * a.kv_split * a.Hk * a.B), 256, lds, stream>>>(a);
         CHECK_LAUNCH();
@@ -1421,9 +1524,7 @@ int launch_bwd(const RArgs& a, hipStream_t stream) {
         }
     }
     if (a.Lq > 0) {
-        if constexpr (D == 64)
-            if (small_groups(D, a.Lq, a.H, a.B)) return launch_dq<D, MODE, 2>(a, stream);
-        return launch_dq<D, MODE, 4>(a, stream);
+        return small_groups(a.D, a.Lq, a.H, a.B) ? launch_dq<D, MODE, 2>(a, stream) : launch_dq<D, MODE, 1>(a, stream);
     }
     return 0;
 }
