@@ -80,16 +80,21 @@ PF_DEVICE bool sees(const Vis& v, int key) {
     return (unsigned)(key - v.alo) < (unsigned)v.na || (unsigned)(key - v.blo) < (unsigned)v.nb;
 }
 
-PF_DEVICE int wave_min(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x = min(x, __shfl_xor(x, o));
-    return x;
+// over the wave, as a scalar: four cross-lane moves inside each row of 16 lanes, then one lane of each row (64-lane butterflies
+// through LDS are 6 round trips each, and a workgroup starts with eight of these)
+template <int CTRL>
+PF_DEVICE int dpp(int x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false); }
+template <typename F>
+PF_DEVICE int wave_fold(int x, F f) {
+    x = f(x, dpp<0xB1>(x));                    // lanes 1 0 3 2
+    x = f(x, dpp<0x4E>(x));                    // lanes 2 3 0 1
+    x = f(x, dpp<0x141>(x));                   // halves of 8 mirrored
+    x = f(x, dpp<0x140>(x));                   // 16 mirrored
+    auto at = [&](int lane) { return __builtin_amdgcn_readlane(x, lane); };
+    return f(f(at(0), at(16)), f(at(32), at(48)));
 }
-PF_DEVICE int wave_max(int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x = max(x, __shfl_xor(x, o));
-    return x;
-}
+PF_DEVICE int wave_min(int x) { return wave_fold(x, [](int a, int b) { return min(a, b); }); }
+PF_DEVICE int wave_max(int x) { return wave_fold(x, [](int a, int b) { return max(a, b); }); }
 PF_DEVICE float wave_add(float x) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
@@ -117,6 +122,10 @@ PF_DEVICE TileList tile_list(int amin, int amax, int bmin, int bmax) {
 
 template <int D, int KS>
 constexpr int FWD_KB = D == 64 || KS == 2 ? 64 : 32;     // keys of a forward tile
+// waves per SIMD the registers are cut for: latency is what is left over (D = 128, 16 heads of 8000 rows: 3 waves and two tiles
+// in LDS 576 us, 2 waves 624 us, 2 waves and three tiles 613 us)
+template <int D, int KS>
+constexpr int FWD_WAVES = D == 64 ? 4 : KS == 1 ? 3 : 2;
 
 // ---------------------------------------------------------------------------------------------- LDS tiles
 // Row-major bf16 rows of D channels, 16-byte chunk c of row r at c ^ swz(r).  A row read (ds_read_b128, one chunk of 16
@@ -168,11 +177,9 @@ struct Bounds {
     PF_DEVICE bool full(int j0, int j1) const { return (alo <= j0 && ahi >= j1) || (blo <= j0 && bhi >= j1); }
 };
 PF_DEVICE Bounds wave_bounds(const Vis& v) {
-    auto lo = [](int x) { return __builtin_amdgcn_readfirstlane(wave_min(x)); };
-    auto hi = [](int x) { return __builtin_amdgcn_readfirstlane(wave_max(x)); };
     constexpr int BIG = 0x7fffffff;
-    return {lo(v.na ? v.alo : BIG), hi(v.na ? v.alo + v.na : 0), lo(v.nb ? v.blo : BIG), hi(v.nb ? v.blo + v.nb : 0),
-            hi(v.na ? v.alo : BIG), lo(v.na ? v.alo + v.na : 0), hi(v.nb ? v.blo : BIG), lo(v.nb ? v.blo + v.nb : 0)};
+    return {wave_min(v.na ? v.alo : BIG), wave_max(v.na ? v.alo + v.na : 0), wave_min(v.nb ? v.blo : BIG), wave_max(v.nb ? v.blo + v.nb : 0),
+            wave_max(v.na ? v.alo : BIG), wave_min(v.na ? v.alo + v.na : 0), wave_max(v.nb ? v.blo : BIG), wave_min(v.nb ? v.blo + v.nb : 0)};
 }
 // the key tiles of a workgroup of 4 waves (`red`: 16 ints of LDS, read behind a barrier)
 template <int KB>
@@ -461,15 +468,16 @@ PF_DEVICE void add_bias(const RArgs& p, f32x16_t& s, const float* tab, int d0, i
 // half of each head's tiles -- the ones that causal and frame-wise masks make long -- for all of its heads and then the second
 // halves: the launch ends on short workgroups.  Tile numbers here count from the heavy end.  (Head after head instead: 1415, now
 // 1308 us for 30 heads of the 15488-row video sequence; 1500, now 1333 us for the gradients at 7808 rows.)
-PF_DEVICE int heavy_first(int block, int n, int nwg) {
+struct Place { int head, rank; };
+PF_DEVICE Place heavy_first(int block, int n, int nwg) {
     const int q = nwg >> 3, r = nwg & 7, xcd = block & 7, i = block >> 3;
     const int c0 = xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q, c1 = c0 + q + (xcd < r ? 1 : 0);
     const int nh = (n + 1) / 2, nl = n - nh;
-    auto heavy_below = [&](int c) { return c / n * nh + min(c % n, nh); };
+    auto heavy_below = [&](int c) { const int w = c / n; return w * nh + min(c - w * n, nh); };
     const int h0 = heavy_below(c0), hn = heavy_below(c1) - h0;
-    if (i < hn) return (h0 + i) / nh * n + (h0 + i) % nh;
-    const int k = (c0 - h0) + (i - hn);
-    return k / nl * n + nh + k % nl;
+    const bool heavy = i < hn;
+    const int k = heavy ? h0 + i : (c0 - h0) + (i - hn), m = heavy ? nh : nl, w = k / m;
+    return {w, k - w * m + (heavy ? 0 : nh)};
 }
 
 // ---------------------------------------------------------------------------------------------- forward, many rows
@@ -483,34 +491,28 @@ PF_DEVICE int heavy_first(int block, int n, int nwg) {
 // so the result is the same.  If a sum or a result of the workgroup came out non-finite, it runs again with the running maximum
 // (CAREFUL), and rows that are still non-finite and had hidden keys are recomputed from their visible keys (exact_o).
 template <int D, int MODE, int KS>
-__global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
+__global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(const RArgs p) {
     constexpr bool BIAS = MODE & 2;
     constexpr int KB = FWD_KB<D, KS>, NI = KB / 32 / KS, TILE = KB * 2 * D, BUF = 2 * TILE, RW = 4 / KS;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    int* const redo_flag = (int*)(smem + 2 * BUF);
-    float* const meet = (float*)(smem + 2 * BUF + 16);              // KS = 2: [row wave][3][64] maximum, sum, whole
+    int* const red = (int*)(smem + 2 * BUF);
+    int* const redo_flag = red + 16;
+    float* const meet = (float*)(smem + 2 * BUF + 80);           // KS = 2: [row wave][3][64] maximum, sum, whole
     float* const tab_ = meet + (KS == 2 ? RW * 192 : 0);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
-    const int t = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
-    const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
+    const Place at = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
+    const int bh = at.head, qt = p.nqt - 1 - at.rank;
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
     const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
-    const int pmin = BIAS ? __builtin_amdgcn_readfirstlane(wave_min(pos)) : 0, pmax = BIAS ? __builtin_amdgcn_readfirstlane(wave_max(pos)) : 0;
+    const int pmin = BIAS ? wave_min(pos) : 0, pmax = BIAS ? wave_max(pos) : 0;
     const Bounds wb = wave_bounds(vis);
-    const float* const tab = BIAS ? load_table(p, h, tab_) : nullptr;
     if (threadIdx.x == 0) *redo_flag = 0;
-    const TileList tl = workgroup_tiles<KB>(wb, (int*)smem, wid, lane);
+    const TileList tl = workgroup_tiles<KB>(wb, red, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
     const Stager<D, KB, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
-    bf16x8_t qf[D / 16];
-    {
-        const bf16_t* q = p.q.p + b * p.q.bs + (long long)min(row, p.Lq - 1) * p.q.ld + h * p.q.hs + hi * 8;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8_t*)(q + ks * 16);
-    }
     const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
     f32x16_t o[D / 32];
     float m, l;
@@ -521,6 +523,14 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
         sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
         sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
     };
+    if (tl.n > 0) issue(0);                        // the first tile is on its way before the rows are read
+    const float* const tab = BIAS ? load_table(p, h, tab_) : nullptr;
+    bf16x8_t qf[D / 16];
+    {
+        const bf16_t* q = p.q.p + b * p.q.bs + (long long)min(row, p.Lq - 1) * p.q.ld + h * p.q.hs + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8_t*)(q + ks * 16);
+    }
     auto pass = [&](auto careful) {
         constexpr bool CAREFUL = decltype(careful)::value;
         const float zs = BIAS ? 1.f : p.zs;
@@ -530,8 +540,10 @@ __global__ __launch_bounds__(256, 2) void range_fwd_kernel(const RArgs p) {
         l = 0.f;
         whole = true;
         unsigned long long fresh = __builtin_amdgcn_ballot_w64(vis.na + vis.nb > 0);     // rows without a reference yet
-        drain_barrier();                           // nobody reads what lay in the tiles' memory any more
-        if (tl.n > 0) issue(0);
+        if (CAREFUL) {
+            drain_barrier();                       // nobody reads the first pass's tiles any more
+            if (tl.n > 0) issue(0);
+        }
         for (int n = 0; n < tl.n; ++n) {
             drain_barrier();
             if (n + 1 < tl.n) issue(n + 1);
@@ -673,11 +685,10 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
     const int pos = BIAS ? row_pos(p, b, row) : 0;
     const float* const bias = BIAS ? p.bias + (long long)h * (2 * p.R + 1) + p.R : nullptr;
     const float far_below = BIAS ? bias2(bias[-p.R]) : 0.f, far_above = BIAS ? bias2(bias[p.R]) : 0.f;
-    const int pmin = BIAS ? __builtin_amdgcn_readfirstlane(wave_min(pos)) : 0, pmax = BIAS ? __builtin_amdgcn_readfirstlane(wave_max(pos)) : 0;
+    const int pmin = BIAS ? wave_min(pos) : 0, pmax = BIAS ? wave_max(pos) : 0;
     const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
     const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
-    const TileList tl = tile_list<32>(__builtin_amdgcn_readfirstlane(amin), __builtin_amdgcn_readfirstlane(amax),
-                                      __builtin_amdgcn_readfirstlane(bmin), __builtin_amdgcn_readfirstlane(bmax));
+    const TileList tl = tile_list<32>(amin, amax, bmin, bmax);
     const int n0 = (int)((long long)tl.n * part / p.nsplit), n1 = (int)((long long)tl.n * (part + 1) / p.nsplit);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
@@ -895,21 +906,24 @@ __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
 // -delta enters through the C operand of the dP product.  kv_split > 1: this workgroup takes an even part of the (head, tile)
 // pairs that the keys need and leaves 32-bit sums for range_kvjoin_kernel.
 //
-// D = 64: 64-row tiles, K and V fragments and both results in registers (two workgroups per compute unit).  D = 128 has twice
-// the results (128 registers): 32-row tiles and V read from LDS leave room for the second workgroup (with V in registers and
-// 64-row tiles one wave per SIMD ran everything in series, 8400 cycles per tile, 800 of its instructions register moves).
+// D = 64: 64-row tiles, K and both results in registers, V in LDS: three waves per SIMD (1370 us for the whole gradient of 30 heads
+// of the 7808-row video sequence; V in registers and two waves 1430 us; with a bias table the third wave spills: 53 instead of
+// 48 us at 2 x 12 heads of 301 rows).  D = 128 has twice the results (128 registers): 32-row tiles and V in LDS leave room for
+// a second workgroup (with V in registers and 64-row tiles one wave per SIMD ran everything in series, 8400 cycles per tile,
+// 800 of its instructions register moves).
 template <int D, int MODE>
-__global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
-    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, VLDS = D == 128;
+constexpr bool KV_V_LDS = D == 128 || !(MODE & 2);
+template <int D, int MODE>
+__global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv_kernel(const RArgs p) {
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2, VLDS = KV_V_LDS<D, MODE>;
     constexpr int RT = D == 64 ? 64 : 32, HALVES = 64 / RT, TILE = RT * 2 * D, BUF = 2 * TILE + 2048, VTILE = VLDS ? 32 * 2 * D : 0;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     char* const vtile = smem + 2 * BUF + wid * VTILE;
     float* const tab_ = (float*)(smem + 2 * BUF + 4 * VTILE);
     const float* tab = nullptr;
-    const int t = heavy_first(blockIdx.x, p.nkt * p.kv_split, p.nkt * p.kv_split * p.Hk * p.B);
-    const int unit = t / p.kv_split, part = t - unit * p.kv_split;
-    const int bk = unit / p.nkt, kt = unit - bk * p.nkt;
+    const Place at = heavy_first(blockIdx.x, p.nkt * p.kv_split, p.nkt * p.kv_split * p.Hk * p.B);
+    const int bk = at.head, kt = at.rank / p.kv_split, part = at.rank - kt * p.kv_split;
     const int b = bk / p.Hk, hk = bk - b * p.Hk;
     const int hi = lane >> 5;
     const int w0 = kt * 128 + wid * 32, key = w0 + (lane & 31);
@@ -1034,9 +1048,9 @@ __global__ __launch_bounds__(256, 2) void range_dkv_kernel(const RArgs p) {
                     }
                 }
                 if (BIAS) {
-                    const int* at = (const int*)(sq + 2 * TILE) + 192;
-                    const int lo = __builtin_amdgcn_readfirstlane(at[0]), hi_ = __builtin_amdgcn_readfirstlane(at[1]);
-                    if (__builtin_amdgcn_readfirstlane(at[2]) != 0) {        // consecutive rows
+                    const int* of_tile = (const int*)(sq + 2 * TILE) + 192;
+                    const int lo = __builtin_amdgcn_readfirstlane(of_tile[0]), hi_ = __builtin_amdgcn_readfirstlane(of_tile[1]);
+                    if (__builtin_amdgcn_readfirstlane(of_tile[2]) != 0) {        // consecutive rows
                         const int p0 = lo + cur.half * RT + qb * 32;
                         add_bias<-1>(p, s, tab, key - p0 - 4 * hi, w0 - p0 - 31, w0 + 31 - p0);
                     } else if (reach(p.R, w0 - hi_, w0 + 31 - lo) == FAR) {
@@ -1191,29 +1205,37 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
     constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE, RW = 4 / KS, NI = 2 / KS;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    float* const meet = (float*)(smem + 2 * BUF);                   // KS = 2: [row wave] whole
+    int* const red = (int*)(smem + 2 * BUF);
+    float* const meet = (float*)(red + 16);                         // KS = 2: [row wave] whole
     float* const tab_ = meet + 4;
     const int NB = 2 * p.R + 1, TS = (table_floats(p.R) + 3) / 4 * 4;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
     float* const hists = tab_ + TS;
     float* const hist = hists + wid * NB;
     float* const skew = hists + (4 * NB + 3) / 4 * 4 + wid * SKEW;
-    const int t = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
-    const int bh = t / p.nqt, qt = p.nqt - 1 - (t - bh * p.nqt);
+    const Place at = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
+    const int bh = at.head, qt = p.nqt - 1 - at.rank;
     const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
     const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31), rc = min(row, p.Lq - 1);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, rc) : 0;
     const Bounds wb = wave_bounds(vis);
+    const TileList tl = workgroup_tiles<64>(wb, red, wid, lane);
+    const Stager<D, 64, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
+    const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
+    const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
+    auto issue = [&](int n) {
+        const int j0 = tl.at(n) * 64;
+        char* buf = smem + (n & 1) * BUF;
+        sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
+        sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
+    };
+    if (tl.n > 0) issue(0);                        // the first tile is on its way before the rows are read
     const float* const tab = BIAS ? load_table(p, h, tab_) : nullptr;
     if (BIAS && p.dbias) {
         for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
         for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
     }
-    const TileList tl = workgroup_tiles<64>(wb, (int*)smem, wid, lane);
-    const Stager<D, 64, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
-    const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
-    const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
     bf16x8_t qf[D / 16], of[D / 16];
     {
         const bf16_t* q = p.q.p + b * p.q.bs + rc * p.q.ld + h * p.q.hs + hi * 8;
@@ -1231,18 +1253,10 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[c] = zero16();
     float below = 0.f, above = 0.f;                 // dbias of distances <= -R and >= R
-    const int pmin = BIAS ? __builtin_amdgcn_readfirstlane(wave_min(pos)) : 0, pmax = BIAS ? __builtin_amdgcn_readfirstlane(wave_max(pos)) : 0;
+    const int pmin = BIAS ? wave_min(pos) : 0, pmax = BIAS ? wave_max(pos) : 0;
     const int pos0 = __builtin_amdgcn_readfirstlane(pos);
     const bool in_line = __builtin_amdgcn_ballot_w64(row < p.Lq && pos != pos0 + (lane & 31)) == 0;
     bool whole = true;
-    drain_barrier();
-    auto issue = [&](int n) {
-        const int j0 = tl.at(n) * 64;
-        char* buf = smem + (n & 1) * BUF;
-        sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
-        sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
-    };
-    if (tl.n > 0) issue(0);
     for (int n = 0; n < tl.n; ++n) {
         drain_barrier();
         if (n + 1 < tl.n) issue(n + 1);
@@ -1405,11 +1419,13 @@ const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
 bool few_rows(const pf_attn_ranges_desc* d) {
     return (long long)((d->Lq + 127) / 128) * d->H * d->B < 256 || (long long)d->Lq * (d->H / d->Hkv) <= 32;
 }
-// 64-row instead of 128-row workgroups where a head_dim-64 problem has fewer than four of the latter per compute unit: 24.4 instead
-// of 27.6 us for 2 x 64 heads of 512 rows; 1670 instead of 1415 us for 30 heads of 15488.  At head_dim 128 the tiles of the
-// smaller workgroups take the LDS that a third one needs: slower at every size measured.
-bool small_groups(int D, long long Lq, long long H, long long B) { return (Lq + 127) / 128 * H * B < (D == 64 ? 1024 : 2048); }
-int row_groups(const pf_attn_ranges_desc* d) { return small_groups(d->D, d->Lq, d->H, d->B) ? (d->Lq + 63) / 64 : (d->Lq + 127) / 128; }
+// 64-row workgroups (KS = 2) instead of 128-row ones where those would be few: half the chain per wave for twice the tile traffic.
+// Forward: 21.5 instead of 22 us at 2 x 64 heads of 512 rows of 64; 55 instead of 67 us with 128-row workgroups at 16 x 16 heads of
+// 500 rows of 128.  dQ: 48 instead of 55 us for the whole gradient of 2 x 12 heads of 301 rows of 64, 240 instead of 263 us for that
+// of 16 heads of 4001 rows of 128.
+bool small_fwd(int D, long long Lq, long long H, long long B) { return (Lq + 127) / 128 * H * B < (D == 64 ? 1024 : 512); }
+bool small_dq(int D, long long Lq, long long H, long long B) { return (Lq + 127) / 128 * H * B < (D == 64 ? 1024 : 2048); }
+int row_groups(int Lq, bool small) { return small ? (Lq + 63) / 64 : (Lq + 127) / 128; }
 int mode(const pf_attn_ranges_desc* d) { return (d->cap > 64.f ? 5 : (d->cap > 0.f ? 1 : 0)) + (d->bias ? 2 : 0); }
 int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * (d->H / d->Hkv) + 31) / 32); }
 int splits(const pf_attn_ranges_desc* d) {
@@ -1440,7 +1456,7 @@ BwdSizes bwd_sizes(const pf_attn_ranges_desc* d) {
     s.stat = (long long)d->B * d->H * nq * 1024;
     s.vis = (long long)d->B * nq * 1024;
     s.tiles = up16((long long)d->B * nq * 32);
-    s.parts = d->dbias ? up16((long long)d->B * d->H * row_groups(d) * (2 * d->bias_radius + 1) * 4) : 0;
+    s.parts = d->dbias ? up16((long long)d->B * d->H * row_groups(d->Lq, small_dq(d->D, d->Lq, d->H, d->B)) * (2 * d->bias_radius + 1) * 4) : 0;
     const int n = kv_splits(d);
     s.kv = n > 1 ? (long long)n * d->B * d->Hkv * d->Lk * 2 * d->D * 4 : 0;
     return s;
@@ -1463,7 +1479,7 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
     a.shift = fast ? a.cap2 : 0.f;
     a.dscale = fast ? 4.f * d->scale : d->scale;
     a.D = d->D; a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
-    a.nqt = row_groups(d); a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
+    a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
     return a;
 }
 
@@ -1475,7 +1491,7 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
 
 template <int D, int MODE, int KS>
 int launch_fwd_rows(const RArgs& a, hipStream_t stream) {
-    const size_t lds = 4 * FWD_KB<D, KS> * 2 * D + 16 + (KS == 2 ? 2 * 192 * 4 : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
+    const size_t lds = 4 * FWD_KB<D, KS> * 2 * D + 80 + (KS == 2 ? 2 * 192 * 4 : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
     PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, MODE, KS>), (int)lds);
     range_fwd_kernel<D, MODE, KS><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
     CHECK_LAUNCH();
@@ -1484,7 +1500,7 @@ int launch_fwd_rows(const RArgs& a, hipStream_t stream) {
 
 template <int D, int MODE>
 int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
-    if (!few) return small_groups(a.D, a.Lq, a.H, a.B) ? launch_fwd_rows<D, MODE, 2>(a, stream) : launch_fwd_rows<D, MODE, 1>(a, stream);
+    if (!few) return small_fwd(a.D, a.Lq, a.H, a.B) ? launch_fwd_rows<D, MODE, 2>(a, stream) : launch_fwd_rows<D, MODE, 1>(a, stream);
     const size_t lds = 4 * 4 * 32 * 2 * D;                           // the meeting area [4][32][D + 4] fp32 is smaller
     PF_SET_MAX_LDS_ONCE((range_split_kernel<D, MODE>), (int)lds);
     range_split_kernel<D, MODE><<<(unsigned)(a.nrb * a.Hk * a.B * a.nsplit), 256, lds, stream>>>(a);
@@ -1499,7 +1515,7 @@ int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
 
 template <int D, int MODE, int KS>
 int launch_dq(const RArgs& a, hipStream_t stream) {
-    auto lds = [](int R) { return 4 * 64 * 2 * D + 16 + (MODE & 2 ? (table_floats(R) + 3 + 4 * (2 * R + 1) + 3 + 4 * SKEW) * 4 : 0); };
+    auto lds = [](int R) { return 4 * 64 * 2 * D + 80 + (MODE & 2 ? (table_floats(R) + 3 + 4 * (2 * R + 1) + 3 + 4 * SKEW) * 4 : 0); };
     PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE, KS>), lds(MAX_RADIUS));
     range_dq_kernel<D, MODE, KS><<<(unsigned)(a.nqt * a.H * a.B), 256, (size_t)lds(a.R), stream>>>(a);
     CHECK_LAUNCH();
@@ -1514,7 +1530,7 @@ int launch_bwd(const RArgs& a, hipStream_t stream) {
     }
     if (a.Lk > 0) {
         const int rt = D == 64 ? 64 : 32;
-        const size_t lds = 2 * (2 * rt * 2 * D + 2048) + (D == 128 ? 4 * 32 * 2 * D : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
+        const size_t lds = 2 * (2 * rt * 2 * D + 2048) + (KV_V_LDS<D, MODE> ? 4 * 32 * 2 * D : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
         PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, MODE>), (int)lds);
         range_dkv_kernel<D, MODE><<<(unsigned)(a.nkt * a.kv_split * a.Hk * a.B), 256, lds, stream>>>(a);
         CHECK_LAUNCH();
@@ -1524,7 +1540,7 @@ int launch_bwd(const RArgs& a, hipStream_t stream) {
         }
     }
     if (a.Lq > 0) {
-        return small_groups(a.D, a.Lq, a.H, a.B) ? launch_dq<D, MODE, 2>(a, stream) : launch_dq<D, MODE, 1>(a, stream);
+        return small_dq(a.D, a.Lq, a.H, a.B) ? launch_dq<D, MODE, 2>(a, stream) : launch_dq<D, MODE, 1>(a, stream);
     }
     return 0;
 }
@@ -1553,8 +1569,9 @@ extern "C" int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, hipStream_
         return pf_set_err("pf_attention_ranges_bf16: workspace missing, unaligned or too small");
     RArgs a = range_args(d);
     const bool few = few_rows(d);
-    const long long grid = few ? (long long)row_blocks(d) * d->Hkv * d->B * splits(d) : (long long)a.nqt * d->H * d->B;
+    const long long grid = few ? (long long)row_blocks(d) * d->Hkv * d->B * splits(d) : (long long)row_groups(d->Lq, true) * d->H * d->B;
     if (grid > 0x7fffffffLL) return pf_set_err("pf_attention_ranges_bf16: too many workgroups");
+    a.nqt = row_groups(d->Lq, small_fwd(d->D, d->Lq, d->H, d->B));
     a.nrb = row_blocks(d);
     a.nsplit = few ? splits(d) : 1;
     a.parts = (float*)d->workspace;
@@ -1581,7 +1598,7 @@ extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t
     if (need && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need))
         return pf_set_err("pf_attention_ranges_bwd: workspace missing, unaligned or too small");
     if (d->B > 65535 || d->H > 65535) return pf_set_err("pf_attention_ranges_bwd: more than 65535 batch entries or heads");
-    if ((long long)((d->Lq + 127) / 128) * d->H * d->B > 0x7fffffffLL || (long long)((d->Lk + 127) / 128) * d->H * d->B * 16 > 0x7fffffffLL ||
+    if ((long long)row_groups(d->Lq, true) * d->H * d->B > 0x7fffffffLL || (long long)((d->Lk + 127) / 128) * d->H * d->B * 16 > 0x7fffffffLL ||
         (long long)(d->Lq + 63) / 64 * (d->H / (d->Hkv ? d->Hkv : 1)) > 0x7fffffffLL)
         return pf_set_err("pf_attention_ranges_bwd: too many workgroups");
     if (!d->H) return 0;
@@ -1593,6 +1610,7 @@ extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t
     a.dbias_parts = (float*)(w += s.tiles);
     a.kv_parts = (float*)(w += s.parts);
     a.kv_split = kv_splits(d);
+    a.nqt = row_groups(d->Lq, small_dq(d->D, d->Lq, d->H, d->B));
     a.dbias = d->dbias;
     int rc = 0;
     if (d->B) switch ((d->D == 64 ? 0 : 8) + mode(d)) {
