@@ -39,9 +39,10 @@ struct RArgs {
     const int* a_lo; const int* a_hi; const int* b_lo; const int* b_hi; long long range_bs;
     const int* q_pos; long long pos_bs;
     const float* bias; int R;
-    // z = q.k.  Scores in base 2 are x zs + shift with x = z (uncapped), x = cap_u(z zc) (cap) or x = cap log2 e tanh(z zc) (SERIES);
+    // z = q.k.  Scores in base 2 are x zs + shift with x = z (uncapped), x = cap_u(z zc) (cap) or x = tanh(z zc) (SERIES);
     // the shift is left out wherever only differences of scores count
     float zs, zc, shift, cap2;
+    float zn, shift_n;                 // zs and shift in natural units
     float scale, dscale;               // dQ, dK = dscale times the products of dZ (4 scale with cap_u's slope)
     int series;
     int D, B, H, Hk, G, Lq, Lk;
@@ -259,8 +260,10 @@ PF_DEVICE float cap_u(float x) { return __builtin_amdgcn_rcpf(-1.f - __builtin_a
 PF_DEVICE float tanh_f(float x) {
     const float y = x * x;
     const float near = x * __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
-    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x));
-    return fabsf(x) < 0.3f ? near : far;
+    const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * fabsf(x)), d = 1.f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
+    return fabsf(x) < 0.3f ? near : copysignf((1.f - e) * r, x);
 }
 // x of one product and the slope of the cap (a quarter of it with cap_u)
 template <int MODE>
@@ -270,7 +273,7 @@ PF_DEVICE float capped(const RArgs& p, float z, float& slope) {
     } else if constexpr ((MODE & 4) != 0) {
         const float y = tanh_f(z * p.zc);
         slope = __builtin_fmaf(-y, y, 1.f);
-        return p.cap2 * y;
+        return y;
     } else {
         const float u = cap_u(z * p.zc);
         slope = __builtin_fmaf(-u, u, -u);
@@ -419,14 +422,16 @@ PF_DEVICE bool any_nonfinite(const f32x16_t* o) {
     return t != t;
 }
 
-// The bias table of head h in LDS, base 2, continued by PAD entries of its end values on both sides: a 32 x 64 block of consecutive
+// The bias table of head h in LDS, base 2 (or times `unit`), continued by PAD entries of its end values on both sides: a 32 x 64 block of consecutive
 // rows whose distances are not all behind an end stays inside it, so its entries lie at fixed offsets from one address per
 // lane (a subtraction, a clamp and an address per score otherwise).  Returned: the entry of distance 0.
 constexpr int PAD = 96;
 constexpr int table_floats(int R) { return 2 * R + 1 + 2 * PAD; }
-PF_DEVICE const float* load_table(const RArgs& p, int h, float* tab) {
-    for (int i = threadIdx.x; i < table_floats(p.R); i += 256)
-        tab[i] = bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(i - PAD, 0), 2 * p.R)]);
+PF_DEVICE const float* load_table(const RArgs& p, int h, float* tab, float unit = LOG2E) {
+    for (int i = threadIdx.x; i < table_floats(p.R); i += 256) {
+        const float b = p.bias[(long long)h * (2 * p.R + 1) + min(max(i - PAD, 0), 2 * p.R)];
+        tab[i] = b <= HIDDEN ? -__builtin_inff() : b * unit;
+    }
     return tab + PAD + p.R;
 }
 // how a block with distances lo .. hi (wave-uniform) reads it
@@ -446,21 +451,21 @@ PF_DEVICE void cap_only(const RArgs& p, f32x16_t& s) {
         }
     }
 }
-// x -> score with the bias; d0 = distance of this lane's register 0 (SIGN 1: registers are keys, -1: rows), lo, hi = of the block
+// x -> x zs + bias; d0 = distance of this lane's register 0 (SIGN 1: registers are keys, -1: rows), lo, hi = of the block
 template <int SIGN>
-PF_DEVICE void add_bias(const RArgs& p, f32x16_t& s, const float* tab, int d0, int lo, int hi) {
+PF_DEVICE void add_bias(const RArgs& p, f32x16_t& s, float zs, const float* tab, int d0, int lo, int hi) {
     const Reach how = reach(p.R, lo, hi);
     if (how == NEAR) {
         const float* at = tab + d0;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.zs, at[SIGN * reg_row(r)]);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], zs, at[SIGN * reg_row(r)]);
     } else if (how == FAR) {
         const float c = tab[hi <= -p.R ? -p.R : p.R];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.zs, c);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], zs, c);
     } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.zs, tab[min(max(d0 + SIGN * reg_row(r), -p.R), p.R)]);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], zs, tab[min(max(d0 + SIGN * reg_row(r), -p.R), p.R)]);
     }
 }
 
@@ -565,7 +570,7 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 cap_only<MODE>(p, s[i]);
-                if (BIAS) add_bias<1>(p, s[i], tab, j0 + 32 * i + 4 * hi - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
+                if (BIAS) add_bias<1>(p, s[i], p.zs, tab, j0 + 32 * i + 4 * hi - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
             }
             if (!full) {
 #pragma unroll
@@ -1052,9 +1057,9 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
                     const int lo = __builtin_amdgcn_readfirstlane(of_tile[0]), hi_ = __builtin_amdgcn_readfirstlane(of_tile[1]);
                     if (__builtin_amdgcn_readfirstlane(of_tile[2]) != 0) {        // consecutive rows
                         const int p0 = lo + cur.half * RT + qb * 32;
-                        add_bias<-1>(p, s, tab, key - p0 - 4 * hi, w0 - p0 - 31, w0 + 31 - p0);
+                        add_bias<-1>(p, s, p.zs, tab, key - p0 - 4 * hi, w0 - p0 - 31, w0 + 31 - p0);
                     } else if (reach(p.R, w0 - hi_, w0 + 31 - lo) == FAR) {
-                        add_bias<-1>(p, s, tab, 0, w0 - hi_, w0 + 31 - lo);
+                        add_bias<-1>(p, s, p.zs, tab, 0, w0 - hi_, w0 + 31 - lo);
                     } else {
 #pragma unroll
                         for (int q4 = 0; q4 < 4; ++q4) {
@@ -1231,7 +1236,7 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
         sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
     };
     if (tl.n > 0) issue(0);                        // the first tile is on its way before the rows are read
-    const float* const tab = BIAS ? load_table(p, h, tab_) : nullptr;
+    const float* const tab = BIAS ? load_table(p, h, tab_, 1.f) : nullptr;
     if (BIAS && p.dbias) {
         for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
         for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
@@ -1247,7 +1252,10 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
         }
     }
     const float* const st = p.stat + (((long long)b * p.H + h) * p.nq64 + (rc >> 6)) * 256 + (rc & 63);
-    const float ls = st[0], de = st[64];                            // log-sum-exp (base 2), -delta
+    const float ls = st[0], de = st[64];                            // log-sum-exp (base 2, less the shift), -delta
+    // dbias is a 32-bit result: with a bias the scores stay in natural units here, so that only their difference from the row's lse
+    // is rounded again by the change of base (lse, cap and bias times log2 e leave 5e-7 each, the same for whole rows and distances)
+    const float lse = BIAS ? p.lse[((long long)b * p.H + h) * p.Lq + rc] - p.shift_n : 0.f;
     const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
     f32x16_t dq[D / 32];
 #pragma unroll
@@ -1289,10 +1297,10 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
                     else dp[r] *= slope;
                 }
             }
-            if (BIAS) add_bias<1>(p, s, tab, k0 - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
+            if (BIAS) add_bias<1>(p, s, p.zn, tab, k0 - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                if (BIAS) s[r] = s[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s[r] - ls) * dp[r];
+                if (BIAS) s[r] = s[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((s[r] - lse) * LOG2E) * dp[r];
                 else s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls)) * dp[r];
             }
             if (!full) {
@@ -1426,7 +1434,9 @@ bool few_rows(const pf_attn_ranges_desc* d) {
 bool small_fwd(int D, long long Lq, long long H, long long B) { return (Lq + 127) / 128 * H * B < (D == 64 ? 1024 : 512); }
 bool small_dq(int D, long long Lq, long long H, long long B) { return (Lq + 127) / 128 * H * B < (D == 64 ? 1024 : 2048); }
 int row_groups(int Lq, bool small) { return small ? (Lq + 63) / 64 : (Lq + 127) / 128; }
-int mode(const pf_attn_ranges_desc* d) { return (d->cap > 64.f ? 5 : (d->cap > 0.f ? 1 : 0)) + (d->bias ? 2 : 0); }
+// SERIES also where the bias's gradient is wanted: it is a 32-bit result, and cap_u's 2^-23 of the cap would be all of its error
+bool series(const pf_attn_ranges_desc* d) { return d->cap > 64.f || (d->cap > 0.f && d->dbias); }
+int mode(const pf_attn_ranges_desc* d) { return (d->cap > 0.f ? 1 : 0) + (d->bias ? 2 : 0) + (series(d) ? 4 : 0); }
 int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * (d->H / d->Hkv) + 31) / 32); }
 int splits(const pf_attn_ranges_desc* d) {
     const long long units = (long long)row_blocks(d) * d->Hkv * d->B, tiles = (d->Lk + 31) / 32;
@@ -1472,11 +1482,13 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
     a.bias = d->bias; a.R = d->bias ? d->bias_radius : 0;
     a.scale = d->scale;
     a.cap2 = d->cap * LOG2E;
-    a.series = d->cap > 64.f;
+    a.series = series(d);
     const bool fast = d->cap > 0.f && !a.series;
     a.zc = d->cap > 0.f ? d->scale / d->cap * (fast ? 2.f * LOG2E : 1.f) : 0.f;
-    a.zs = fast ? 2.f * a.cap2 : a.series ? 1.f : d->scale * LOG2E;
+    a.zs = fast ? 2.f * a.cap2 : a.series ? a.cap2 : d->scale * LOG2E;
     a.shift = fast ? a.cap2 : 0.f;
+    a.zn = fast ? 2.f * d->cap : a.series ? d->cap : d->scale;
+    a.shift_n = fast ? d->cap : 0.f;
     a.dscale = fast ? 4.f * d->scale : d->scale;
     a.D = d->D; a.B = d->B; a.H = d->H; a.Hk = d->Hkv; a.G = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
     a.nkt = (d->Lk + 127) / 128; a.nq64 = (d->Lq + 63) / 64;
