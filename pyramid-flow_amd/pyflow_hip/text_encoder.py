@@ -14,8 +14,8 @@ concatenated :127, same T5 call).  The encoder arithmetic the reference gets fro
   LayerNorm, pooled = the EOS token's row (argmax of the ids for the legacy ``eos_token_id == 2`` configs), optional
   bias-free ``text_projection``.
 
-Everything on the device goes through the C ABI (pf_gemm_bf16, pf_attention_small_bf16, pf_rmsnorm, pf_ln_modulate,
-pf_glu_mul, pf_embed_rows, pf_copy_rows); torch is used for buffers only.  Tokenisation is host string work and stays
+Everything on the device goes through the C ABI (pf_gemm_bf16, pf_attention_small_bf16 -- beyond 256 tokens
+pf_attention_ranges_bf16 --, pf_rmsnorm, pf_ln_modulate, pf_glu_mul, pf_embed_rows, pf_copy_rows); torch is used for buffers only.  Tokenisation is host string work and stays
 with the transformers tokenizers, exactly as in the reference (injectable for tests: any callable with the
 tokenizer call signature returning ``input_ids`` / ``attention_mask``).
 """
@@ -26,6 +26,7 @@ import os
 import torch
 
 from . import ops
+from .plan import KeyRanges
 from .lib import GEMM_GATE_RES, GEMM_ACT_QUICK_GELU, GEMM_ACT_GELU_ERF
 from .refapi import DeviceModuleAPI
 
@@ -50,6 +51,13 @@ def t5_relative_position_buckets(L, num_buckets=32, max_distance=128):
     of_dist = torch.where(dist < max_exact, dist, large)               # [L]
     rel = torch.arange(L)[None, :] - torch.arange(L)[:, None]          # j - i
     return of_dist[rel.abs()] + (rel > 0).long() * half
+
+
+def t5_bias_by_distance(rel_bias, num_buckets=32, max_distance=128):
+    """fp32 [H][2 max_distance + 1]: the bias of the distances (key j - query i) -max_distance .. max_distance.  Buckets do not
+    change any more behind max_distance, so with distances clamped this is the bias of a sequence of any length."""
+    buckets = t5_relative_position_buckets(max_distance + 1, num_buckets, max_distance)
+    return rel_bias[torch.cat([buckets[1:, 0].flip(0), buckets[0]])].t().contiguous()
 
 
 def _bf16(t, device):
@@ -115,6 +123,7 @@ class T5EncoderHIP:
             ))
         self.ln_f = _f32(sd["encoder.final_layer_norm.weight"].to(torch.bfloat16), device)
         self._bias_cache = {}
+        self._bias_table = None                   # by distance, for sequences beyond 256 tokens
 
     @property
     def dtype(self):
@@ -127,15 +136,28 @@ class T5EncoderHIP:
             self._bias_cache[L] = self.rel_bias[buckets].permute(2, 0, 1).contiguous().to(self.device)
         return self._bias_cache[L]
 
+    def bias_table(self):
+        """fp32 [H][2 max_distance + 1] device table of t5_bias_by_distance"""
+        if self._bias_table is None:
+            self._bias_table = t5_bias_by_distance(self.rel_bias, self.num_buckets, self.max_distance).to(self.device)
+        return self._bias_table
+
     def forward(self, input_ids, attention_mask=None):
+        """last_hidden_state [B, L, d_model].  Up to 256 tokens any attention_mask; beyond (ops.attention_ranges) one whose visible
+        tokens form at most two runs, which is read back to the host once per call."""
         B, L = input_ids.shape
-        if L > 256:
-            raise ValueError("T5EncoderHIP: at most 256 tokens")
+        long = L > 256
+        if long and self.max_distance > 512:
+            raise ValueError("T5EncoderHIP: beyond 256 tokens relative_attention_max_distance must be at most 512")
         rows, d, inner, dff = B * L, self.d_model, self.inner, self.d_ff
         dev = self.device
         ids = input_ids.to(device=dev, dtype=torch.int32).contiguous()
-        km = None if attention_mask is None else attention_mask.to(device=dev, dtype=torch.int32).contiguous()
-        bias = self.position_bias(L)
+        if long:
+            ranges = None if attention_mask is None else KeyRanges.from_key_mask(attention_mask, L, dev)
+            bias = self.bias_table()
+        else:
+            km = None if attention_mask is None else attention_mask.to(device=dev, dtype=torch.int32).contiguous()
+            bias = self.position_bias(L)
         h = torch.empty(rows, d, dtype=torch.bfloat16, device=dev)
         n = torch.empty(rows, d, dtype=torch.bfloat16, device=dev)
         qkv = torch.empty(rows, 3 * inner, dtype=torch.bfloat16, device=dev)
@@ -147,7 +169,11 @@ class T5EncoderHIP:
         for w in self.layers:
             ops.rmsnorm(h, n, w["ln1"], d, rows, eps=self.eps)
             ops.gemm(n, w["wqkv"], qkv, rows, 3 * inner, d, d, d, 3 * inner, workspace=ws)
-            ops.attention_small(qkv, att, 0, inner, 2 * inner, 3 * inner, inner, B, self.H, L, 1.0, bias=bias, key_mask=km)
+            if long:
+                q, k, v = qkv.view(B, L, 3, self.H, 64).unbind(2)
+                ops.attention_ranges(q, k, v, att.view(B, L, self.H, 64), ranges=ranges, scale=1.0, bias=bias)
+            else:
+                ops.attention_small(qkv, att, 0, inner, 2 * inner, 3 * inner, inner, B, self.H, L, 1.0, bias=bias, key_mask=km)
             ops.gemm(att, w["wo"], h, rows, d, inner, inner, inner, d, res=h, ldr=d, flags=GEMM_GATE_RES, workspace=ws)
             ops.rmsnorm(h, n, w["ln2"], d, rows, eps=self.eps)
             ops.gemm(n, w["wi"], ff, rows, 2 * dff, d, d, d, 2 * dff, gelu_from=dff, workspace=ws)
