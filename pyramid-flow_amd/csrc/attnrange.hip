@@ -67,12 +67,13 @@ PF_DEVICE Vis load_vis(const RArgs& p, int b, int row) {
         return v;
     }
     const long long at = b * p.range_bs + row;
-    v.alo = max(p.a_lo[at], 0);
-    v.na = max(min(p.a_hi[at], p.Lk) - v.alo, 0);
+    const auto inside = [&](int x) { return min(max(x, 0), p.Lk); };          // any integers: clipped before they are subtracted
+    v.alo = inside(p.a_lo[at]);
+    v.na = max(inside(p.a_hi[at]) - v.alo, 0);
     if (v.na == 0) v.alo = 0;
     if (p.b_lo) {
-        v.blo = max(p.b_lo[at], 0);
-        v.nb = max(min(p.b_hi[at], p.Lk) - v.blo, 0);
+        v.blo = inside(p.b_lo[at]);
+        v.nb = max(inside(p.b_hi[at]) - v.blo, 0);
         if (v.nb == 0) v.blo = 0;
     }
     return v;
@@ -289,8 +290,10 @@ PF_DEVICE float score2(const RArgs& p, float z, int h, int dist, float& slope) {
     const float t = __builtin_fmaf(x, p.zs, p.shift);
     return p.bias ? t + bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(dist, -p.R), p.R) + p.R]) : t;
 }
-// positions in front of every key by more than any radius count alike: differences stay inside 32 bits
-PF_DEVICE int row_pos(const RArgs& p, int b, int row) { return p.q_pos ? max(p.q_pos[b * p.pos_bs + row], 4096 - (1 << 30)) : row + p.Lk - p.Lq; }
+// positions in front of or behind every key by more than any radius count alike: differences stay inside 32 bits
+PF_DEVICE int row_pos(const RArgs& p, int b, int row) {
+    return p.q_pos ? min(max(p.q_pos[b * p.pos_bs + row], 4096 - (1 << 30)), (1 << 30) + 4096) : row + p.Lk - p.Lq;
+}
 
 template <int D>
 PF_DEVICE float dot_row(const bf16_t* a, const bf16_t* b) {
@@ -1202,9 +1205,39 @@ PF_DEVICE void add_diagonals(const f32x16_t& dt, float* skew, float* hist, int R
     }
 }
 
+// The same for rows at any positions: a row's distances differ, so row after row the lanes (keys now) add to distinct entries.
+PF_DEVICE void add_rowwise(const f32x16_t& dt, float* skew, float* hist, int R, int key0, int pos, float& below, float& above) {
+    const int lane = threadIdx.x & 63, hi = lane >> 5, r = lane & 15;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        if (((lane >> 4) & 1) == half) {
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                f32x4_t w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = dt[4 * q4 + e];
+                *(f32x4_t*)(skew + 32 + 64 * r + 8 * q4 + 4 * hi) = w;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int i = 0; i < 16; ++i) {
+            const int d = key0 + lane - __builtin_amdgcn_readlane(pos, 16 * half + i);
+            if (lane < 32) {
+                const float a = skew[32 + 64 * i + lane];
+                if (d <= -R) below += a;
+                else if (d >= R) above += a;
+                else hist[d + R] += a;
+            }
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
+}
+
 // dQ of 128 rows of one head (a wave's 32 rows held in registers; KS = 2: 64 rows, as in the forward kernel) over its key tiles, and this workgroup's part of dbias: every
-// wave adds dT of its pairs into a table of its own (by diagonals, or pair by pair where positions are not consecutive: LDS adds
-// of one wave run in program order; pairs behind the table's ends are summed in registers), the tables are added in wave order.
+// wave adds dT of its pairs into a table of its own (pairs behind the table's ends are summed in registers), the tables are added in
+// wave order: no atomics, the same bits every time.
 template <int D, int MODE, int KS>
 __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
@@ -1318,13 +1351,7 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
                 } else if (in_line) {
                     add_diagonals(s, skew, hist, p.R, j0 + 32 * i - pos0, below, above);
                 } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int d = k0 + reg_row(r) - pos;
-                        if (d <= -p.R) below += s[r];
-                        else if (d >= p.R) above += s[r];
-                        else __hip_atomic_fetch_add(hist + d + p.R, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                    }
+                    add_rowwise(s, skew, hist, p.R, j0 + 32 * i, pos, below, above);
                 }
             }
             if (CAP && BIAS) {
@@ -1407,6 +1434,7 @@ const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
     if (d->Lq > (1 << 30) || d->Lk > (1 << 30)) return "pf_attention_ranges: more than 2^30 rows or keys";
     if (!(d->scale - d->scale == 0.f) || d->scale <= 0.f) return "pf_attention_ranges: scale must be positive and finite";
     if (!(d->cap >= 0.f) || d->cap > 1e30f) return "pf_attention_ranges: cap must be 0 (none) or positive and finite";
+    if (d->cap > 0.f && !(d->scale / d->cap < 1e30f)) return "pf_attention_ranges: cap too small for this scale";
     if ((d->a_lo == nullptr) != (d->a_hi == nullptr) || (d->b_lo == nullptr) != (d->b_hi == nullptr) || (d->b_lo && !d->a_lo))
         return "pf_attention_ranges: a range needs its start and its end, the second one the first";
     if (d->range_batch < 0 || d->q_pos_batch < 0) return "pf_attention_ranges: negative stride";

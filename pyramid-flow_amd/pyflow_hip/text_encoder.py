@@ -153,6 +153,8 @@ class T5EncoderHIP:
         dev = self.device
         ids = input_ids.to(device=dev, dtype=torch.int32).contiguous()
         if long:
+            if attention_mask is not None and attention_mask.shape != input_ids.shape:
+                raise ValueError("T5EncoderHIP: attention_mask and input_ids must have one shape")
             ranges = None if attention_mask is None else KeyRanges.from_key_mask(attention_mask, L, dev)
             bias = self.bias_table()
         else:

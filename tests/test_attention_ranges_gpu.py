@@ -33,6 +33,10 @@ def _ranges(kind, B, Lq, Lk, g):
     r[1][:, ::7] = r[0][:, ::7]
     r[3][:, ::7] = r[2][:, ::7] - 2
     r[1][:, 1::7] = r[2][:, 1::7]
+    i = torch.iinfo(torch.int32)
+    if Lq > 20:                                   # the ends of the type, alone and against each other
+        r[0][:, 5], r[1][:, 5], r[0][:, 6], r[1][:, 6] = i.max, i.min, i.min, i.max
+        r[2][:, 12], r[3][:, 12], r[2][:, 13], r[3][:, 13] = i.min, i.max, i.max, i.min
     return KeyRanges(*[t.cuda() for t in r])
 
 
@@ -55,6 +59,8 @@ def _case(B, Lq, Lk, H, Hkv, D, kind, radius, cap, seed=0, layout="dense", pos=F
     ranges = _ranges(kind, B, Lq, Lk, g)
     bias = torch.randn(H, 2 * radius + 1, generator=g) * 2 if radius is not None else None
     q_pos = torch.randint(-3, Lk + 3, (B, Lq), generator=g).int() if pos else None
+    if pos:
+        q_pos[:, 3], q_pos[:, 4], q_pos[:, 8] = torch.iinfo(torch.int32).max, torch.iinfo(torch.int32).min, 1 << 30
     how = dict(ranges=ranges, bias=None if bias is None else bias.cuda(), q_pos=None if q_pos is None else q_pos.cuda(), cap=cap)
     ref = dict(mask=None if ranges is None else ranges.dense_mask(Lk).cpu(), bias=bias, pos=q_pos, cap=cap)
     return (q, k, v), dev, how, ref, g
@@ -101,6 +107,9 @@ MANY = [  # enough workgroups of 128 rows for the first form
     (3, 200, 200, 48, 12, 64, "documents", 9, 25.0),
     (8, 128, 64, 32, 32, 128, "padded", 64, 0.0),
     (2, 385, 385, 40, 8, 64, "prefix", None, 0.0),
+    (8, 130, 130, 64, 64, 64, "random", 33, 0.0),         # 128-row workgroups at either head size from here on
+    (8, 140, 90, 64, 16, 64, "documents causal", None, 12.0),
+    (4, 70, 200, 128, 32, 128, "random", None, 20.0),
     (4, 130, 130, 32, 8, 128, "random", 100, 300.0),
     (4, 150, 150, 32, 32, 64, "causal", 30, 0.0),
 ]
@@ -171,7 +180,8 @@ def test_no_keys_no_rows(H, Lq):
     assert db.abs().max() == 0
 
 
-@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(1, 66, 130, 2, 1, 64), (1, 1, 130, 4, 2, 128), (2, 130, 130, 128, 64, 64), (2, 3, 2000, 4, 2, 64)])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(1, 66, 130, 2, 1, 64), (1, 1, 130, 4, 2, 128), (2, 130, 130, 128, 64, 64), (2, 3, 2000, 4, 2, 64),
+                                             (8, 130, 130, 64, 64, 64), (4, 70, 100, 128, 64, 128)])
 def test_hidden_values_do_not_matter(B, Lq, Lk, H, Hkv, D):
     """infinities and NaN in keys that a row does not see change none of its bits' meaning: rows that see them get NaN, others
     their own result"""
@@ -214,6 +224,32 @@ def test_hidden_values_do_not_matter(B, Lq, Lk, H, Hkv, D):
     want = attention_grad64(do, *clean, out.cpu(), lse.cpu(), mask=r2.dense_mask(Lk).cpu())
     for name, got in (("dq", dq), ("dk", dk), ("dv", dv)):
         assert within(got, *want[name]) <= 1, name
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D,radius,cap", [
+    (1, 40, 300, 2, 2, 64, None, 0.0), (2, 130, 300, 128, 64, 64, None, 0.0), (8, 130, 300, 64, 64, 64, 5, 0.0),
+    (4, 70, 200, 128, 32, 128, None, 0.0), (2, 130, 300, 64, 64, 64, None, 800.0)])
+def test_scores_that_outgrow_the_first_tile(B, Lq, Lk, H, Hkv, D, radius, cap):
+    """later keys whose weights exceed those of the first keys by 2^200 and more: sums and results stay finite, in every form; also
+    for rows that see the first tile only, and with keys in falling order"""
+    from pyflow_hip.plan import KeyRanges
+    host, dev, how, ref, g = _case(B, Lq, Lk, H, Hkv, D, None, radius, cap, seed=11)
+    how["cap"] = ref["cap"] = cap
+    rise = torch.linspace(0, 1, Lk)[None, :, None, None] if Lq != 70 else torch.linspace(1, 0, Lk)[None, :, None, None]
+    q = torch.sign(host[0].float() + 0.01) * 6
+    k = (q[:, :1, ::H // Hkv].expand(B, Lk, Hkv, D) * rise * (8 * 300 / 36 / D) + host[1].float() * 0.1).bfloat16()
+    q = (q[:, :1].expand(B, Lq, H, D) + host[0].float() * 0.2).bfloat16()
+    hi = torch.full((B, Lq), Lk).int()
+    hi[:, ::5] = 20
+    ranges = KeyRanges(torch.zeros_like(hi).cuda(), hi.cuda())
+    how["ranges"], ref["mask"] = ranges, ranges.dense_mask(Lk).cpu()
+    host = (q, k, host[2])
+    out, lse = _forward([t.cuda() for t in host], how)
+    want, want_lse, bound = attention64(*host, **ref)
+    assert (want_lse.max() - want_lse.min()) > 150
+    # scores of several hundred carry 2^-24 of themselves into every weight
+    assert within(out, want, bound + 2.0 ** -22 * want_lse.abs().max() * host[2].float().abs().max()) <= 1
+    assert within(lse, want_lse, torch.full((), 2.0 ** -20).double() * want_lse.abs().max()) <= 1
 
 
 def test_hidden_distances():

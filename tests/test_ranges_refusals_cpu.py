@@ -28,7 +28,7 @@ BAD = [
     (dict(D=96), b"head_dim"), (dict(D=0), b"head_dim"), (dict(H=3), b"multiple of the key heads"), (dict(Hkv=0), b"key heads"),
     (dict(B=-1), b"negative"), (dict(Lk=-1), b"negative"), (dict(Lq=(1 << 30) + 1), b"2^30"), (dict(scale=0.0), b"scale"),
     (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"), (dict(scale=-1.0), b"scale"),
-    (dict(cap=-1.0), b"cap"), (dict(cap=float("nan")), b"cap"), (dict(cap=float("inf")), b"cap"),
+    (dict(cap=-1.0), b"cap"), (dict(cap=float("nan")), b"cap"), (dict(cap=float("inf")), b"cap"), (dict(cap=1e-38), b"cap too small"),
     (dict(a_lo=64), b"range"), (dict(b_lo=64, b_hi=64), b"range"), (dict(range_batch=-1), b"stride"),
     (dict(bias=64, bias_radius=513), b"radius"), (dict(bias=64, bias_radius=-1), b"radius"), (dict(dbias=64), b"without a bias"),
 ]
