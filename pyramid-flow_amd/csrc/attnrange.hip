@@ -6,7 +6,7 @@
 //     backward   dV = P^T dO, dP = dO V^T, dT = P (dP - delta), delta = sum_c dO O, dbias = sum of dT by distance,
 //                dZ = dT (1 - (c / cap)^2), dQ = scale dZ K, dK = scale dZ^T Q
 // Scores live in base 2 (t log2 e), maxima and sums in 32 bits; P and dZ are rounded to bf16 once, as operands of the next
-// matrix product (half a step of 2^-9 per weight, the size of the rounding of the result itself).
+// matrix product (at most 2^-8 of each weight, like the rounding of the result itself).
 //
 // All products are 32 x 32 x 16 MFMAs in the "swapped" form: the result of the first product has the long axis of the second
 // one's contraction in its registers (rows 4 (l / 32) + 8 (r / 4) + r % 4 of lane l, register r), which is how the second
@@ -15,7 +15,8 @@
 // are XOR-swizzled by row so that both kinds of reads hit all banks (swz below).
 //
 // A hidden key must not reach a row's result even as 0 x inf: the matrix products cannot tell, so a result row that came out
-// non-finite although some of the row's keys were hidden is recomputed by a plain loop over its visible keys (exact_*).
+// non-finite although some of the row's keys were hidden (by a range or by the bias) is recomputed by a plain loop over its
+// visible keys (exact_*), which ends early where every channel is NaN anyway.
 #include <type_traits>
 #include "common.h"
 #include "pyflow_hip.h"
@@ -282,13 +283,15 @@ PF_DEVICE float capped(const RArgs& p, float z, float& slope) {
     }
 }
 PF_DEVICE float bias2(float b) { return b <= HIDDEN ? -__builtin_inff() : b * LOG2E; }
+// a hidden distance hides a score that is not finite, too
+PF_DEVICE float with_bias(float t, float b) { return b == -__builtin_inff() ? b : t + b; }
 
 // base-2 score of one pair from global memory (exact_* and nothing else)
 PF_DEVICE float score2(const RArgs& p, float z, int h, int dist, float& slope) {
     slope = 1.f;
     const float x = p.cap2 == 0.f ? z : p.series ? capped<5>(p, z, slope) : capped<1>(p, z, slope);
     const float t = __builtin_fmaf(x, p.zs, p.shift);
-    return p.bias ? t + bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(dist, -p.R), p.R) + p.R]) : t;
+    return p.bias ? with_bias(t, bias2(p.bias[(long long)h * (2 * p.R + 1) + min(max(dist, -p.R), p.R) + p.R])) : t;
 }
 // positions in front of or behind every key by more than any radius count alike: differences stay inside 32 bits
 PF_DEVICE int row_pos(const RArgs& p, int b, int row) {
@@ -322,6 +325,13 @@ PF_DEVICE void add_rows(const bf16_t* base, long long ld, int j0, unsigned long 
         for (int c = 0; c < D / 64; ++c) acc[c] = __builtin_fmaf(wt, (float)r[c], acc[c]);
     }
 }
+// a NaN stays one: nothing that is added later changes the row any more
+template <int D>
+PF_DEVICE bool all_nan(const float* acc) {
+    bool nan = acc[0] != acc[0];
+    if (D == 128) nan = nan && acc[1] != acc[1];
+    return __builtin_amdgcn_ballot_w64(!nan) == 0;
+}
 template <int D>
 PF_DEVICE void store_row(bf16_t* row, const float* acc) {
     const int lane = threadIdx.x & 63;
@@ -350,6 +360,7 @@ PF_DEVICE void exact_o(const RArgs& p, int b, int h, int i, float m, float l) {
             w = __builtin_amdgcn_exp2f(t - m) / l;
         }
         add_rows<D>(V, p.v.ld, j0, __builtin_amdgcn_ballot_w64(use), w, acc);
+        if (all_nan<D>(acc)) break;
     }
     store_row<D>(p.o.p + b * p.o.bs + i * p.o.ld + h * p.o.hs, acc);
 }
@@ -379,6 +390,7 @@ PF_DEVICE void exact_dq(const RArgs& p, int b, int h, int i) {
         float P = 0.f, dz = 0.f;
         if (use) use = exact_pair<D>(p, b, h, hk, i, j, P, dz);
         add_rows<D>(p.k.p + b * p.k.bs + hk * p.k.hs, p.k.ld, j0, __builtin_amdgcn_ballot_w64(use), dz * p.dscale, acc);
+        if (all_nan<D>(acc)) break;
     }
     store_row<D>(p.dq.p + b * p.dq.bs + i * p.dq.ld + h * p.dq.hs, acc);
 }
@@ -386,8 +398,9 @@ template <int D>
 PF_DEVICE void exact_dkv(const RArgs& p, int b, int hk, int j) {
     const int lane = threadIdx.x & 63;
     float ak[2] = {0.f, 0.f}, av[2] = {0.f, 0.f};
-    for (int h = hk * p.G; h < (hk + 1) * p.G; ++h)
-        for (int i0 = 0; i0 < p.Lq; i0 += 64) {
+    bool done = false;
+    for (int h = hk * p.G; h < (hk + 1) * p.G && !done; ++h)
+        for (int i0 = 0; i0 < p.Lq && !done; i0 += 64) {
             const int i = i0 + lane;
             bool use = i < p.Lq && sees(load_vis(p, b, i), j);
             if (__builtin_amdgcn_ballot_w64(use) == 0) continue;
@@ -396,6 +409,7 @@ PF_DEVICE void exact_dkv(const RArgs& p, int b, int hk, int j) {
             const unsigned long long m = __builtin_amdgcn_ballot_w64(use);
             add_rows<D>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, i0, m, dz * p.dscale, ak);
             add_rows<D>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, i0, m, P, av);
+            done = all_nan<D>(ak) && all_nan<D>(av);
         }
     store_row<D>(p.dk.p + b * p.dk.bs + j * p.dk.ld + hk * p.dk.hs, ak);
     store_row<D>(p.dv.p + b * p.dv.bs + j * p.dv.ld + hk * p.dv.hs, av);
@@ -425,9 +439,9 @@ PF_DEVICE bool any_nonfinite(const f32x16_t* o) {
     return t != t;
 }
 
-// The bias table of head h in LDS, base 2 (or times `unit`), continued by PAD entries of its end values on both sides: a 32 x 64 block of consecutive
-// rows whose distances are not all behind an end stays inside it, so its entries lie at fixed offsets from one address per
-// lane (a subtraction, a clamp and an address per score otherwise).  Returned: the entry of distance 0.
+// The bias table of head h in LDS, base 2 (or times `unit`), continued by PAD entries of its end values on both sides: a 32 x 64
+// block of consecutive rows whose distances are not all behind an end stays inside it, so its entries lie at fixed offsets from one
+// address per lane (a subtraction, a clamp and an address per score otherwise).  Returned: the entry of distance 0.
 constexpr int PAD = 96;
 constexpr int table_floats(int R) { return 2 * R + 1 + 2 * PAD; }
 PF_DEVICE const float* load_table(const RArgs& p, int h, float* tab, float unit = LOG2E) {
@@ -454,7 +468,7 @@ PF_DEVICE void cap_only(const RArgs& p, f32x16_t& s) {
         }
     }
 }
-// x -> x zs + bias; d0 = distance of this lane's register 0 (SIGN 1: registers are keys, -1: rows), lo, hi = of the block
+// x -> x zs + bias (a NaN stays one even where the bias hides it: what comes out of it is not finite, and is done again with care); d0 = distance of this lane's register 0 (SIGN 1: registers are keys, -1: rows), lo, hi = of the block
 template <int SIGN>
 PF_DEVICE void add_bias(const RArgs& p, f32x16_t& s, float zs, const float* tab, int d0, int lo, int hi) {
     const Reach how = reach(p.R, lo, hi);
@@ -524,7 +538,7 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
     f32x16_t o[D / 32];
     float m, l;
-    bool whole;                                    // wave-uniform: no row of the wave had a hidden key in any tile
+    bool whole;                                    // wave-uniform: no row of the wave had a hidden key in any tile (a bias may hide some)
     auto issue = [&](int n) {
         const int j0 = tl.at(n) * KB;
         char* buf = smem + (n & 1) * BUF;
@@ -546,7 +560,7 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
         for (int c = 0; c < D / 32; ++c) o[c] = zero16();
         m = -__builtin_inff();
         l = 0.f;
-        whole = true;
+        whole = !BIAS;
         unsigned long long fresh = __builtin_amdgcn_ballot_w64(vis.na + vis.nb > 0);     // rows without a reference yet
         if (CAREFUL) {
             drain_barrier();                       // nobody reads the first pass's tiles any more
@@ -574,6 +588,15 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
             for (int i = 0; i < NI; ++i) {
                 cap_only<MODE>(p, s[i]);
                 if (BIAS) add_bias<1>(p, s[i], p.zs, tab, j0 + 32 * i + 4 * hi - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
+            }
+            if (CAREFUL && BIAS) {                 // NaN + -inf: hidden
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float b = tab[min(max(j0 + 32 * i + 4 * hi + reg_row(r) - pos, -p.R), p.R)];
+                        s[i][r] = b == -__builtin_inff() ? b : s[i][r];
+                    }
             }
             if (!full) {
 #pragma unroll
@@ -741,7 +764,7 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
         for (int r = 0; r < 16; ++r) {
             float slope;
             float t = capped<MODE>(p, s[r], slope) * p.zs;
-            if (BIAS) t += far ? (j0 + 31 - pmin <= -p.R ? far_below : far_above) : bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]);
+            if (BIAS) t = with_bias(t, far ? (j0 + 31 - pmin <= -p.R ? far_below : far_above) : bias2(bias[min(max(k0 + reg_row(r) - pos, -p.R), p.R)]));
             s[r] = sees(vis, k0 + reg_row(r)) ? t : -__builtin_inff();
         }
         float mt = s[0];
@@ -867,8 +890,9 @@ __global__ __launch_bounds__(256) void range_join_kernel(const RArgs p) {
 
 // ---------------------------------------------------------------------------------------------- backward
 // What both gradient kernels need of a row, in 1-KiB pieces of 64 rows that the LDS-DMA can take as they are: log-sum-exp (base 2,
-// less the scores' shift) and -delta = -sum_c dO O per head, the ranges per batch entry; and for each such tile the bounds of its ranges: 0..3 the smallest
-// start and largest end of the a and b ranges that are not empty, 4..7 the largest start and smallest end over ALL its rows.
+// less the scores' shift) and -delta = -sum_c dO O per head, the ranges per batch entry; and for each such tile the bounds of its
+// ranges: 0..3 the smallest start and largest end of the a and b ranges that are not empty, 4..7 the largest start and smallest
+// end over ALL its rows.
 template <int D>
 __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
     const int qt = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
@@ -1018,6 +1042,7 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
     };
     Item cur = pop();
     int buf = 0, table_of = -1;
+    bool whole = !BIAS;                             // as in the forward kernel, with rows and keys exchanged
     if (cur.g >= 0) issue(cur, 0);
     while (cur.g >= 0) {
         drain_barrier();
@@ -1029,6 +1054,7 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
         const Item nxt = follow(cur);
         if (nxt.g >= 0) issue(nxt, buf ^ 1);
         if (cur.any) {
+            whole = whole && cur.full;
             const char* sq = smem + buf * BUF;
             const char* so = sq + TILE;
             const float* st = (const float*)(sq + 2 * TILE) + cur.half * RT;
@@ -1130,7 +1156,7 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
         }
         return;
     }
-    const bool bad = key < p.Lk && (any_nonfinite<D / 32>(dk) || any_nonfinite<D / 32>(dv));
+    const bool bad = key < p.Lk && !whole && (any_nonfinite<D / 32>(dk) || any_nonfinite<D / 32>(dv));
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
     redo = (redo | (redo >> 32)) & 0xffffffffull;
     if (key < p.Lk && !((redo >> (lane & 31)) & 1)) {
@@ -1235,9 +1261,9 @@ PF_DEVICE void add_rowwise(const f32x16_t& dt, float* skew, float* hist, int R, 
     }
 }
 
-// dQ of 128 rows of one head (a wave's 32 rows held in registers; KS = 2: 64 rows, as in the forward kernel) over its key tiles, and this workgroup's part of dbias: every
-// wave adds dT of its pairs into a table of its own (pairs behind the table's ends are summed in registers), the tables are added in
-// wave order: no atomics, the same bits every time.
+// dQ of 128 rows of one head (a wave's 32 rows held in registers; KS = 2: 64 rows, as in the forward kernel) over its key tiles, and
+// this workgroup's part of dbias: every wave adds dT of its pairs into a table of its own (pairs behind the table's ends are summed
+// in registers), the tables are added in wave order: no atomics, the same bits every time.
 template <int D, int MODE, int KS>
 __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
@@ -1297,7 +1323,7 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     const int pmin = BIAS ? wave_min(pos) : 0, pmax = BIAS ? wave_max(pos) : 0;
     const int pos0 = __builtin_amdgcn_readfirstlane(pos);
     const bool in_line = __builtin_amdgcn_ballot_w64(row < p.Lq && pos != pos0 + (lane & 31)) == 0;
-    bool whole = true;
+    bool whole = !BIAS;                             // as in the forward kernel
     for (int n = 0; n < tl.n; ++n) {
         drain_barrier();
         if (n + 1 < tl.n) issue(n + 1);
@@ -1408,7 +1434,8 @@ __global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
     }
 }
 
-// dbias[h][i] = sum over batch entries and row tiles of the parts, in order: 64 entries per workgroup, 4 groups of parts
+// dbias[h][i] = sum over batch entries and row tiles of the parts, in order: 64 entries per workgroup, 4 groups of parts.  A hidden
+// distance has none, whatever keys that are not finite left there.
 __global__ __launch_bounds__(256) void range_dbias_kernel(const RArgs p) {
     __shared__ float red[4][64];
     const int NB = 2 * p.R + 1, i = blockIdx.x * 64 + (threadIdx.x & 63), h = blockIdx.y, grp = threadIdx.x >> 6;
@@ -1417,7 +1444,7 @@ __global__ __launch_bounds__(256) void range_dbias_kernel(const RArgs p) {
         for (int u = grp; u < p.B * p.nqt; u += 4) a += p.dbias_parts[(((long long)(u / p.nqt) * p.H + h) * p.nqt + u % p.nqt) * NB + i];
     red[grp][threadIdx.x & 63] = a;
     __syncthreads();
-    if (grp == 0 && i < NB) p.dbias[(long long)h * NB + i] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    if (grp == 0 && i < NB) p.dbias[(long long)h * NB + i] = p.bias[(long long)h * NB + i] <= HIDDEN ? 0.f : (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
 }
 
 // ---------------------------------------------------------------------------------------------- host side

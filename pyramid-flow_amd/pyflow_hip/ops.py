@@ -320,7 +320,7 @@ def _rows(view, t, shape, what, out=False):
         raise ValueError(f"{what}: expected bfloat16 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
     sb, sr, sh, sc = t.stride()
     p = t.data_ptr()
-    if sc != 1 or (sb | sr | sh) & 7 or p & 15 or (out and not (sb and sr and sh)):
+    if sc != 1 or (sb | sr | sh) & 7 or p & 15 or sr >= 1 << 25 or (out and not (sb and sr and sh)):
         if not t.numel():
             return
         if sc != 1:

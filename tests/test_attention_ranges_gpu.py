@@ -267,6 +267,49 @@ def test_hidden_distances():
         _check_backward(host, dev, how, ref, g)
 
 
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(1, 70, 150, 2, 1, 64), (2, 130, 200, 128, 64, 64), (8, 130, 200, 64, 64, 64), (4, 70, 100, 128, 64, 128),
+                                             (1, 1, 150, 2, 1, 128)])
+def test_values_behind_hidden_distances_do_not_matter(B, Lq, Lk, H, Hkv, D):
+    """infinities and NaN at keys that the bias alone hides, and in the gradients of rows that it hides from a key"""
+    from pyflow_hip import ops
+    host, dev, how, ref, g = _case(B, Lq, Lk, H, Hkv, D, None, 8, 0.0, seed=13)
+    for t in (how["bias"], ref["bias"]):
+        t[:, 9:] = -math.inf                      # later keys, from the first on
+    last = Lk - 1                                 # seen by the last row alone
+    clean = [t.clone() for t in host]
+    for n, t in ((1, clean[1]), (2, clean[2])):
+        dev[n][:, last] = float("nan") if n == 1 else float("inf")
+        t[:, last] = 0
+    out, lse = _forward(dev, how)
+    want, want_lse, bound = attention64(*clean, **ref)
+    if Lq > 1:
+        assert within(out[:, :-1], want[:, :-1], bound[:, :-1]) <= 1
+    assert torch.isnan(out[:, -1]).all()
+    # the last row (the only one that may see the last key) has a gradient that is not finite: keys it does not see do not notice.  It
+    # sees all keys but those of a hidden distance, so hide the near ones from it: the keys behind Lk - 6
+    if Lq == 1:
+        return
+    for t in (how["bias"], ref["bias"]):
+        t[:, 3:] = -math.inf                      # distances beyond -6 hidden
+    dev2 = [t.cuda() for t in host]
+    for n in (1, 2):
+        dev2[n][:, last] = dev[n][:, last]        # nobody sees it now
+    out, lse = _forward(dev2, how)
+    do = torch.randn(host[0].shape, generator=g).bfloat16()
+    dq, dk, dv, db = torch.empty_like(dev2[0]), torch.empty_like(dev2[1]), torch.empty_like(dev2[1]), torch.empty_like(how["bias"])
+    ops.attention_ranges_backward(do.cuda(), *dev2, out, lse, dq, dk, dv, dbias=db, **how)
+    grads = attention_grad64(do, *clean, out.cpu(), lse.cpu(), **ref)
+    for name, got in (("dq", dq), ("dk", dk), ("dv", dv), ("dbias", db)):
+        assert within(got, *grads[name]) <= 1, name
+    do2 = do.cuda()
+    do2[:, -1] = float("inf")
+    ops.attention_ranges_backward(do2, *dev2, out, lse, dq, dk, dv, **how)
+    seen = Lk - 6                                 # keys that the last row sees
+    for name, got, part in (("dq", dq, slice(0, Lq - 1)), ("dk", dk, slice(seen, Lk)), ("dv", dv, slice(seen, Lk))):
+        assert within(got[:, part], *[x[:, part] for x in grads[name]]) <= 1, name
+    assert not torch.isfinite(dv[:, :seen]).any()
+
+
 def _check_backward(host, dev, how, ref, g, **more):
     from pyflow_hip import ops
     q, k, v = host
