@@ -1042,7 +1042,6 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
     };
     Item cur = pop();
     int buf = 0, table_of = -1;
-    bool whole = !BIAS;                             // as in the forward kernel, with rows and keys exchanged
     if (cur.g >= 0) issue(cur, 0);
     while (cur.g >= 0) {
         drain_barrier();
@@ -1054,7 +1053,6 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
         const Item nxt = follow(cur);
         if (nxt.g >= 0) issue(nxt, buf ^ 1);
         if (cur.any) {
-            whole = whole && cur.full;
             const char* sq = smem + buf * BUF;
             const char* so = sq + TILE;
             const float* st = (const float*)(sq + 2 * TILE) + cur.half * RT;
@@ -1156,8 +1154,16 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
         }
         return;
     }
-    const bool bad = key < p.Lk && !whole && (any_nonfinite<D / 32>(dk) || any_nonfinite<D / 32>(dv));
+    const bool bad = key < p.Lk && (any_nonfinite<D / 32>(dk) || any_nonfinite<D / 32>(dv));
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
+    if (!BIAS && redo != 0) {                      // only tiles with hidden pairs can have brought in what does not belong there
+        unsigned long long partial = 0;
+        for (int n = 0; n < nq; n += 64) {
+            test(n);
+            partial |= some & ~all;
+        }
+        if (partial == 0) redo = 0;
+    }
     redo = (redo | (redo >> 32)) & 0xffffffffull;
     if (key < p.Lk && !((redo >> (lane & 31)) & 1)) {
         store_cols<D>(p.dk.p + b * p.dk.bs + key * p.dk.ld + hk * p.dk.hs, dk, p.dscale);
