@@ -48,6 +48,7 @@ struct RArgs {
     int series;
     int D, B, H, Hk, G, Lq, Lk;
     int nqt, nkt, nrb, nsplit;
+    int key_wgs, key_pad;              // backward: workgroups for the key gradients, the first of those for the row gradients
     float* parts;                      // split forward: [unit][split][32][D + 2]
     float* stat;                       // backward: [B][H][nq64][4][64] lse log2 e - shift, -delta, position, the tile's positions
     int* vis;                          // backward: [B][nq64][4][64] the rows' ranges (Vis)
@@ -933,6 +934,273 @@ __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
     }
 }
 
+// one wave per key: the parts' dK and dV, added in part order
+template <int D>
+__global__ __launch_bounds__(256) void range_kvjoin_kernel(const RArgs p) {
+    const int lane = threadIdx.x & 63;
+    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), keys = (long long)p.B * p.Hk * p.Lk;
+    if (w >= keys) return;
+    const int bk = (int)(w / p.Lk), j = (int)(w - (long long)bk * p.Lk), b = bk / p.Hk, hk = bk - b * p.Hk;
+    float k[2] = {0.f, 0.f}, v[2] = {0.f, 0.f};
+    for (int s = 0; s < p.kv_split; ++s) {
+        const float* a = p.kv_parts + (s * keys + w) * (2 * D) + lane * (D / 64);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) { k[c] += a[c]; v[c] += a[D + c]; }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+        bad = bad || !(fabsf(k[c]) < __builtin_inff()) || !(fabsf(v[c]) < __builtin_inff());
+        k[c] *= p.dscale;
+    }
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+        exact_dkv<D>(p, b, hk, j);
+        return;
+    }
+    store_row<D>(p.dk.p + b * p.dk.bs + j * p.dk.ld + hk * p.dk.hs, k);
+    store_row<D>(p.dv.p + b * p.dv.bs + j * p.dv.ld + hk * p.dv.hs, v);
+}
+
+// Adds the 32 x 32 block dT (lane: row lane % 32, keys in registers) to the wave's table of distances.  Rows that follow one another
+// make every distance a diagonal: 16 rows at a time go to LDS with 32 columns of zeros between them, and lane l sums diagonal
+// l - 15 without a test.  d0 = distance of key 0 of the block from row 0.  (One LDS float add per pair instead: about 200 cycles per
+// instruction, 57 us for the query gradients of 2 x 12 heads x 301 rows instead of 30.)
+constexpr int SKEW = 16 * 64 + 64;                          // floats per wave
+PF_DEVICE void add_diagonals(const f32x16_t& dt, float* skew, float* hist, int R, int d0, float& below, float& above) {
+    const int lane = threadIdx.x & 63, hi = lane >> 5, r = lane & 15;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        if (((lane >> 4) & 1) == half) {
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                f32x4_t w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = dt[4 * q4 + e];
+                *(f32x4_t*)(skew + 32 + 64 * r + 8 * q4 + 4 * hi) = w;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (lane < 47) {
+            float a = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) a += skew[32 + 65 * i + lane - 15];
+            const int d = d0 - 16 * half + lane - 15;
+            if (d <= -R) below += a;
+            else if (d >= R) above += a;
+            else hist[d + R] += a;
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+// The same for rows at any positions: a row's distances differ, so row after row the lanes (keys now) add to distinct entries.
+PF_DEVICE void add_rowwise(const f32x16_t& dt, float* skew, float* hist, int R, int key0, int pos, float& below, float& above) {
+    const int lane = threadIdx.x & 63, hi = lane >> 5, r = lane & 15;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        if (((lane >> 4) & 1) == half) {
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                f32x4_t w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = dt[4 * q4 + e];
+                *(f32x4_t*)(skew + 32 + 64 * r + 8 * q4 + 4 * hi) = w;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int i = 0; i < 16; ++i) {
+            const int d = key0 + lane - __builtin_amdgcn_readlane(pos, 16 * half + i);
+            if (lane < 32) {
+                const float a = skew[32 + 64 * i + lane];
+                if (d <= -R) below += a;
+                else if (d >= R) above += a;
+                else hist[d + R] += a;
+            }
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
+}
+
+// dQ of 128 rows of one head (a wave's 32 rows held in registers; KS = 2: 64 rows, as in the forward kernel) over its key tiles, and
+// this workgroup's part of dbias: every wave adds dT of its pairs into a table of its own (pairs behind the table's ends are summed
+// in registers), the tables are added in wave order: no atomics, the same bits every time.
+template <int D, int MODE, int KS>
+PF_DEVICE void row_gradients(const RArgs& p, int block) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
+    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE, RW = 4 / KS, NI = 2 / KS;
+    int* const red = (int*)(smem + 2 * BUF);
+    float* const meet = (float*)(red + 16);                         // KS = 2: [row wave] whole
+    float* const tab_ = meet + 4;
+    const int NB = 2 * p.R + 1, TS = (table_floats(p.R) + 3) / 4 * 4;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
+    float* const hists = tab_ + TS;
+    float* const hist = hists + wid * NB;
+    float* const skew = hists + (4 * NB + 3) / 4 * 4 + wid * SKEW;
+    const Place at = heavy_first(block, p.nqt, p.nqt * p.H * p.B);
+    const int bh = at.head, qt = p.nqt - 1 - at.rank;
+    const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+    const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31), rc = min(row, p.Lq - 1);
+    const Vis vis = load_vis(p, b, row);
+    const int pos = BIAS ? row_pos(p, b, rc) : 0;
+    const Bounds wb = wave_bounds(vis);
+    const TileList tl = workgroup_tiles<64>(wb, red, wid, lane);
+    const Stager<D, 64, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
+    const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
+    const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
+    auto issue = [&](int n) {
+        const int j0 = tl.at(n) * 64;
+        char* buf = smem + (n & 1) * BUF;
+        sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
+        sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
+    };
+    if (tl.n > 0) issue(0);                        // the first tile is on its way before the rows are read
+    const float* const tab = BIAS ? load_table(p, h, tab_, 1.f) : nullptr;
+    if (BIAS && p.dbias) {
+        for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
+        for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
+    }
+    bf16x8_t qf[D / 16], of[D / 16];
+    {
+        const bf16_t* q = p.q.p + b * p.q.bs + rc * p.q.ld + h * p.q.hs + hi * 8;
+        const bf16_t* g = p.dO.p + b * p.dO.bs + rc * p.dO.ld + h * p.dO.hs + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            qf[ks] = *(const bf16x8_t*)(q + ks * 16);
+            of[ks] = *(const bf16x8_t*)(g + ks * 16);
+        }
+    }
+    const float* const st = p.stat + (((long long)b * p.H + h) * p.nq64 + (rc >> 6)) * 256 + (rc & 63);
+    const float ls = st[0], de = st[64];                            // log-sum-exp (base 2, less the shift), -delta
+    // dbias is a 32-bit result: with a bias the scores stay in natural units here, so that only their difference from the row's lse
+    // is rounded again by the change of base (lse, cap and bias times log2 e leave 5e-7 each, the same for whole rows and distances)
+    const float lse = BIAS ? p.lse[((long long)b * p.H + h) * p.Lq + rc] - p.shift_n : 0.f;
+    const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
+    f32x16_t dq[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dq[c] = zero16();
+    float below = 0.f, above = 0.f;                 // dbias of distances <= -R and >= R
+    const int pmin = BIAS ? wave_min(pos) : 0, pmax = BIAS ? wave_max(pos) : 0;
+    const int pos0 = __builtin_amdgcn_readfirstlane(pos);
+    const bool in_line = __builtin_amdgcn_ballot_w64(row < p.Lq && pos != pos0 + (lane & 31)) == 0;
+    bool whole = !BIAS;                             // as in the forward kernel
+    for (int n = 0; n < tl.n; ++n) {
+        drain_barrier();
+        if (n + 1 < tl.n) issue(n + 1);
+        const int j0 = tl.at(n) * 64 + kw * 32 * NI;                // this wave's keys of the tile
+        const char* sk = smem + (n & 1) * BUF + kw * NI * 64 * D;
+        const char* sv = sk + TILE;
+        const bool full = wb.full(j0, j0 + 32 * NI);
+        if (!full) {
+            whole = false;
+            if (!wb.any(j0, j0 + 32 * NI)) continue;
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            f32x16_t s = zero16(), dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = de;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+                s = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s);
+                dp = mfma(row_frag<D>(sv, roff, i, ks), of[ks], dp);
+            }
+            const int k0 = j0 + 32 * i + 4 * hi;
+            f32x16_t fac;                                           // dbias wants dT without the slope
+            if (CAP) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float slope;
+                    s[r] = capped<MODE>(p, s[r], slope);
+                    if (BIAS) fac[r] = slope;
+                    else dp[r] *= slope;
+                }
+            }
+            if (BIAS) add_bias<1>(p, s, p.zn, tab, k0 - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                if (BIAS) s[r] = s[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((s[r] - lse) * LOG2E) * dp[r];
+                else s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls)) * dp[r];
+            }
+            if (!full) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = sees(vis, k0 + reg_row(r)) ? s[r] : 0.f;
+            }
+            if (BIAS && p.dbias) {
+                const int lo = j0 + 32 * i - pmax, hi_ = j0 + 32 * i + 31 - pmin;     // distances of this block, wave-uniform
+                if (hi_ <= -p.R || lo >= p.R) {
+                    float a = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) a += s[r];
+                    if (lo >= p.R) above += a;
+                    else below += a;
+                } else if (in_line) {
+                    add_diagonals(s, skew, hist, p.R, j0 + 32 * i - pos0, below, above);
+                } else {
+                    add_rowwise(s, skew, hist, p.R, j0 + 32 * i, pos, below, above);
+                }
+            }
+            if (CAP && BIAS) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] *= fac[r];
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const bf16x8_t zf = half_of(s, g);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) dq[c] = mfma(tr_frag<D>(sk, t0, t8, c, 2 * i + g), zf, dq[c]);
+            }
+        }
+    }
+    if constexpr (KS == 2) {
+        float* const acc = (float*)smem + rw * (D / 32) * 16 * 64;
+        __syncthreads();
+        if (kw == 1) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[(c * 16 + r) * 64 + lane] = dq[c][r];
+            if (lane == 0) meet[rw] = whole ? 1.f : 0.f;
+        }
+        __syncthreads();
+        if (kw == 0) {
+            whole = whole && meet[rw] != 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dq[c][r] += acc[(c * 16 + r) * 64 + lane];
+        }
+    }
+    const bool store = row < p.Lq && kw == 0;
+    const bool bad = any_nonfinite<D / 32>(dq) && !whole && store;
+    unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
+    redo = (redo | (redo >> 32)) & 0xffffffffull;
+    if (store && !((redo >> (lane & 31)) & 1)) store_cols<D>(p.dq.p + b * p.dq.bs + row * p.dq.ld + h * p.dq.hs, dq, p.dscale);
+    while (redo) {
+        const int i = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        exact_dq<D>(p, b, h, row0 + i);
+    }
+    if (BIAS && p.dbias) {
+        below = wave_add(below);
+        above = wave_add(above);
+        if (lane == 0) {
+            hist[0] = below;
+            hist[2 * p.R] = p.R == 0 ? below + above : above;
+        }
+        __syncthreads();
+        float* out = p.dbias_parts + ((long long)bh * p.nqt + qt) * NB;
+        for (int i = threadIdx.x; i < NB; i += 256) out[i] = (hists[i] + hists[NB + i]) + (hists[2 * NB + i] + hists[3 * NB + i]);
+    }
+}
+
+template <int D, int MODE, int KS>
+__global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) { row_gradients<D, MODE, KS>(p, blockIdx.x); }
+
 // dK, dV of 128 keys of one key head: 4 waves x 32 keys, looping over the row tiles (of every query head that shares the key head)
 // that see any of them.  The bounds of 64 tiles are tested at once (one lane each); the next tile is in flight while one is used.
 // -delta enters through the C operand of the dP product.  kv_split > 1: this workgroup takes an even part of the (head, tile)
@@ -943,13 +1211,20 @@ __global__ __launch_bounds__(256) void range_prep_kernel(const RArgs p) {
 // 48 us at 2 x 12 heads of 301 rows).  D = 128 has twice the results (128 registers): 32-row tiles and V in LDS leave room for
 // a second workgroup (with V in registers and 64-row tiles one wave per SIMD ran everything in series, 8400 cycles per tile,
 // 800 of its instructions register moves).
+//
+// Neither gradient needs the other: small problems run both in this launch (BOTH), where the row workgroups fill what the key
+// workgroups leave of the chip; the number of key workgroups is padded to the XCDs, so that a block's place tells its XCD in both.
 template <int D, int MODE>
 constexpr bool KV_V_LDS = D == 128 || !(MODE & 2);
-template <int D, int MODE>
+template <int D, int MODE, bool BOTH>
 __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv_kernel(const RArgs p) {
+    if constexpr (BOTH) {
+        if ((int)blockIdx.x >= p.key_pad) return row_gradients<D, MODE, 2>(p, blockIdx.x - p.key_pad);
+        if ((int)blockIdx.x >= p.key_wgs) return;
+    }
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2, VLDS = KV_V_LDS<D, MODE>;
     constexpr int RT = D == 64 ? 64 : 32, HALVES = 64 / RT, TILE = RT * 2 * D, BUF = 2 * TILE + 2048, VTILE = VLDS ? 32 * 2 * D : 0;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     char* const vtile = smem + 2 * BUF + wid * VTILE;
     float* const tab_ = (float*)(smem + 2 * BUF + 4 * VTILE);
@@ -1176,270 +1451,6 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
     }
 }
 
-// one wave per key: the parts' dK and dV, added in part order
-template <int D>
-__global__ __launch_bounds__(256) void range_kvjoin_kernel(const RArgs p) {
-    const int lane = threadIdx.x & 63;
-    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), keys = (long long)p.B * p.Hk * p.Lk;
-    if (w >= keys) return;
-    const int bk = (int)(w / p.Lk), j = (int)(w - (long long)bk * p.Lk), b = bk / p.Hk, hk = bk - b * p.Hk;
-    float k[2] = {0.f, 0.f}, v[2] = {0.f, 0.f};
-    for (int s = 0; s < p.kv_split; ++s) {
-        const float* a = p.kv_parts + (s * keys + w) * (2 * D) + lane * (D / 64);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) { k[c] += a[c]; v[c] += a[D + c]; }
-    }
-    bool bad = false;
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-        bad = bad || !(fabsf(k[c]) < __builtin_inff()) || !(fabsf(v[c]) < __builtin_inff());
-        k[c] *= p.dscale;
-    }
-    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
-        exact_dkv<D>(p, b, hk, j);
-        return;
-    }
-    store_row<D>(p.dk.p + b * p.dk.bs + j * p.dk.ld + hk * p.dk.hs, k);
-    store_row<D>(p.dv.p + b * p.dv.bs + j * p.dv.ld + hk * p.dv.hs, v);
-}
-
-// Adds the 32 x 32 block dT (lane: row lane % 32, keys in registers) to the wave's table of distances.  Rows that follow one another
-// make every distance a diagonal: 16 rows at a time go to LDS with 32 columns of zeros between them, and lane l sums diagonal
-// l - 15 without a test.  d0 = distance of key 0 of the block from row 0.  (One LDS float add per pair instead: about 200 cycles per
-// instruction, 57 us for the query gradients of 2 x 12 heads x 301 rows instead of 30.)
-constexpr int SKEW = 16 * 64 + 64;                          // floats per wave
-PF_DEVICE void add_diagonals(const f32x16_t& dt, float* skew, float* hist, int R, int d0, float& below, float& above) {
-    const int lane = threadIdx.x & 63, hi = lane >> 5, r = lane & 15;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        if (((lane >> 4) & 1) == half) {
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                f32x4_t w;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = dt[4 * q4 + e];
-                *(f32x4_t*)(skew + 32 + 64 * r + 8 * q4 + 4 * hi) = w;
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (lane < 47) {
-            float a = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) a += skew[32 + 65 * i + lane - 15];
-            const int d = d0 - 16 * half + lane - 15;
-            if (d <= -R) below += a;
-            else if (d >= R) above += a;
-            else hist[d + R] += a;
-        }
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-}
-
-// The same for rows at any positions: a row's distances differ, so row after row the lanes (keys now) add to distinct entries.
-PF_DEVICE void add_rowwise(const f32x16_t& dt, float* skew, float* hist, int R, int key0, int pos, float& below, float& above) {
-    const int lane = threadIdx.x & 63, hi = lane >> 5, r = lane & 15;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        if (((lane >> 4) & 1) == half) {
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                f32x4_t w;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = dt[4 * q4 + e];
-                *(f32x4_t*)(skew + 32 + 64 * r + 8 * q4 + 4 * hi) = w;
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        for (int i = 0; i < 16; ++i) {
-            const int d = key0 + lane - __builtin_amdgcn_readlane(pos, 16 * half + i);
-            if (lane < 32) {
-                const float a = skew[32 + 64 * i + lane];
-                if (d <= -R) below += a;
-                else if (d >= R) above += a;
-                else hist[d + R] += a;
-            }
-            __builtin_amdgcn_wave_barrier();
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
-    }
-}
-
-// dQ of 128 rows of one head (a wave's 32 rows held in registers; KS = 2: 64 rows, as in the forward kernel) over its key tiles, and
-// this workgroup's part of dbias: every wave adds dT of its pairs into a table of its own (pairs behind the table's ends are summed
-// in registers), the tables are added in wave order: no atomics, the same bits every time.
-template <int D, int MODE, int KS>
-__global__ __launch_bounds__(256, 2) void range_dq_kernel(const RArgs p) {
-    constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
-    constexpr int TILE = 64 * 2 * D, BUF = 2 * TILE, RW = 4 / KS, NI = 2 / KS;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    int* const red = (int*)(smem + 2 * BUF);
-    float* const meet = (float*)(red + 16);                         // KS = 2: [row wave] whole
-    float* const tab_ = meet + 4;
-    const int NB = 2 * p.R + 1, TS = (table_floats(p.R) + 3) / 4 * 4;
-    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
-    float* const hists = tab_ + TS;
-    float* const hist = hists + wid * NB;
-    float* const skew = hists + (4 * NB + 3) / 4 * 4 + wid * SKEW;
-    const Place at = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
-    const int bh = at.head, qt = p.nqt - 1 - at.rank;
-    const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
-    const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31), rc = min(row, p.Lq - 1);
-    const Vis vis = load_vis(p, b, row);
-    const int pos = BIAS ? row_pos(p, b, rc) : 0;
-    const Bounds wb = wave_bounds(vis);
-    const TileList tl = workgroup_tiles<64>(wb, red, wid, lane);
-    const Stager<D, 64, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
-    const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
-    const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
-    auto issue = [&](int n) {
-        const int j0 = tl.at(n) * 64;
-        char* buf = smem + (n & 1) * BUF;
-        sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
-        sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
-    };
-    if (tl.n > 0) issue(0);                        // the first tile is on its way before the rows are read
-    const float* const tab = BIAS ? load_table(p, h, tab_, 1.f) : nullptr;
-    if (BIAS && p.dbias) {
-        for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
-        for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
-    }
-    bf16x8_t qf[D / 16], of[D / 16];
-    {
-        const bf16_t* q = p.q.p + b * p.q.bs + rc * p.q.ld + h * p.q.hs + hi * 8;
-        const bf16_t* g = p.dO.p + b * p.dO.bs + rc * p.dO.ld + h * p.dO.hs + hi * 8;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            qf[ks] = *(const bf16x8_t*)(q + ks * 16);
-            of[ks] = *(const bf16x8_t*)(g + ks * 16);
-        }
-    }
-    const float* const st = p.stat + (((long long)b * p.H + h) * p.nq64 + (rc >> 6)) * 256 + (rc & 63);
-    const float ls = st[0], de = st[64];                            // log-sum-exp (base 2, less the shift), -delta
-    // dbias is a 32-bit result: with a bias the scores stay in natural units here, so that only their difference from the row's lse
-    // is rounded again by the change of base (lse, cap and bias times log2 e leave 5e-7 each, the same for whole rows and distances)
-    const float lse = BIAS ? p.lse[((long long)b * p.H + h) * p.Lq + rc] - p.shift_n : 0.f;
-    const unsigned roff = row_offset<D>(lane), t0 = tr_offset<D>(lane, 0), t8 = tr_offset<D>(lane, 8);
-    f32x16_t dq[D / 32];
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) dq[c] = zero16();
-    float below = 0.f, above = 0.f;                 // dbias of distances <= -R and >= R
-    const int pmin = BIAS ? wave_min(pos) : 0, pmax = BIAS ? wave_max(pos) : 0;
-    const int pos0 = __builtin_amdgcn_readfirstlane(pos);
-    const bool in_line = __builtin_amdgcn_ballot_w64(row < p.Lq && pos != pos0 + (lane & 31)) == 0;
-    bool whole = !BIAS;                             // as in the forward kernel
-    for (int n = 0; n < tl.n; ++n) {
-        drain_barrier();
-        if (n + 1 < tl.n) issue(n + 1);
-        const int j0 = tl.at(n) * 64 + kw * 32 * NI;                // this wave's keys of the tile
-        const char* sk = smem + (n & 1) * BUF + kw * NI * 64 * D;
-        const char* sv = sk + TILE;
-        const bool full = wb.full(j0, j0 + 32 * NI);
-        if (!full) {
-            whole = false;
-            if (!wb.any(j0, j0 + 32 * NI)) continue;
-        }
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            f32x16_t s = zero16(), dp;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) dp[r] = de;
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-                s = mfma(row_frag<D>(sk, roff, i, ks), qf[ks], s);
-                dp = mfma(row_frag<D>(sv, roff, i, ks), of[ks], dp);
-            }
-            const int k0 = j0 + 32 * i + 4 * hi;
-            f32x16_t fac;                                           // dbias wants dT without the slope
-            if (CAP) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float slope;
-                    s[r] = capped<MODE>(p, s[r], slope);
-                    if (BIAS) fac[r] = slope;
-                    else dp[r] *= slope;
-                }
-            }
-            if (BIAS) add_bias<1>(p, s, p.zn, tab, k0 - pos, j0 + 32 * i - pmax, j0 + 32 * i + 31 - pmin);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                if (BIAS) s[r] = s[r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((s[r] - lse) * LOG2E) * dp[r];
-                else s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.zs, -ls)) * dp[r];
-            }
-            if (!full) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = sees(vis, k0 + reg_row(r)) ? s[r] : 0.f;
-            }
-            if (BIAS && p.dbias) {
-                const int lo = j0 + 32 * i - pmax, hi_ = j0 + 32 * i + 31 - pmin;     // distances of this block, wave-uniform
-                if (hi_ <= -p.R || lo >= p.R) {
-                    float a = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) a += s[r];
-                    if (lo >= p.R) above += a;
-                    else below += a;
-                } else if (in_line) {
-                    add_diagonals(s, skew, hist, p.R, j0 + 32 * i - pos0, below, above);
-                } else {
-                    add_rowwise(s, skew, hist, p.R, j0 + 32 * i, pos, below, above);
-                }
-            }
-            if (CAP && BIAS) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] *= fac[r];
-            }
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const bf16x8_t zf = half_of(s, g);
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) dq[c] = mfma(tr_frag<D>(sk, t0, t8, c, 2 * i + g), zf, dq[c]);
-            }
-        }
-    }
-    if constexpr (KS == 2) {
-        float* const acc = (float*)smem + rw * (D / 32) * 16 * 64;
-        __syncthreads();
-        if (kw == 1) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[(c * 16 + r) * 64 + lane] = dq[c][r];
-            if (lane == 0) meet[rw] = whole ? 1.f : 0.f;
-        }
-        __syncthreads();
-        if (kw == 0) {
-            whole = whole && meet[rw] != 0.f;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) dq[c][r] += acc[(c * 16 + r) * 64 + lane];
-        }
-    }
-    const bool store = row < p.Lq && kw == 0;
-    const bool bad = any_nonfinite<D / 32>(dq) && !whole && store;
-    unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
-    redo = (redo | (redo >> 32)) & 0xffffffffull;
-    if (store && !((redo >> (lane & 31)) & 1)) store_cols<D>(p.dq.p + b * p.dq.bs + row * p.dq.ld + h * p.dq.hs, dq, p.dscale);
-    while (redo) {
-        const int i = __builtin_ctzll(redo);
-        redo &= redo - 1;
-        exact_dq<D>(p, b, h, row0 + i);
-    }
-    if (BIAS && p.dbias) {
-        below = wave_add(below);
-        above = wave_add(above);
-        if (lane == 0) {
-            hist[0] = below;
-            hist[2 * p.R] = p.R == 0 ? below + above : above;
-        }
-        __syncthreads();
-        float* out = p.dbias_parts + ((long long)bh * p.nqt + qt) * NB;
-        for (int i = threadIdx.x; i < NB; i += 256) out[i] = (hists[i] + hists[NB + i]) + (hists[2 * NB + i] + hists[3 * NB + i]);
-    }
-}
-
 // dbias[h][i] = sum over batch entries and row tiles of the parts, in order: 64 entries per workgroup, 4 groups of parts.  A hidden
 // distance has none, whatever keys that are not finite left there.
 __global__ __launch_bounds__(256) void range_dbias_kernel(const RArgs p) {
@@ -1511,14 +1522,16 @@ long long fwd_bytes(const pf_attn_ranges_desc* d) {
     return s > 1 ? (long long)row_blocks(d) * d->Hkv * d->B * s * 32 * (d->D + 2) * 4 : 0;
 }
 long long up16(long long n) { return (n + 15) / 16 * 16; }
-// the (head, row tile) list of a key block in parts where the key blocks alone leave compute units empty: four tiles per part at least
+// The (head, row tile) list of a key block in n parts: the longest chain shrinks as tiles / n (0.8 .. 1.3 us per tile), the parts'
+// traffic grows as n units (128 keys, 8 D bytes each way: 26 .. 52 ns), so n = sqrt(25 tiles / units).  Whole gradients at 8 heads
+// of 2000 rows over 2 key heads of 128: n = 8 96 us, 16 126 us; 12 heads over 3 of 4 x 300 rows of 64: n = 1 78 us, 2 53 us, 5 40 us;
+// 16 heads of 2 x 1000 rows of 64: n = 1 52 us, 2 58 us, 3 66 us.
 int kv_splits(const pf_attn_ranges_desc* d) {
     if (!d->B || !d->H || !d->Lk || !d->Lq) return 1;
     const long long units = (long long)((d->Lk + 127) / 128) * d->Hkv * d->B, tiles = (long long)((d->Lq + 63) / 64) * (d->H / d->Hkv);
-    long long n = 1024 / units;
-    if (n > tiles / 4) n = tiles / 4;
-    if (n > 16) n = 16;
-    return (int)(n < 1 ? 1 : n);
+    long long n = 1, most = 768 / units < 32 ? 768 / units : 32;
+    while (n < most && (2 * n + 1) * (2 * n + 1) * units <= 100 * tiles) ++n;      // rounded
+    return (int)n;
 }
 struct BwdSizes { long long stat, vis, tiles, parts, kv; long long all() const { return stat + vis + tiles + parts + kv; } };
 BwdSizes bwd_sizes(const pf_attn_ranges_desc* d) {
@@ -1586,11 +1599,20 @@ int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
     return 0;
 }
 
+template <int D, int MODE>
+int lds_dq(int R) { return 4 * 64 * 2 * D + 80 + (MODE & 2 ? (table_floats(R) + 3 + 4 * (2 * R + 1) + 3 + 4 * SKEW) * 4 : 0); }
+template <int D, int MODE, bool BOTH>
+int lds_dkv(int R) {
+    const int rt = D == 64 ? 64 : 32, rows = BOTH ? lds_dq<D, MODE>(R) : 0;
+    const int keys = 2 * (2 * rt * 2 * D + 2048) + (KV_V_LDS<D, MODE> ? 4 * 32 * 2 * D : 0) + (MODE & 2 ? table_floats(R) * 4 : 0);
+    return keys > rows ? keys : rows;
+}
+
 template <int D, int MODE, int KS>
-int launch_dq(const RArgs& a, hipStream_t stream) {
-    auto lds = [](int R) { return 4 * 64 * 2 * D + 80 + (MODE & 2 ? (table_floats(R) + 3 + 4 * (2 * R + 1) + 3 + 4 * SKEW) * 4 : 0); };
-    PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE, KS>), lds(MAX_RADIUS));
-    range_dq_kernel<D, MODE, KS><<<(unsigned)(a.nqt * a.H * a.B), 256, (size_t)lds(a.R), stream>>>(a);
+int launch_dq(const RArgs& a, unsigned row_wgs, hipStream_t stream) {
+    if (row_wgs == 0) return 0;
+    PF_SET_MAX_LDS_ONCE((range_dq_kernel<D, MODE, KS>), (lds_dq<D, MODE>(MAX_RADIUS)));
+    range_dq_kernel<D, MODE, KS><<<row_wgs, 256, (size_t)lds_dq<D, MODE>(a.R), stream>>>(a);
     CHECK_LAUNCH();
     return 0;
 }
@@ -1601,19 +1623,27 @@ int launch_bwd(const RArgs& a, hipStream_t stream) {
         range_prep_kernel<D><<<dim3((a.Lq + 63) / 64, a.H, a.B), 256, 0, stream>>>(a);
         CHECK_LAUNCH();
     }
-    if (a.Lk > 0) {
-        const int rt = D == 64 ? 64 : 32;
-        const size_t lds = 2 * (2 * rt * 2 * D + 2048) + (KV_V_LDS<D, MODE> ? 4 * 32 * 2 * D : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
-        PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, MODE>), (int)lds);
-        range_dkv_kernel<D, MODE><<<(unsigned)(a.nkt * a.kv_split * a.Hk * a.B), 256, lds, stream>>>(a);
-        CHECK_LAUNCH();
-        if (a.kv_split > 1) {
-            range_kvjoin_kernel<D><<<(unsigned)(((long long)a.B * a.Hk * a.Lk + 3) / 4), 256, 0, stream>>>(a);
+    const unsigned row_wgs = (unsigned)(a.nqt * a.H * a.B);
+    const bool small = small_dq(a.D, a.Lq, a.H, a.B);
+    // with D = 128 and a bias the row workgroups' LDS would leave one key workgroup per compute unit
+    constexpr bool BOTH = D == 64 || !(MODE & 2);
+    if (BOTH && small) {
+        if (a.key_wgs + row_wgs > 0) {
+            PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, MODE, BOTH>), (lds_dkv<D, MODE, BOTH>(MAX_RADIUS)));
+            range_dkv_kernel<D, MODE, BOTH><<<a.key_pad + row_wgs, 256, (size_t)lds_dkv<D, MODE, BOTH>(a.R), stream>>>(a);
             CHECK_LAUNCH();
         }
+    } else {
+        if (a.key_wgs > 0) {
+            PF_SET_MAX_LDS_ONCE((range_dkv_kernel<D, MODE, false>), (lds_dkv<D, MODE, false>(MAX_RADIUS)));
+            range_dkv_kernel<D, MODE, false><<<(unsigned)a.key_wgs, 256, (size_t)lds_dkv<D, MODE, false>(a.R), stream>>>(a);
+            CHECK_LAUNCH();
+        }
+        if (const int rc = BOTH || !small ? launch_dq<D, MODE, 1>(a, row_wgs, stream) : launch_dq<D, MODE, BOTH ? 1 : 2>(a, row_wgs, stream)) return rc;
     }
-    if (a.Lq > 0) {
-        return small_dq(a.D, a.Lq, a.H, a.B) ? launch_dq<D, MODE, 2>(a, stream) : launch_dq<D, MODE, 1>(a, stream);
+    if (a.kv_split > 1) {
+        range_kvjoin_kernel<D><<<(unsigned)(((long long)a.B * a.Hk * a.Lk + 3) / 4), 256, 0, stream>>>(a);
+        CHECK_LAUNCH();
     }
     return 0;
 }
@@ -1671,7 +1701,7 @@ extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t
     if (need && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need))
         return pf_set_err("pf_attention_ranges_bwd: workspace missing, unaligned or too small");
     if (d->B > 65535 || d->H > 65535) return pf_set_err("pf_attention_ranges_bwd: more than 65535 batch entries or heads");
-    if ((long long)row_groups(d->Lq, true) * d->H * d->B > 0x7fffffffLL || (long long)((d->Lk + 127) / 128) * d->H * d->B * 16 > 0x7fffffffLL ||
+    if ((long long)row_groups(d->Lq, true) * d->H * d->B + (long long)((d->Lk + 127) / 128) * d->H * d->B * 16 > 0x7fffff00LL ||
         (long long)(d->Lq + 63) / 64 * (d->H / (d->Hkv ? d->Hkv : 1)) > 0x7fffffffLL)
         return pf_set_err("pf_attention_ranges_bwd: too many workgroups");
     if (!d->H) return 0;
@@ -1683,6 +1713,8 @@ extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t
     a.dbias_parts = (float*)(w += s.tiles);
     a.kv_parts = (float*)(w += s.parts);
     a.kv_split = kv_splits(d);
+    a.key_wgs = a.nkt * a.kv_split * a.Hk * a.B;
+    a.key_pad = (a.key_wgs + 7) / 8 * 8;
     a.nqt = row_groups(d->Lq, small_dq(d->D, d->Lq, d->H, d->B));
     a.dbias = d->dbias;
     int rc = 0;
