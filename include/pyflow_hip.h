@@ -386,7 +386,7 @@ int pf_qk_norm_rope_axes_bwd(const pf_heads_desc* d, float* dwq, float* dwk, voi
  *   (natural logarithm of sum exp t) or NULL.  D = 64 or 128.  O may be Q.
  *   workspace: pf_attention_ranges_workspace_bytes(d) bytes, 16-byte aligned (0 for most calls: only problems with few rows
  *   split the keys); not shared by launches that may overlap.  Rows of a tensor lie less than 2^25 elements apart.
- * pf_attention_ranges_which: 1 = 128 rows of one head per workgroup, 2 = 32 (row, head) pairs of one key head per workgroup with the
+ * pf_attention_ranges_which: 1 = 128 or 64 rows of one head per workgroup, 2 = 32 (row, head) pairs of one key head per workgroup with the
  *   keys split over waves and workgroups, -1 = invalid descriptor.
  * pf_attention_ranges_bwd: given dO, O, LSE of the forward, writes dQ, dK, dV and (dbias != NULL) the bias's gradient fp32
  *   [H][2 R + 1]; the same bits every time.  Gradients of shared key heads are summed over their H / Hkv query heads.  Rows that

@@ -426,6 +426,53 @@ def test_graphs_streams_and_workspaces():
             assert all(torch.equal(x, y) for x, y in zip(got, eager)), n
 
 
+@pytest.mark.parametrize("D,cap", [(64, 0.0), (128, 30.0)])
+def test_decoding_through_a_graph(D, cap):
+    """norm + rotation of one new token per request, its key and value into the cache, attention over the cache: captured once,
+    replayed token after token with the lengths and positions advanced on the device; the rest of the cache holds NaN"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import KeyRanges, RopeAxes
+    B, S, H, Hkv = 3, 2500, 8, 2
+    g = torch.Generator().manual_seed(21)
+    start = torch.tensor([0, 130, 2400])
+    k_cache, v_cache = (torch.full((B, S, Hkv, D), float("nan"), dtype=torch.bfloat16) for _ in range(2))
+    for b, n in enumerate(start):
+        k_cache[b, :n], v_cache[b, :n] = torch.randn(n, Hkv, D, generator=g).bfloat16(), torch.randn(n, Hkv, D, generator=g).bfloat16()
+    k_cache, v_cache = k_cache.cuda(), v_cache.cuda()
+    rope = RopeAxes.build([D], "cuda", halves=True)
+    wq, wk = torch.full((D,), 1.5, device="cuda"), torch.full((D,), 0.5, device="cuda")
+    zeros, lengths = torch.zeros(B, 1, dtype=torch.int32, device="cuda"), start.int()[:, None].cuda()
+    pos = lengths[..., None].float()
+    q, k, v = (torch.zeros(B, 1, n, D, dtype=torch.bfloat16, device="cuda") for n in (H, Hkv, Hkv))
+    out, lse, ranges = torch.empty_like(q), torch.empty(B, H, 1, device="cuda"), KeyRanges(zeros, lengths)
+    workspace, rows = torch.empty(1 << 24, dtype=torch.uint8, device="cuda"), torch.arange(B, device="cuda")
+
+    def step():
+        ops.qk_norm_rope_axes(q, k, q, k, wq, wk, rope, pos)
+        k_cache[rows, lengths[:, 0].long()], v_cache[rows, lengths[:, 0].long()] = k[:, 0], v[:, 0]
+        lengths.add_(1)
+        pos.add_(1)
+        ops.attention_ranges(q, k_cache, v_cache, out, ranges=ranges, cap=cap, lse=lse, workspace=workspace)
+    graph = None
+    for n in range(5):
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g).bfloat16())
+        fresh = q.clone()
+        if n == 1:                                # the first token ran as it is; capturing runs nothing
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+        graph.replay() if graph else step()
+        torch.cuda.synchronize()
+        assert (lengths[:, 0].cpu() == start + n + 1).all()
+        assert not torch.equal(fresh, q) and torch.isfinite(out).all()
+        seen = torch.arange(S)[None, None] < (start + n + 1)[:, None, None]
+        clean = [torch.where(seen[:, 0, :, None, None], c.cpu(), torch.zeros((), dtype=torch.bfloat16)) for c in (k_cache, v_cache)]
+        want, want_lse, bound = attention64(q.cpu(), *clean, mask=seen, cap=cap)
+        assert within(out, want, bound) <= 1, n
+        assert (lse.double().cpu() - want_lse).abs().max() <= 1e-4, n
+
+
 def test_wrapper_refusals():
     from pyflow_hip import ops
     from pyflow_hip.plan import KeyRanges
