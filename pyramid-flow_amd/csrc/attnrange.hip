@@ -491,9 +491,14 @@ PF_DEVICE void add_bias(const RArgs& p, f32x16_t& s, float zs, const float* tab,
 // half of each head's tiles -- the ones that causal and frame-wise masks make long -- for all of its heads and then the second
 // halves: the launch ends on short workgroups.  Tile numbers here count from the heavy end.  (Head after head instead: 1415, now
 // 1308 us for 30 heads of the 15488-row video sequence; 1500, now 1333 us for the gradients at 7808 rows.)
+//
+// `resident` > 0: the first workgroups of an XCD go to its 32 compute units in turn, so those that start together on one unit are 32
+// apart; every other 32 come in reverse, which pairs long ones with short ones.
 struct Place { int head, rank; };
-PF_DEVICE Place heavy_first(int block, int n, int nwg) {
-    const int q = nwg >> 3, r = nwg & 7, xcd = block & 7, i = block >> 3;
+PF_DEVICE Place heavy_first(int block, int n, int nwg, int resident = 0) {
+    const int q = nwg >> 3, r = nwg & 7, xcd = block & 7;
+    int i = block >> 3;
+    if (((i >> 5) & 1) && (i >> 5) < resident && (i | 31) < q) i ^= 31;
     const int c0 = xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q, c1 = c0 + q + (xcd < r ? 1 : 0);
     const int nh = (n + 1) / 2, nl = n - nh;
     auto heavy_below = [&](int c) { const int w = c / n; return w * nh + min(c - w * n, nh); };
@@ -501,6 +506,34 @@ PF_DEVICE Place heavy_first(int block, int n, int nwg) {
     const bool heavy = i < hn;
     const int k = heavy ? h0 + i : (c0 - h0) + (i - hn), m = heavy ? nh : nl, w = k / m;
     return {w, k - w * m + (heavy ? 0 : nh)};
+}
+
+// The row tile (of ROWS rows) that comes at place `rank` when a head's tiles start in falling order of their keys: `sort` and at most
+// 256 tiles.  One thread per tile takes the larger count of its first and last row and counts the tiles before it, the same in every
+// workgroup of the batch entry.  Otherwise the tiles come from the sequence's end on.  `mem`: 1028 bytes of LDS, free again behind
+// the caller's next barrier.  Sorted where a launch is one to three rounds of workgroups: with fewer all start at once, with more the
+// unevenness fades and the sorting costs 1 % (16 heads of 128, 8000 rows packed of 5 documents: 127 instead of 137 us, of 12: 63
+// instead of 79 us).
+template <int ROWS>
+PF_DEVICE int ranked_tile(const RArgs& p, int b, int rank, bool sort, int* mem) {
+    if (!sort || !p.a_lo || p.nqt > 256) return p.nqt - 1 - rank;
+    const int t = threadIdx.x;
+    int mine = -1;
+    if (t < p.nqt) {
+        const Vis x = load_vis(p, b, t * ROWS), y = load_vis(p, b, min(t * ROWS + ROWS, p.Lq) - 1);
+        mine = min(max(x.na + x.nb, y.na + y.nb) >> 2, (1 << 23) - 1) << 8 | t;
+    }
+    mem[t] = mine;
+    __syncthreads();
+    int before = 0;
+    for (int i = 0; i < (p.nqt + 3) / 4; ++i) {
+        const u32x4_t k = *(const u32x4_t*)(mem + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) before += (int)k[e] > mine;
+    }
+    if (t < p.nqt && before == rank) mem[256] = t;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(mem[256]);
 }
 
 // ---------------------------------------------------------------------------------------------- forward, many rows
@@ -523,9 +556,11 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     float* const meet = (float*)(smem + 2 * BUF + 80);           // KS = 2: [row wave][3][64] maximum, sum, whole
     float* const tab_ = meet + (KS == 2 ? RW * 192 : 0);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
-    const Place at = heavy_first(blockIdx.x, p.nqt, p.nqt * p.H * p.B);
-    const int bh = at.head, qt = p.nqt - 1 - at.rank;
-    const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+    constexpr int RESIDENT = FWD_WAVES<D, KS>;       // workgroups of a compute unit
+    const int nwg = p.nqt * p.H * p.B;
+    const Place at = heavy_first(blockIdx.x, p.nqt, nwg, RESIDENT);
+    const int bh = at.head, b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+    const int qt = ranked_tile<32 * RW>(p, b, at.rank, nwg > 256 * RESIDENT && nwg <= 768 * RESIDENT, (int*)smem);
     const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
@@ -1046,8 +1081,8 @@ PF_DEVICE void row_gradients(const RArgs& p, int block) {
     float* const hist = hists + wid * NB;
     float* const skew = hists + (4 * NB + 3) / 4 * 4 + wid * SKEW;
     const Place at = heavy_first(block, p.nqt, p.nqt * p.H * p.B);
-    const int bh = at.head, qt = p.nqt - 1 - at.rank;
-    const int b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+    const int bh = at.head, b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+    const int qt = p.nqt - 1 - at.rank;
     const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31), rc = min(row, p.Lq - 1);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, rc) : 0;
