@@ -1540,10 +1540,11 @@ const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
     return nullptr;
 }
 
-// the form with 32 (row, head) pairs per workgroup and the keys split: where 128-row workgroups would leave compute units empty, and
+// the form with 32 (row, head) pairs per workgroup and the keys split: where even 64-row workgroups would be few (1 x 700 rows over 1400
+// keys of 32 heads of 128, 192 in the count below: 87 us, rows 43; 64 rows over 8000 keys of 16 heads of 64, 16: 25 us, rows 82), and
 // where one block of 32 pairs holds all rows that share a key head (each key is then read once, not once per query head)
 bool few_rows(const pf_attn_ranges_desc* d) {
-    return (long long)((d->Lq + 127) / 128) * d->H * d->B < 256 || (long long)d->Lq * (d->H / d->Hkv) <= 32;
+    return (long long)((d->Lq + 127) / 128) * d->H * d->B < 64 || (long long)d->Lq * (d->H / d->Hkv) <= 32;
 }
 // 64-row workgroups (KS = 2) instead of 128-row ones where those would be few: half the chain per wave for twice the tile traffic.
 // Forward: 21.5 instead of 22 us at 2 x 64 heads of 512 rows of 64; 55 instead of 67 us with 128-row workgroups at 16 x 16 heads of
