@@ -489,8 +489,9 @@ PF_DEVICE void add_bias(const RArgs& p, f32x16_t& s, float zs, const float* tab,
 
 // Which (head, tile) a workgroup takes.  Every XCD has a contiguous run of heads (their K and V stay in its L2), walks the first
 // half of each head's tiles -- the ones that causal and frame-wise masks make long -- for all of its heads and then the second
-// halves: the launch ends on short workgroups.  Tile numbers here count from the heavy end.  (Head after head instead: 1415, now
-// 1308 us for 30 heads of the 15488-row video sequence; 1500, now 1333 us for the gradients at 7808 rows.)
+// halves: the launch ends on short workgroups.  Tile numbers here count from the heavy end.  (Against head after
+// head, at the time: 1308 instead of 1415 us for 30 heads of the 15488-row video sequence, today 1240; gradients at 7808 rows 1333
+// instead of 1500, today 1280.)
 //
 // `resident` > 0: the first workgroups of an XCD go to its 32 compute units in turn, so those that start together on one unit are 32
 // apart; every other 32 come in reverse, which pairs long ones with short ones.
@@ -1249,8 +1250,8 @@ __global__ __launch_bounds__(256, D == 128 && (MODE & 2) && KS == 2 ? 1 : 2) voi
 // -delta enters through the C operand of the dP product.  kv_split > 1: this workgroup takes an even part of the (head, tile)
 // pairs that the keys need and leaves 32-bit sums for range_kvjoin_kernel.
 //
-// D = 64: 64-row tiles, K and both results in registers, V in LDS: three waves per SIMD (1370 us for the whole gradient of 30 heads
-// of the 7808-row video sequence; V in registers and two waves 1430 us; with a bias table the third wave spills: 53 instead of
+// D = 64: 64-row tiles, K and both results in registers, V in LDS: three waves per SIMD (when it was built 1370 us for the whole gradient of 30
+// heads of the 7808-row video sequence; V in registers and two waves 1430 us; with a bias table the third wave spills: 53 instead of
 // 48 us at 2 x 12 heads of 301 rows).  D = 128 has twice the results (128 registers): 32-row tiles and V in LDS leave room for
 // a second workgroup (with V in registers and 64-row tiles one wave per SIMD ran everything in series, 8400 cycles per tile,
 // 800 of its instructions register moves).
