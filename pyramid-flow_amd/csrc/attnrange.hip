@@ -340,9 +340,9 @@ PF_DEVICE void store_row(bf16_t* row, const float* acc) {
     for (int c = 0; c < D / 64; ++c) row[lane * (D / 64) + c] = (bf16_t)acc[c];
 }
 
-// one whole wave: O of row i of head h from its visible keys alone (m: base-2 maximum, l: sum of 2^(t - m))
+// one whole wave: O of row i of head h from its visible keys alone (m: base-2 reference, l: sum of 2^(t - m - e))
 template <int D>
-PF_DEVICE void exact_o(const RArgs& p, int b, int h, int i, float m, float l) {
+PF_DEVICE void exact_o(const RArgs& p, int b, int h, int i, float m, float l, float e = 0.f) {
     const int lane = threadIdx.x & 63, hk = h / p.G;
     const Vis v = load_vis(p, b, i);
     const int pos = row_pos(p, b, i);
@@ -358,7 +358,7 @@ PF_DEVICE void exact_o(const RArgs& p, int b, int h, int i, float m, float l) {
         if (use) {
             const float t = score2(p, dot_row<D>(q, K + j * p.k.ld), h, j - pos, slope);
             use = t != -__builtin_inff();
-            w = __builtin_amdgcn_exp2f(t - m) / l;
+            w = __builtin_amdgcn_exp2f((t - m) - e) / l;
         }
         add_rows<D>(V, p.v.ld, j0, __builtin_amdgcn_ballot_w64(use), w, acc);
         if (all_nan<D>(acc)) break;
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     int* const red = (int*)(smem + 2 * BUF);
     int* const redo_flag = red + 16;
-    float* const meet = (float*)(smem + 2 * BUF + 80);           // KS = 2: [row wave][3][64] maximum, sum, whole
+    float* const meet = (float*)(smem + 2 * BUF + 80);           // KS = 2: [row wave][3][64] reference, sum, its exponent and `whole`
     float* const tab_ = meet + (KS == 2 ? RW * 192 : 0);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
     constexpr int RESIDENT = FWD_WAVES<D, KS>;       // workgroups of a compute unit
@@ -692,8 +692,18 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     if (__builtin_amdgcn_ballot_w64(!(l < __builtin_inff()) || any_nonfinite<D / 32>(o)) != 0 && lane == 0) *redo_flag = 1;
     __syncthreads();
     if (*redo_flag != 0) pass(std::true_type{});   // workgroup-uniform: the passes share tiles and barriers
+    float le = 0.f;                                // the row's sum is l 2^(m + le)
     if constexpr (KS == 2) {
+        // The halves' references are the maxima of their first tiles, not of their rows: a half's sum may lie 2^127 above its own.  So
+        // both are brought to sums in [1/2, 1) first (exact), and the powers of two that were taken out go into the halves' distance:
+        // what is then below 2^-126 of the other half counts for nothing, and no sum can overflow.
         float* const acc = (float*)smem + rw * (D / 32) * 16 * 64;   // the tiles' memory: [row wave][register][lane]
+        const int e1 = __builtin_amdgcn_frexp_expf(l);               // 0 where the half saw no key, or l is not finite
+        l = __builtin_amdgcn_ldexpf(l, -e1);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[c][r] = __builtin_amdgcn_ldexpf(o[c][r], -e1);
         __syncthreads();
         if (kw == 1) {
 #pragma unroll
@@ -702,21 +712,25 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
                 for (int r = 0; r < 16; ++r) acc[(c * 16 + r) * 64 + lane] = o[c][r];
             meet[rw * 192 + lane] = m;
             meet[rw * 192 + 64 + lane] = l;
-            meet[rw * 192 + 128 + lane] = whole ? 1.f : 0.f;
+            meet[rw * 192 + 128 + lane] = (float)(2 * e1 + (whole ? 1 : 0));
         }
         __syncthreads();
         if (kw == 1) return;
-        const float m2 = meet[rw * 192 + lane], l2 = meet[rw * 192 + 64 + lane], mm = fmaxf(m, m2);
-        whole = whole && meet[rw * 192 + 128] != 0.f;
+        const float m2 = meet[rw * 192 + lane], l2 = meet[rw * 192 + 64 + lane];
+        const int w2 = (int)meet[rw * 192 + 128 + lane], e2 = w2 >> 1;
+        whole = whole && (__builtin_amdgcn_readfirstlane(w2) & 1) != 0;
         const bool one = m2 == -__builtin_inff(), two = m == -__builtin_inff();       // only one half saw a key
-        const float f = two ? 0.f : m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm), f2 = one ? 0.f : m2 == mm ? 1.f : __builtin_amdgcn_exp2f(m2 - mm);
-        // a half without a key holds zeros (or 0 x inf of hidden keys, which exact_o sees); a NaN sum has its maximum at -inf
+        const float x = (m - m2) + (float)(e1 - e2);                 // log2 of the halves' ratio, but for a factor of two
+        const bool first = one || x >= 0.f;                          // the half whose scale the row keeps
+        const float f = two ? 0.f : first ? 1.f : __builtin_amdgcn_exp2f(x), f2 = one ? 0.f : first ? __builtin_amdgcn_exp2f(-x) : 1.f;
+        // a half without a key holds zeros (or 0 x inf of hidden keys, which exact_o sees); a NaN sum has its reference at -inf
         l = (two && l == 0.f ? 0.f : two ? l : f * l) + (one ? l2 : f2 * l2);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[c][r] = f * o[c][r] + f2 * acc[(c * 16 + r) * 64 + lane];
-        m = mm;
+        m = first ? m : m2;
+        le = (float)(first ? e1 : e2);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const bool bad = any_nonfinite<D / 32>(o) && !whole && l == l && row < p.Lq;
@@ -725,13 +739,13 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     const bool mine = (redo >> (lane & 31)) & 1;
     if (row < p.Lq) {
         if (!mine) store_cols<D>(p.o.p + b * p.o.bs + row * p.o.ld + h * p.o.hs, o, inv);
-        if (p.lse && hi == 0) p.lse[((long long)b * p.H + h) * p.Lq + row] = l == 0.f ? -__builtin_inff() : (m + p.shift + __builtin_amdgcn_logf(l)) * LN2;
+        if (p.lse && hi == 0) p.lse[((long long)b * p.H + h) * p.Lq + row] = l == 0.f ? -__builtin_inff() : (m + p.shift + (le + __builtin_amdgcn_logf(l))) * LN2;
     }
     while (redo) {
         const int i = __builtin_ctzll(redo);
         redo &= redo - 1;
         exact_o<D>(p, b, h, row0 + i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), i)) + p.shift,
-                   __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), i)));
+                   __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), i)), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(le), i)));
     }
 }
 
