@@ -105,23 +105,38 @@ PF_DEVICE float wave_add(float x) {
     return x;
 }
 
+// the rows of memory that a tile may be filled from: [a0, a1) and [b0, b1) (an empty one: 0, 0)
+struct Cover {
+    int a0, a1, b0, b1;
+    PF_DEVICE bool has(int j) const { return (unsigned)(j - a0) < (unsigned)(a1 - a0) || (unsigned)(j - b0) < (unsigned)(b1 - b0); }
+    PF_DEVICE bool whole(int j0, int j1) const { return (a0 <= j0 && a1 >= j1) || (b0 <= j0 && b1 >= j1); }
+    PF_DEVICE int some(int j0, int j1) const { return max(j0, a0 < j1 && a1 > j0 ? a0 : b0); }      // one of them in [j0, j1), which has one
+};
+PF_DEVICE Cover scalar(const Cover& c) {       // the same in every lane
+    auto one = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    return {one(c.a0), one(c.a1), one(c.b0), one(c.b1)};
+}
 // the key tiles (of KB keys) that a set of rows needs: the union of its two key ranges' tiles, each tile once
 struct TileList {
     int s0, n0, s1, n;                         // tiles s0 .. s0 + n0 - 1, then s1 .. ; n in all
+    Cover keys;
     PF_DEVICE int at(int i) const { return i < n0 ? s0 + i : s1 + (i - n0); }
+    // at no end of a run: all of its keys are in the cover, which the loops then need not keep in registers
+    PF_DEVICE bool inner(int i) const { return i > 0 && i < n - 1 && (unsigned)(i + 1 - n0) > 1u; }
 };
 template <int KB>
 PF_DEVICE TileList tile_list(int amin, int amax, int bmin, int bmax) {
     int as = 0, ae = 0, bs = 0, be = 0;
-    if (amax > amin) { as = amin / KB; ae = (amax + KB - 1) / KB; }
-    if (bmax > bmin) { bs = bmin / KB; be = (bmax + KB - 1) / KB; }
+    Cover keys = {0, 0, 0, 0};
+    if (amax > amin) { as = amin / KB; ae = (amax + KB - 1) / KB; keys.a0 = amin; keys.a1 = amax; }
+    if (bmax > bmin) { bs = bmin / KB; be = (bmax + KB - 1) / KB; keys.b0 = bmin; keys.b1 = bmax; }
     if (ae == as) { as = bs; ae = be; bs = be = 0; }
     if (be > bs) {
         if (bs < as) { int t = as; as = bs; bs = t; t = ae; ae = be; be = t; }
         bs = max(bs, ae);
         be = max(be, bs);
     }
-    return {as, ae - as, bs, (ae - as) + (be - bs)};
+    return {as, ae - as, bs, (ae - as) + (be - bs), keys};
 }
 
 template <int D, int KS>
@@ -143,7 +158,11 @@ PF_DEVICE int swz(int r) {
 
 // Rows [row0, row0 + ROWS) of a head -> LDS, by the NW waves that share the tile.  A lane's 32-bit byte offsets inside a tile are
 // fixed, the tile's base is wave-uniform: no vector arithmetic per tile (64-bit addresses per piece were a sixth of the forward
-// kernel's vector instructions).  Rows behind `last` repeat it (hidden later).  Row strides are below 2^25 elements (host check).
+// kernel's vector instructions).  Rows outside the cover repeat one inside it (hidden later): what a cache holds in slots that nobody
+// sees does not even arrive, so that infinities and NaN there cost nothing (NaN behind the last key, the same times as with zeros there,
+// and before, when they were read and rows computed again: 16 rows over 30000 keys of 32 / 8 heads of 128 340 us, 13.5 ms; 2 x 512 rows
+// over 470 keys of 64 heads of 64 22 us, 2.2 ms.  The tests of a tile's place cost 1 % of 15488 rows of 30 heads of 64).  Row strides
+// are below 2^25 elements (host check).
 template <int D, int ROWS, int NW>
 struct Stager {
     static constexpr int LPR = D / 8, RPP = 64 / LPR, N = ROWS / RPP / NW;     // lanes per row, rows per 1-KiB piece
@@ -156,18 +175,31 @@ struct Stager {
             off[j] = (unsigned)r * (unsigned)(2 * ld) + (unsigned)(((lane % LPR) ^ swz<D>(r)) * 16);
         }
     }
-    PF_DEVICE void issue(const bf16_t* head, long long ld, int row0, int last, char* lds, int wid, int lane) const {
+    PF_DEVICE void whole(const bf16_t* head, long long ld, int row0, char* lds, int wid) const {
         const char* base = (const char*)(head + row0 * ld);
-        if (row0 + ROWS - 1 <= last) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) glds16(base + off[j], lds + (wid * N + j) * 1024);
-        } else {
+        for (int j = 0; j < N; ++j) glds16(base + off[j], lds + (wid * N + j) * 1024);
+    }
+    PF_DEVICE void part(const bf16_t* head, long long ld, int row0, const Cover& rows, char* lds, int wid, int lane) const {
+        const char* base = (const char*)(head + row0 * ld);
+        const int spare = rows.some(row0, row0 + ROWS) - row0;
+        asm volatile("" : "+v"(lane));         // what follows from it is worked out here, not kept in registers through the caller's loop
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int r = (wid * N + j) * RPP + lane / LPR;
-                const unsigned o = (unsigned)min(r, last - row0) * (unsigned)(2 * ld) + (unsigned)(((lane % LPR) ^ swz<D>(r)) * 16);
-                glds16(base + o, lds + (wid * N + j) * 1024);
-            }
+        for (int j = 0; j < N; ++j) {
+            const int r = (wid * N + j) * RPP + lane / LPR, from = rows.has(row0 + r) ? r : spare;
+            const unsigned o = (unsigned)from * (unsigned)(2 * ld) + (unsigned)(((lane % LPR) ^ swz<D>(r)) * 16);
+            glds16(base + o, lds + (wid * N + j) * 1024);
+        }
+    }
+    // rows up to `last`, which those behind it repeat
+    PF_DEVICE void upto(const bf16_t* head, long long ld, int row0, int last, char* lds, int wid, int lane) const {
+        if (row0 + ROWS - 1 <= last) return whole(head, ld, row0, lds, wid);
+        const char* base = (const char*)(head + row0 * ld);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = (wid * N + j) * RPP + lane / LPR;
+            const unsigned o = (unsigned)min(r, last - row0) * (unsigned)(2 * ld) + (unsigned)(((lane % LPR) ^ swz<D>(r)) * 16);
+            glds16(base + o, lds + (wid * N + j) * 1024);
         }
     }
 };
@@ -185,9 +217,9 @@ PF_DEVICE Bounds wave_bounds(const Vis& v) {
     return {wave_min(v.na ? v.alo : BIG), wave_max(v.na ? v.alo + v.na : 0), wave_min(v.nb ? v.blo : BIG), wave_max(v.nb ? v.blo + v.nb : 0),
             wave_max(v.na ? v.alo : BIG), wave_min(v.na ? v.alo + v.na : 0), wave_max(v.nb ? v.blo : BIG), wave_min(v.nb ? v.blo + v.nb : 0)};
 }
-// the key tiles of a workgroup of 4 waves (`red`: 16 ints of LDS, read behind a barrier)
+// the key tiles of a workgroup of 4 waves (`red`: 16 ints of LDS, read behind a barrier; `cover`: 4 for all waves to leave the same in)
 template <int KB>
-PF_DEVICE TileList workgroup_tiles(const Bounds& w, int* red, int wid, int lane) {
+PF_DEVICE TileList workgroup_tiles(const Bounds& w, int* red, Cover* cover, int wid, int lane) {
     if (lane == 0) { red[4 * wid] = w.amin; red[4 * wid + 1] = w.amax; red[4 * wid + 2] = w.bmin; red[4 * wid + 3] = w.bmax; }
     __syncthreads();
     int x[4];
@@ -198,7 +230,9 @@ PF_DEVICE TileList workgroup_tiles(const Bounds& w, int* red, int wid, int lane)
         for (int u = 1; u < 4; ++u) x[i] = (i & 1) ? max(x[i], red[4 * u + i]) : min(x[i], red[4 * u + i]);
         x[i] = __builtin_amdgcn_readfirstlane(x[i]);
     }
-    return tile_list<KB>(x[0], x[1], x[2], x[3]);
+    const TileList t = tile_list<KB>(x[0], x[1], x[2], x[3]);
+    *cover = t.keys;
+    return t;
 }
 
 // A operand of a product over channels: row lane % 32 (+ 32 i), channels 16 ks + 8 (lane / 32) ..
@@ -554,7 +588,8 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     int* const red = (int*)(smem + 2 * BUF);
     int* const redo_flag = red + 16;
-    float* const meet = (float*)(smem + 2 * BUF + 80);           // KS = 2: [row wave][3][64] reference, sum, its exponent and `whole`
+    Cover* const cover = (Cover*)(red + 20);
+    float* const meet = (float*)(smem + 2 * BUF + 96);           // KS = 2: [row wave][3][64] reference, sum, its exponent and `whole`
     float* const tab_ = meet + (KS == 2 ? RW * 192 : 0);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
     constexpr int RESIDENT = FWD_WAVES<D, KS>;       // workgroups of a compute unit
@@ -568,7 +603,7 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     const int pmin = BIAS ? wave_min(pos) : 0, pmax = BIAS ? wave_max(pos) : 0;
     const Bounds wb = wave_bounds(vis);
     if (threadIdx.x == 0) *redo_flag = 0;
-    const TileList tl = workgroup_tiles<KB>(wb, red, wid, lane);
+    const TileList tl = workgroup_tiles<KB>(wb, red, cover, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
     const Stager<D, KB, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
@@ -576,13 +611,19 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     f32x16_t o[D / 32];
     float m, l;
     bool whole;                                    // wave-uniform: no row of the wave had a hidden key in any tile (a bias may hide some)
-    auto issue = [&](int n) {
+    auto issue = [&](int n, bool begin = false) {
         const int j0 = tl.at(n) * KB;
         char* buf = smem + (n & 1) * BUF;
-        sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
-        sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
+        if (begin ? tl.keys.whole(j0, j0 + KB) : tl.inner(n)) {
+            sk_.whole(K, p.k.ld, j0, buf, wid);
+            sv_.whole(V, p.v.ld, j0, buf + TILE, wid);
+        } else {
+            const Cover c = begin ? tl.keys : scalar(*cover);
+            sk_.part(K, p.k.ld, j0, c, buf, wid, lane);
+            sv_.part(V, p.v.ld, j0, c, buf + TILE, wid, lane);
+        }
     };
-    if (tl.n > 0) issue(0);                        // the first tile is on its way before the rows are read
+    if (tl.n > 0) issue(0, true);                  // the first tile is on its way before the rows are read
     const float* const tab = BIAS ? load_table(p, h, tab_) : nullptr;
     bf16x8_t qf[D / 16];
     {
@@ -775,6 +816,8 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
     const int amin = wave_min(vis.na ? vis.alo : 0x7fffffff), amax = wave_max(vis.na ? vis.alo + vis.na : 0);
     const int bmin = wave_min(vis.nb ? vis.blo : 0x7fffffff), bmax = wave_max(vis.nb ? vis.blo + vis.nb : 0);
     const TileList tl = tile_list<32>(amin, amax, bmin, bmax);
+    Cover* const cover = (Cover*)(smem + 4 * WAVE) + wid;
+    *cover = tl.keys;
     const int n0 = (int)((long long)tl.n * part / p.nsplit), n1 = (int)((long long)tl.n * (part + 1) / p.nsplit);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
@@ -792,12 +835,19 @@ __global__ __launch_bounds__(256, 1) void range_split_kernel(const RArgs p) {
     char* const mem = smem + wid * WAVE;
     drain();                                                        // the counted waits below see tile pieces only
     const Stager<D, 32, 1> sk_(p.k.ld, 0, lane), sv_(p.v.ld, 0, lane);
-    auto issue = [&](int n, int buf) {
+    auto issue = [&](int n, int buf, bool begin = false) {
         const int j0 = tl.at(n) * 32;
-        sk_.issue(K, p.k.ld, j0, p.Lk - 1, mem + buf * BUF, 0, lane);
-        sv_.issue(V, p.v.ld, j0, p.Lk - 1, mem + buf * BUF + TILE, 0, lane);
+        char* to = mem + buf * BUF;
+        if (begin ? tl.keys.whole(j0, j0 + 32) : tl.inner(n)) {
+            sk_.whole(K, p.k.ld, j0, to, 0);
+            sv_.whole(V, p.v.ld, j0, to + TILE, 0);
+        } else {
+            const Cover c = begin ? tl.keys : scalar(*cover);
+            sk_.part(K, p.k.ld, j0, c, to, 0, lane);
+            sv_.part(V, p.v.ld, j0, c, to + TILE, 0, lane);
+        }
     };
-    if (n0 + wid < n1) issue(n0 + wid, 0);
+    if (n0 + wid < n1) issue(n0 + wid, 0, true);
     int buf = 0;
     for (int n = n0 + wid; n < n1; n += 4, buf ^= 1) {
         if (n + 4 < n1) {
@@ -1092,7 +1142,8 @@ PF_DEVICE void row_gradients(const RArgs& p, int block) {
     constexpr bool CAP = MODE & 1, BIAS = MODE & 2;
     constexpr int KB = DQ_KB<D, MODE, KS>, TILE = KB * 2 * D, BUF = 2 * TILE, RW = 4 / KS, NI = KB / 32 / KS;
     int* const red = (int*)(smem + 2 * BUF);
-    float* const meet = (float*)(red + 16);                         // KS = 2: [row wave] whole
+    Cover* const cover = (Cover*)(red + 16);
+    float* const meet = (float*)(red + 20);                         // KS = 2: [row wave] whole
     float* const tab_ = meet + 4;
     const int NB = 2 * p.R + 1, TS = (table_floats(p.R) + 3) / 4 * 4;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wid % RW, kw = wid / RW;
@@ -1106,17 +1157,23 @@ PF_DEVICE void row_gradients(const RArgs& p, int block) {
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, rc) : 0;
     const Bounds wb = wave_bounds(vis);
-    const TileList tl = workgroup_tiles<KB>(wb, red, wid, lane);
+    const TileList tl = workgroup_tiles<KB>(wb, red, cover, wid, lane);
     const Stager<D, KB, 4> sk_(p.k.ld, wid, lane), sv_(p.v.ld, wid, lane);
     const bf16_t* const K = p.k.p + b * p.k.bs + hk * p.k.hs;
     const bf16_t* const V = p.v.p + b * p.v.bs + hk * p.v.hs;
-    auto issue = [&](int n) {
+    auto issue = [&](int n, bool begin = false) {
         const int j0 = tl.at(n) * KB;
         char* buf = smem + (n & 1) * BUF;
-        sk_.issue(K, p.k.ld, j0, p.Lk - 1, buf, wid, lane);
-        sv_.issue(V, p.v.ld, j0, p.Lk - 1, buf + TILE, wid, lane);
+        if (begin ? tl.keys.whole(j0, j0 + KB) : tl.inner(n)) {
+            sk_.whole(K, p.k.ld, j0, buf, wid);
+            sv_.whole(V, p.v.ld, j0, buf + TILE, wid);
+        } else {
+            const Cover c = begin ? tl.keys : scalar(*cover);
+            sk_.part(K, p.k.ld, j0, c, buf, wid, lane);
+            sv_.part(V, p.v.ld, j0, c, buf + TILE, wid, lane);
+        }
     };
-    if (tl.n > 0) issue(0);                        // the first tile is on its way before the rows are read
+    if (tl.n > 0) issue(0, true);                  // the first tile is on its way before the rows are read
     const float* const tab = BIAS ? load_table(p, h, tab_, 1.f) : nullptr;
     if (BIAS && p.dbias) {
         for (int i = lane; i < NB; i += 64) hist[i] = 0.f;
@@ -1302,7 +1359,7 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
         for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *(const bf16x8_t*)(k + ks * 16);
         if constexpr (VLDS) {
             const Stager<D, 32, 1> s(p.v.ld, 0, lane);
-            s.issue(p.v.p + b * p.v.bs + hk * p.v.hs, p.v.ld, min(w0, p.Lk - 1), p.Lk - 1, vtile, 0, lane);
+            s.upto(p.v.p + b * p.v.bs + hk * p.v.hs, p.v.ld, min(w0, p.Lk - 1), p.Lk - 1, vtile, 0, lane);
         } else {
             const bf16_t* v = p.v.p + b * p.v.bs + kr * p.v.ld + hk * p.v.hs + hi * 8;
 #pragma unroll
@@ -1368,8 +1425,8 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
     auto issue = [&](const Item& n, int buf) {
         const int h = hk * p.G + n.g, r0 = n.qt * 64 + n.half * RT;
         char* dst = smem + buf * BUF;
-        sq_.issue(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, r0, p.Lq - 1, dst, wid, lane);
-        so_.issue(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, r0, p.Lq - 1, dst + TILE, wid, lane);
+        sq_.upto(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, r0, p.Lq - 1, dst, wid, lane);
+        so_.upto(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, r0, p.Lq - 1, dst + TILE, wid, lane);
         if (wid == 0) glds16(p.stat + (((long long)b * p.H + h) * nq + n.qt) * 256 + lane * 4, dst + 2 * TILE);
         if (wid == 1) glds16(p.vis + ((long long)b * nq + n.qt) * 256 + lane * 4, dst + 2 * TILE + 1024);
     };
@@ -1639,7 +1696,7 @@ RArgs range_args(const pf_attn_ranges_desc* d) {
 
 template <int D, int MODE, int KS>
 int launch_fwd_rows(const RArgs& a, hipStream_t stream) {
-    const size_t lds = 4 * FWD_KB<D, KS> * 2 * D + 80 + (KS == 2 ? 2 * 192 * 4 : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
+    const size_t lds = 4 * FWD_KB<D, KS> * 2 * D + 96 + (KS == 2 ? 2 * 192 * 4 : 0) + (MODE & 2 ? table_floats(MAX_RADIUS) * 4 : 0);
     PF_SET_MAX_LDS_ONCE((range_fwd_kernel<D, MODE, KS>), (int)lds);
     range_fwd_kernel<D, MODE, KS><<<(unsigned)(a.nqt * a.H * a.B), 256, lds, stream>>>(a);
     CHECK_LAUNCH();
@@ -1649,7 +1706,7 @@ int launch_fwd_rows(const RArgs& a, hipStream_t stream) {
 template <int D, int MODE>
 int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
     if (!few) return small_fwd(a.D, a.Lq, a.H, a.B) ? launch_fwd_rows<D, MODE, 2>(a, stream) : launch_fwd_rows<D, MODE, 1>(a, stream);
-    const size_t lds = 4 * 4 * 32 * 2 * D;                           // the meeting area [4][32][D + 4] fp32 is smaller
+    const size_t lds = 4 * 4 * 32 * 2 * D + 64;                      // the meeting area [4][32][D + 4] fp32 is smaller
     PF_SET_MAX_LDS_ONCE((range_split_kernel<D, MODE>), (int)lds);
     range_split_kernel<D, MODE><<<(unsigned)(a.nrb * a.Hk * a.B * a.nsplit), 256, lds, stream>>>(a);
     CHECK_LAUNCH();
@@ -1662,7 +1719,7 @@ int launch_fwd(const RArgs& a, bool few, hipStream_t stream) {
 }
 
 template <int D, int MODE, int KS>
-int lds_dq(int R) { return 4 * DQ_KB<D, MODE, KS> * 2 * D + 80 + (MODE & 2 ? (table_floats(R) + 3 + 4 * (2 * R + 1) + 3 + 4 * SKEW) * 4 : 0); }
+int lds_dq(int R) { return 4 * DQ_KB<D, MODE, KS> * 2 * D + 96 + (MODE & 2 ? (table_floats(R) + 3 + 4 * (2 * R + 1) + 3 + 4 * SKEW) * 4 : 0); }
 template <int D, int MODE, bool BOTH>
 int lds_dkv(int R) {
     const int rt = D == 64 ? 64 : 32, rows = BOTH ? lds_dq<D, MODE, 2>(R) : 0;

@@ -41,3 +41,73 @@ def test_halves_with_far_references(keys, radius, cap, D):
     # scores of up to 250 ln 2 carry 2^-23 of themselves into the weights (product, scale, cap: half a step each)
     assert within(out, want, bound + 2.0 ** -23 * 175 * 3) <= 1
     assert within(lse, want_lse, torch.full((), 2.0 ** -23 * 175 * 3).double()) <= 1
+
+
+@pytest.mark.parametrize("cap,radius", [(0.0, None), (20.0, 6)])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [
+    (3, 1, 777, 8, 2, 64), (2, 1, 5000, 8, 2, 128), (2, 5, 300, 6, 3, 128),        # split keys
+    (1, 90, 300, 64, 16, 64), (2, 90, 300, 64, 64, 128),                            # 64 rows
+    (8, 150, 300, 64, 8, 64), (4, 150, 300, 64, 8, 128)])                           # 128 rows
+def test_slots_that_nobody_sees_cost_nothing(B, Lq, Lk, H, Hkv, D, cap, radius):
+    """a cache from torch.empty may hold anything in front of, between and behind the keys that are seen: the same bits as over zeros
+    (a result that is computed again from its visible keys alone rounds its weights elsewhere), forward and gradient of the rows"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import KeyRanges
+    g = torch.Generator().manual_seed(37)
+    q, do = (torch.randn(B, Lq, H, D, generator=g).bfloat16().cuda() for _ in range(2))
+    k, v = (torch.randn(B, Lk, Hkv, D, generator=g).bfloat16().cuda() for _ in range(2))
+    bias = None if radius is None else torch.randn(H, 2 * radius + 1, generator=g).cuda()
+    lo, mid, mid2, hi = 9, Lk // 3, Lk // 3 + 30, Lk - 43
+    for two in (False, True):
+        rows = torch.arange(Lq)[None].expand(B, Lq)
+        a_lo, end = torch.full((B, Lq), lo), (hi - Lq + 1 + rows).clamp(min=mid2)         # the last row sees up to `hi`
+        args = [a_lo, torch.full_like(a_lo, mid), torch.full_like(a_lo, mid2), end] if two else [a_lo, end]
+        ranges = KeyRanges(*[t.int().contiguous().cuda() for t in args])
+        how = dict(ranges=ranges, cap=cap, bias=bias)
+        unseen = torch.ones(Lk, dtype=torch.bool)
+        unseen[lo:hi] = False
+        if two:
+            unseen[mid:mid2] = True
+        got = []
+        for bad in (0.0, float("nan"), float("inf")):
+            kk, vv = k.clone(), v.clone()
+            kk[:, unseen.cuda()], vv[:, unseen.cuda()] = bad, bad
+            out, lse = torch.empty_like(q), torch.empty(B, H, Lq, device="cuda")
+            ops.attention_ranges(q, kk, vv, out, lse=lse, **how)
+            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+            ops.attention_ranges_backward(do, q, kk, vv, out, lse, dq, dk, dv, **how)
+            got.append((out, lse, dq))
+            assert not dk[:, unseen.cuda()].any() and not dv[:, unseen.cuda()].any()
+        assert torch.isfinite(got[0][0]).all() and torch.isfinite(got[0][2]).all()
+        for other in got[1:]:
+            for name, x, y in zip(("out", "lse", "dq"), got[0], other):
+                assert torch.equal(x, y), (two, name)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B", [1, 8])
+def test_slots_that_nobody_sees_in_the_second_pass(B, D):
+    """the same where the first pass overflowed and the workgroup ran again with the running maximum"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import KeyRanges
+    Lq, Lk, H = 70, 400, 64 * (2 if D == 128 else 1) * (1 if B == 1 else 2)
+    g = torch.Generator().manual_seed(38)
+    q, v = torch.zeros(B, Lq, H, D), torch.randn(B, Lk, 1, D, generator=g)
+    q[..., 0] = 1.0
+    k = torch.randn(B, Lk, 1, D, generator=g)
+    k[..., 0] = torch.linspace(0, 600, Lk)[None, :, None]
+    q, k, v = (t.bfloat16().cuda() for t in (q, k, v))
+    lo = torch.full((B, Lq), 13, dtype=torch.int32, device="cuda")
+    ranges = KeyRanges(lo, torch.full_like(lo, 350))
+    got = []
+    for bad in (0.0, float("nan")):
+        for t in (k, v):
+            t[:, :13], t[:, 350:] = bad, bad
+        out, lse = torch.empty_like(q), torch.empty(B, H, Lq, device="cuda")
+        ops.attention_ranges(q, k.expand(B, Lk, H, D) if B > 1 else k, v.expand(B, Lk, H, D) if B > 1 else v, out, ranges=ranges, scale=1.0, lse=lse)
+        got.append((out, lse))
+    clean = torch.where(torch.isnan(k), 0, k).cpu(), torch.where(torch.isnan(v), 0, v).cpu()
+    want, want_lse, bound = attention64(q.cpu(), *clean, mask=ranges.dense_mask(Lk).cpu(), scale=1.0)
+    # scores up to 600 carry 2^-23 of themselves into the weights, three roundings
+    assert within(got[0][0], want, bound + 3 * 2.0 ** -23 * 600 * 4) <= 1
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
