@@ -433,21 +433,58 @@ template <int D>
 PF_DEVICE void exact_dkv(const RArgs& p, int b, int hk, int j) {
     const int lane = threadIdx.x & 63;
     float ak[2] = {0.f, 0.f}, av[2] = {0.f, 0.f};
-    bool done = false;
-    for (int h = hk * p.G; h < (hk + 1) * p.G && !done; ++h)
-        for (int i0 = 0; i0 < p.Lq && !done; i0 += 64) {
+    bool nan_k = false, nan_v = false;
+    for (int h = hk * p.G; h < (hk + 1) * p.G && !(nan_k && nan_v); ++h)
+        for (int i0 = 0; i0 < p.Lq && !(nan_k && nan_v); i0 += 64) {
             const int i = i0 + lane;
             bool use = i < p.Lq && sees(load_vis(p, b, i), j);
             if (__builtin_amdgcn_ballot_w64(use) == 0) continue;
             float P = 0.f, dz = 0.f;
             if (use) use = exact_pair<D>(p, b, h, hk, i, j, P, dz);
             const unsigned long long m = __builtin_amdgcn_ballot_w64(use);
-            add_rows<D>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, i0, m, dz * p.dscale, ak);
-            add_rows<D>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, i0, m, P, av);
-            done = all_nan<D>(ak) && all_nan<D>(av);
+            if (!nan_k) add_rows<D>(p.q.p + b * p.q.bs + h * p.q.hs, p.q.ld, i0, m, dz * p.dscale, ak);
+            if (!nan_v) add_rows<D>(p.dO.p + b * p.dO.bs + h * p.dO.hs, p.dO.ld, i0, m, P, av);
+            nan_k = nan_k || all_nan<D>(ak);
+            nan_v = nan_v || all_nan<D>(av);
         }
     store_row<D>(p.dk.p + b * p.dk.bs + j * p.dk.ld + hk * p.dk.hs, ak);
     store_row<D>(p.dv.p + b * p.dv.bs + j * p.dv.ld + hk * p.dv.hs, av);
+}
+
+// One whole wave: whether the sums of keys w0 .. w0 + 31 may hold what does not belong there -- a row that shares a tile with them does
+// not see one of them, a bias hides some distance, or the last row, which a short tile repeats with weights of 0, is not finite.
+// Where none of this is so, a result that is not finite is right as it is: one infinite entry of dout costs nothing (16 heads of 64
+// over 4 key heads, 2048 rows, nothing hidden: 106 us with and 112 without it, 2320 when all keys were computed again).
+template <int D>
+PF_DEVICE bool strangers(const RArgs& p, int b, int hk, int w0) {
+    const int lane = threadIdx.x & 63, w1 = min(w0 + 32, p.Lk), rest = p.Lq & 63;
+    const int* const tiles = p.tiles + (long long)b * p.nq64 * 8;
+    bool bad = false;
+    if (p.bias)
+        for (long long i = (long long)hk * p.G * (2 * p.R + 1) + lane; i < (long long)(hk + 1) * p.G * (2 * p.R + 1); i += 64) bad = bad || p.bias[i] <= HIDDEN;
+    for (int n = lane; n < p.nq64 - (rest ? 1 : 0); n += 64) {
+        const int* x = tiles + n * 8LL;
+        const bool some = (x[0] < w1 && x[1] > w0) || (x[2] < w1 && x[3] > w0);
+        bad = bad || (some && !((x[4] <= w0 && x[5] >= w1) || (x[6] <= w0 && x[7] >= w1)));
+    }
+    if (rest) {                                    // row by row: the rows behind the last one see nothing
+        const int* x = tiles + (p.nq64 - 1) * 8LL;
+        const int* v = p.vis + ((long long)b * p.nq64 + p.nq64 - 1) * 256 + lane;
+        const int alo = v[0], ahi = alo + v[64], blo = v[128], bhi = blo + v[192];
+        const bool all = (alo <= w0 && ahi >= w1) || (blo <= w0 && bhi >= w1);
+        if ((x[0] < w1 && x[1] > w0) || (x[2] < w1 && x[3] > w0)) {
+            bad = bad || (lane < rest && !all);
+            const long long last = p.Lq - 1;
+            for (int h = hk * p.G; h < (hk + 1) * p.G; ++h)
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) {
+                    const int at = lane * (D / 64) + c;
+                    bad = bad || !(fabsf((float)p.q.p[b * p.q.bs + last * p.q.ld + h * p.q.hs + at]) < __builtin_inff()) ||
+                          !(fabsf((float)p.dO.p[b * p.dO.bs + last * p.dO.ld + h * p.dO.hs + at]) < __builtin_inff());
+                }
+        }
+    }
+    return __builtin_amdgcn_ballot_w64(bad) != 0;
 }
 
 // lane l holds column l % 32 of a [D][32] result, channels reg_row(r) + 4 (l / 32) + 32 c: 8-byte stores into its row
@@ -1057,7 +1094,7 @@ __global__ __launch_bounds__(256) void range_kvjoin_kernel(const RArgs p) {
         bad = bad || !(fabsf(k[c]) < __builtin_inff()) || !(fabsf(v[c]) < __builtin_inff());
         k[c] *= p.dscale;
     }
-    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+    if (__builtin_amdgcn_ballot_w64(bad) != 0 && strangers<D>(p, b, hk, j & ~31)) {
         exact_dkv<D>(p, b, hk, j);
         return;
     }
@@ -1549,14 +1586,7 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
     }
     const bool bad = key < p.Lk && (any_nonfinite<D / 32>(dk) || any_nonfinite<D / 32>(dv));
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
-    if (!BIAS && redo != 0) {                      // only tiles with hidden pairs can have brought in what does not belong there
-        unsigned long long partial = 0;
-        for (int n = 0; n < nq; n += 64) {
-            test(n);
-            partial |= some & ~all;
-        }
-        if (partial == 0) redo = 0;
-    }
+    if (redo != 0 && !strangers<D>(p, b, hk, w0)) redo = 0;
     redo = (redo | (redo >> 32)) & 0xffffffffull;
     if (key < p.Lk && !((redo >> (lane & 31)) & 1)) {
         store_cols<D>(p.dk.p + b * p.dk.bs + key * p.dk.ld + hk * p.dk.hs, dk, p.dscale);

@@ -111,3 +111,38 @@ def test_slots_that_nobody_sees_in_the_second_pass(B, D):
     # scores up to 600 carry 2^-23 of themselves into the weights, three roundings
     assert within(got[0][0], want, bound + 3 * 2.0 ** -23 * 600 * 4) <= 1
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.parametrize("radius", [None, 5])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [
+    (1, 320, 140, 8, 2, 64), (1, 300, 140, 8, 2, 128), (2, 301, 77, 4, 4, 64),     # the rows in parts
+    (2, 64, 300, 16, 16, 64), (2, 70, 300, 16, 16, 64), (1, 90, 300, 24, 24, 128)])   # all rows in one workgroup
+def test_one_infinite_gradient_entry(B, Lq, Lk, H, Hkv, D, radius):
+    """nothing is hidden and one entry of dout is infinite: the gradients of its channel say so, those of v's other channels keep their
+    bits (keys that are computed again, one by one, would round their weights elsewhere), also where the last row tile is short"""
+    from pyflow_hip import ops
+    g = torch.Generator().manual_seed(41)
+    q, do = (torch.randn(B, Lq, H, D, generator=g).bfloat16().cuda() for _ in range(2))
+    k, v = (torch.randn(B, Lk, Hkv, D, generator=g).bfloat16().cuda() for _ in range(2))
+    bias = None if radius is None else torch.randn(H, 2 * radius + 1, generator=g).cuda()
+    out, lse = torch.empty_like(q), torch.empty(B, H, Lq, device="cuda")
+    ops.attention_ranges(q, k, v, out, lse=lse, bias=bias)
+
+    def gradients(do):
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        ops.attention_ranges_backward(do, q, k, v, out, lse, dq, dk, dv, bias=bias)
+        return dq, dk, dv
+    clean = gradients(do)
+    for row in (3, Lq - 1):
+        bad = do.clone()
+        bad[0, row, 0, 7] = math.inf
+        dq, dk, dv = gradients(bad)
+        assert (dv[0, :, 0, 7] == math.inf).all() and not torch.isfinite(dk[0, :, 0]).any() and not torch.isfinite(dq[0, row, 0]).any()
+        others = torch.ones_like(dv, dtype=torch.bool)
+        others[0, :, 0, 7] = False
+        if row == 3 or Lq % 64 == 0:              # a short tile repeats the last row, whose infinity then has to be kept away
+            assert torch.equal(dv[others], clean[2][others])
+        assert torch.equal(dv[:, :, 1:], clean[2][:, :, 1:]) and torch.equal(dk[:, :, 1:], clean[1][:, :, 1:])
+        others = torch.ones_like(dq, dtype=torch.bool)
+        others[0, row, 0] = False
+        assert torch.equal(dq[others], clean[0][others])
