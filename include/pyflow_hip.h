@@ -355,6 +355,10 @@ int pf_attention_small_bf16(const pf_attn_small_desc* d, pf_stream_t stream);
  * and softmax statistics fp32.  A view names element (batch b, row r, head h, channel c) = p[b batch + r row + h head + c];
  * strides in elements, >= 0, multiples of 8; p 16-byte aligned. */
 typedef struct { void* p; long long batch, row, head; } pf_rows_view;
+/* whether two views of B x L x H rows of D elements share an element (columns of one buffer that lie side by side do not).  The
+ * operators below refuse outputs that share one with an input or another output, but for those they name, and outputs that are
+ * folded onto themselves. */
+int pf_rows_views_share(const pf_rows_view* a, int Ba, int La, int Ha, const pf_rows_view* b, int Bb, int Lb, int Hb, int D);
 
 /* pf_qk_norm_rope_axes: RMSNorm (gains wq / wk fp32 [D]; NULL = none) of every head of Q [B][L][H][D] and K [B][L][Hkv][D], then the
  *   rotation of the first 2 n_pairs channels: pair p turns by pos[b][row][axis[p]] * freq[p] radians (pos fp32 with strides
@@ -362,7 +366,7 @@ typedef struct { void* p; long long batch, row, head; } pf_rows_view;
  *   with `halves` (n_pairs % 8 == 0 then).  Q is multiplied by q_scale before its one rounding.  D = 64 or 128; H or Hkv may be
  *   0.  Qo / Ko may be Q / K (in place), and must not overlap them otherwise.
  * pf_qk_norm_rope_axes_bwd: dQ, dK = gradients of the results, Q, K = the inputs of the forward; writes the gradients of the
- *   inputs to Qo, Ko (may be dQ, dK) and, where not NULL, of the gains to dwq / dwk fp32 [D] (workspace of
+ *   inputs to Qo, Ko (may be dQ, dK, or Q, K) and, where not NULL, of the gains to dwq / dwk fp32 [D] (workspace of
  *   pf_qk_norm_rope_axes_bwd_workspace_bytes, 16-byte aligned; the same bits every time). */
 typedef struct {
     pf_rows_view Q, K, Qo, Ko, dQ, dK;

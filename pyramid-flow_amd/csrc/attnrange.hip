@@ -20,6 +20,7 @@
 #include <type_traits>
 #include "common.h"
 #include "pyflow_hip.h"
+#include "rows_view.h"
 
 int pf_set_err(const char* m);
 
@@ -1642,6 +1643,31 @@ const char* check_ranges(const pf_attn_ranges_desc* d, bool grad) {
     return nullptr;
 }
 
+// outputs share no element with an input or each other; O may be Q, element for element
+const char* check_overlap(const pf_attn_ranges_desc* d, bool grad) {
+    struct One { const pf_rows_view* v; int L, H; };
+    const One q = {&d->Q, d->Lq, d->H}, k = {&d->K, d->Lk, d->Hkv}, v = {&d->V, d->Lk, d->Hkv}, o = {&d->O, d->Lq, d->H};
+    const One dO = {&d->dO, d->Lq, d->H}, dq = {&d->dQ, d->Lq, d->H}, dk = {&d->dK, d->Lk, d->Hkv}, dv = {&d->dV, d->Lk, d->Hkv};
+    const int B = d->B, D = d->D;
+    auto share = [&](const One& x, const One& y) { return rows_share(*x.v, B, x.L, x.H, *y.v, B, y.L, y.H, D); };
+    auto folded = [&](const One& x) { return rows_folded(*x.v, B, x.L, x.H, D); };
+    if (!grad) {
+        if (folded(o)) return "pf_attention_ranges_bf16: the output overlaps itself";
+        if (share(o, k) || share(o, v)) return "pf_attention_ranges_bf16: the output overlaps the keys or values";
+        if (!rows_same(d->O, d->Q, B, d->Lq, d->H) && share(o, q)) return "pf_attention_ranges_bf16: the output overlaps the queries and is not them";
+        return nullptr;
+    }
+    const One out[3] = {dq, dk, dv}, in[5] = {q, k, v, o, dO};
+    for (int x = 0; x < 3; ++x) {
+        if (folded(out[x])) return "pf_attention_ranges_bwd: a gradient overlaps itself";
+        for (const One& y : in)
+            if (share(out[x], y)) return "pf_attention_ranges_bwd: a gradient overlaps an input";
+        for (int y = 0; y < x; ++y)
+            if (share(out[x], out[y])) return "pf_attention_ranges_bwd: two gradients overlap";
+    }
+    return nullptr;
+}
+
 // the form with 32 (row, head) pairs per workgroup and the keys split: where even 64-row workgroups would be few (1 x 700 rows over 1400
 // keys of 32 heads of 128, 192 in the count below: 87 us, rows 43; 64 rows over 8000 keys of 16 heads of 64, 16: 25 us, rows 82), and
 // where one block of 32 pairs holds all rows that share a key head (each key is then read once, not once per query head)
@@ -1823,6 +1849,7 @@ extern "C" int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, hipStream_
     const bool few = few_rows(d);
     const long long grid = few ? (long long)row_blocks(d) * d->Hkv * d->B * splits(d) : (long long)row_groups(d->Lq, true) * d->H * d->B;
     if (grid > 0x7fffffffLL) return pf_set_err("pf_attention_ranges_bf16: too many workgroups");
+    if (const char* e = check_overlap(d, false)) return pf_set_err(e);
     a.nqt = row_groups(d->Lq, small_fwd(d->D, d->Lq, d->H, d->B));
     a.nrb = row_blocks(d);
     a.nsplit = few ? splits(d) : 1;
@@ -1854,6 +1881,7 @@ extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t
         (long long)(d->Lq + 63) / 64 * (d->H / (d->Hkv ? d->Hkv : 1)) > 0x7fffffffLL)
         return pf_set_err("pf_attention_ranges_bwd: too many workgroups");
     if (!d->H) return 0;
+    if (const char* e = check_overlap(d, true)) return pf_set_err(e);
     RArgs a = range_args(d);
     char* w = (char*)d->workspace;
     a.stat = (float*)w;

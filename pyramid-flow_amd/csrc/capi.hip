@@ -1,6 +1,7 @@
 // Error channel + version of the C ABI (include/pyflow_hip.h).
 #include <stdio.h>
 #include "pyflow_hip.h"
+#include "rows_view.h"
 
 static thread_local char g_err[512];
 
@@ -23,4 +24,7 @@ extern "C" int pf_struct_size(int which) {
         case 5: return (int)sizeof(pf_attn_ranges_desc);
         default: return -1;
     }
+}
+extern "C" int pf_rows_views_share(const pf_rows_view* a, int Ba, int La, int Ha, const pf_rows_view* b, int Bb, int Lb, int Hb, int D) {
+    return a && b && rows_share(*a, Ba, La, Ha, *b, Bb, Lb, Hb, D) ? 1 : 0;
 }

@@ -13,6 +13,7 @@
 // head row = D / 8 lanes of 16 bytes; a wave owns one token (or a slice of its heads when there are few tokens).
 #include "common.h"
 #include "pyflow_hip.h"
+#include "rows_view.h"
 
 int pf_set_err(const char* m);
 
@@ -306,6 +307,21 @@ const char* check_heads(const pf_heads_desc* d, bool grad) {
     return nullptr;
 }
 
+// an output may be the input (gradient: or the gradient) of its own heads, element for element, and shares nothing else
+const char* check_overlap(const pf_heads_desc* d, bool grad) {
+    const int B = d->B, L = d->L, H[2] = {d->H, d->Hkv}, D = d->D;
+    const pf_rows_view* const out[2] = {&d->Qo, &d->Ko};
+    const pf_rows_view* const in[2][2] = {{&d->Q, &d->dQ}, {&d->K, &d->dK}};
+    for (int o = 0; o < 2; ++o) {
+        if (rows_folded(*out[o], B, L, H[o], D)) return "pf_qk_norm_rope_axes: an output overlaps itself";
+        for (int i = 0; i < 2; ++i)
+            for (int n = 0; n < (grad ? 2 : 1); ++n)
+                if (!(i == o && rows_same(*out[o], *in[i][n], B, L, H[i])) && rows_share(*out[o], B, L, H[o], *in[i][n], B, L, H[i], D))
+                    return "pf_qk_norm_rope_axes: an output overlaps an input and is not it";
+    }
+    return rows_share(d->Qo, B, L, H[0], d->Ko, B, L, H[1], D) ? "pf_qk_norm_rope_axes: the outputs overlap" : nullptr;
+}
+
 HArgs heads_args(const pf_heads_desc* d) {
     HArgs a{};
     a.q = view(d->Q); a.k = view(d->K); a.qo = view(d->Qo); a.ko = view(d->Ko); a.dq = view(d->dQ); a.dk = view(d->dK);
@@ -329,6 +345,7 @@ HArgs heads_args(const pf_heads_desc* d) {
 extern "C" int pf_qk_norm_rope_axes(const pf_heads_desc* d, hipStream_t stream) {
     if (const char* e = check_heads(d, false)) return pf_set_err(e);
     if (d->B == 0 || d->L == 0 || d->H + d->Hkv == 0) return 0;
+    if (const char* e = check_overlap(d, false)) return pf_set_err(e);
     const HArgs a = heads_args(d);
     const unsigned grid = (unsigned)(((long long)d->B * d->L * a.chunks + 3) / 4);
     if (d->D == 64) heads_fwd_kernel<64><<<grid, 256, 0, stream>>>(a);
@@ -352,6 +369,7 @@ extern "C" int pf_qk_norm_rope_axes_bwd(const pf_heads_desc* d, float* dwq, floa
     const bool gains = dwq || dwk, empty = d->B == 0 || d->L == 0 || d->H + d->Hkv == 0;
     if (gains && !empty && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < pf_qk_norm_rope_axes_bwd_workspace_bytes(d)))
         return pf_set_err("pf_qk_norm_rope_axes_bwd: workspace missing, unaligned or too small");
+    if (const char* e = check_overlap(d, true)) return pf_set_err(e);
     HArgs a = heads_args(d);
     int grid = 0;
     if (!empty) {

@@ -146,3 +146,45 @@ def test_one_infinite_gradient_entry(B, Lq, Lk, H, Hkv, D, radius):
         others = torch.ones_like(dq, dtype=torch.bool)
         others[0, row, 0] = False
         assert torch.equal(dq[others], clean[0][others])
+
+
+def test_outputs_beside_their_inputs_and_over_them():
+    """columns of one buffer, head-major halves and the queries themselves take results; anything that overlaps otherwise is refused"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import RopeAxes
+    B, L, H, D = 2, 90, 4, 64
+    g = torch.Generator().manual_seed(43)
+    apart = [torch.randn(B, L, H, D, generator=g).bfloat16().cuda() for _ in range(3)]
+    want = torch.empty_like(apart[0])
+    ops.attention_ranges(*apart, want)
+    wide = torch.empty(B, L, 4 * H + 1, D, dtype=torch.bfloat16, device="cuda")
+    major = torch.empty(B, 4, H, L, D, dtype=torch.bfloat16, device="cuda")
+    mixed = torch.empty(B, L, H, 4, D, dtype=torch.bfloat16, device="cuda")
+    for places in ([wide[:, :, n * H:(n + 1) * H] for n in range(4)], [major[:, n].transpose(1, 2) for n in range(4)], [mixed[:, :, :, n] for n in range(4)]):
+        for x, t in zip(places, apart):
+            x.copy_(t)
+        ops.attention_ranges(*places)
+        assert torch.equal(places[3], want) and all(torch.equal(x, t) for x, t in zip(places, apart))
+        ops.attention_ranges(*places[:3], places[0])
+        assert torch.equal(places[0], want)
+    shifted = wide[:, :, 1:H + 1]
+    for out in (shifted, wide[:, :, H:2 * H], wide[:, :, 2 * H + 1:3 * H + 1]):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ops.attention_ranges(wide[:, :, :H], wide[:, :, H:2 * H], wide[:, :, 2 * H:3 * H], out)
+    lse = torch.zeros(B, H, L, device="cuda")
+    ops.attention_ranges(*apart, want, lse=lse)
+    grads = [torch.empty_like(t) for t in apart]
+    for n in range(3):
+        for taken in (apart[0], apart[2], want, grads[(n + 1) % 3]):
+            outs = list(grads)
+            outs[n] = taken
+            with pytest.raises(RuntimeError, match="overlap"):
+                ops.attention_ranges_backward(apart[1], *apart, want, lse, *outs)
+    rope = RopeAxes.build([D], "cuda")
+    pos = torch.zeros(1, L, 1, device="cuda")
+    q, k = wide[:, :, :H], wide[:, :, H:2 * H]
+    ops.qk_norm_rope_axes(q, k, q, k, None, None, rope, pos)
+    ops.qk_norm_rope_axes(q, k, wide[:, :, 2 * H:3 * H], wide[:, :, 3 * H:4 * H], None, None, rope, pos)
+    for qo, ko in ((k, q), (shifted, k), (q, wide[:, :, H + 1:2 * H + 1])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.qk_norm_rope_axes(q, k, qo, ko, None, None, rope, pos)
