@@ -392,6 +392,8 @@ int pf_qk_norm_rope_axes_bwd(const pf_heads_desc* d, float* dwq, float* dwk, voi
  *   split the keys); not shared by launches that may overlap.  Rows of a tensor lie less than 2^25 elements apart.
  * pf_attention_ranges_which: 1 = 128 or 64 rows of one head per workgroup, 2 = 32 (row, head) pairs of one key head per workgroup with the
  *   keys split over waves and workgroups, -1 = invalid descriptor.
+ * pf_attention_ranges_rows: rows of one head per workgroup: 128 or 64 (+ 1 where the row tiles start in falling order of their keys), 32
+ *   for the split-key form; of the gradient's dQ: 128 or 64.  -1 = invalid descriptor.
  * pf_attention_ranges_bwd: given dO, O, LSE of the forward, writes dQ, dK, dV and (dbias != NULL) the bias's gradient fp32
  *   [H][2 R + 1]; the same bits every time.  Gradients of shared key heads are summed over their H / Hkv query heads.  Rows that
  *   see nothing get zeros, keys nobody sees too.  dQ, dK, dV must not overlap the inputs. */
@@ -408,6 +410,7 @@ typedef struct {
 long long pf_attention_ranges_workspace_bytes(const pf_attn_ranges_desc* d);     /* -1 = invalid descriptor */
 long long pf_attention_ranges_bwd_workspace_bytes(const pf_attn_ranges_desc* d); /* -1 = invalid descriptor */
 int pf_attention_ranges_which(const pf_attn_ranges_desc* d);
+int pf_attention_ranges_rows(const pf_attn_ranges_desc* d, int gradient);
 int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, pf_stream_t stream);
 int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, pf_stream_t stream);
 

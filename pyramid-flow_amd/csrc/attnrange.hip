@@ -581,6 +581,10 @@ PF_DEVICE Place heavy_first(int block, int n, int nwg, int resident = 0) {
     return {w, k - w * m + (heavy ? 0 : nh)};
 }
 
+// whether the row tiles of a forward launch of nwg workgroups, `resident` to a compute unit, start in falling order of their keys
+constexpr int SORTED_TILES = 256;
+__host__ __device__ constexpr bool sorted_launch(int nwg, int resident) { return nwg > 256 * resident && nwg <= 768 * resident; }
+
 // The row tile (of ROWS rows) that comes at place `rank` when a head's tiles start in falling order of their keys: `sort` and at most
 // 256 tiles.  One thread per tile takes the larger count of its first and last row and counts the tiles before it, the same in every
 // workgroup of the batch entry.  Otherwise the tiles come from the sequence's end on.  `mem`: 1028 bytes of LDS, free again behind
@@ -589,7 +593,7 @@ PF_DEVICE Place heavy_first(int block, int n, int nwg, int resident = 0) {
 // instead of 79 us).
 template <int ROWS>
 PF_DEVICE int ranked_tile(const RArgs& p, int b, int rank, bool sort, int* mem) {
-    if (!sort || !p.a_lo || p.nqt > 256) return p.nqt - 1 - rank;
+    if (!sort || !p.a_lo || p.nqt > SORTED_TILES) return p.nqt - 1 - rank;
     const int t = threadIdx.x;
     int mine = -1;
     if (t < p.nqt) {
@@ -634,7 +638,7 @@ __global__ __launch_bounds__(256, (FWD_WAVES<D, KS>)) void range_fwd_kernel(cons
     const int nwg = p.nqt * p.H * p.B;
     const Place at = heavy_first(blockIdx.x, p.nqt, nwg, RESIDENT);
     const int bh = at.head, b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
-    const int qt = ranked_tile<32 * RW>(p, b, at.rank, nwg > 256 * RESIDENT && nwg <= 768 * RESIDENT, (int*)smem);
+    const int qt = ranked_tile<32 * RW>(p, b, at.rank, sorted_launch(nwg, RESIDENT), (int*)smem);
     const int hi = lane >> 5, row0 = (qt * RW + rw) * 32, row = row0 + (lane & 31);
     const Vis vis = load_vis(p, b, row);
     const int pos = BIAS ? row_pos(p, b, min(row, p.Lq - 1)) : 0;
@@ -1837,6 +1841,16 @@ extern "C" long long pf_attention_ranges_bwd_workspace_bytes(const pf_attn_range
 
 extern "C" int pf_attention_ranges_which(const pf_attn_ranges_desc* d) {
     return check_ranges(d, false) ? -1 : (d->H == 0 || few_rows(d) ? 2 : 1);
+}
+
+extern "C" int pf_attention_ranges_rows(const pf_attn_ranges_desc* d, int gradient) {
+    if (check_ranges(d, gradient != 0)) return -1;
+    if (gradient) return small_dq(d->D, d->Lq, d->H, d->B) ? 64 : 128;
+    if (d->H == 0 || few_rows(d)) return 32;
+    const bool small = small_fwd(d->D, d->Lq, d->H, d->B);
+    const int nqt = row_groups(d->Lq, small), resident = d->D == 64 ? (small ? FWD_WAVES<64, 2> : FWD_WAVES<64, 1>) : (small ? FWD_WAVES<128, 2> : FWD_WAVES<128, 1>);
+    const long long nwg = (long long)nqt * d->H * d->B;
+    return (small ? 64 : 128) + (d->a_lo && nqt <= SORTED_TILES && nwg <= 0x7fffffffLL && sorted_launch((int)nwg, resident) ? 1 : 0);
 }
 
 extern "C" int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, hipStream_t stream) {

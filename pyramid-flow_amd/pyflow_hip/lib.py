@@ -109,7 +109,7 @@ EXPORTS = [
     "pf_embed_rows", "pf_rmsnorm", "pf_glu_mul", "pf_attention_small_bf16", "pf_rgb_to_yuv420",
     "pf_qk_norm_rope_axes", "pf_qk_norm_rope_axes_bwd", "pf_qk_norm_rope_axes_bwd_workspace_bytes",
     "pf_attention_ranges_bf16", "pf_attention_ranges_bwd", "pf_attention_ranges_workspace_bytes",
-    "pf_attention_ranges_bwd_workspace_bytes", "pf_attention_ranges_which", "pf_rows_views_share",
+    "pf_attention_ranges_bwd_workspace_bytes", "pf_attention_ranges_which", "pf_attention_ranges_rows", "pf_rows_views_share",
     "pf_comm_unique_id", "pf_comm_init", "pf_comm_destroy", "pf_comm_rank", "pf_comm_world", "pf_all_to_all_v",
     "pf_halo_send_recv", "pf_all_gather_v", "pf_all_reduce_sum_f32", "pf_broadcast_bytes", "pf_comm_wait",
     "pf_cmdlist_create", "pf_cmdlist_destroy", "pf_cmdlist_clear", "pf_cmdlist_size", "pf_cmdlist_is_graph", "pf_cmdlist_gemm",

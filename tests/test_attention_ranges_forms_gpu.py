@@ -8,7 +8,8 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.join(os.path.dirname(__file__), "helpers"))
-from ranges_ref import attention64, within  # noqa: E402
+from ranges_ref import attention64, attention_grad64, within  # noqa: E402
+from test_attention_ranges_gpu import _case, _check_backward, _check_forward, _forward  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -188,3 +189,131 @@ def test_outputs_beside_their_inputs_and_over_them():
     for qo, ko in ((k, q), (shifted, k), (q, wide[:, :, H + 1:2 * H + 1])):
         with pytest.raises(RuntimeError, match="overlap"):
             ops.qk_norm_rope_axes(q, k, qo, ko, None, None, rope, pos)
+
+
+def _rows(B, Lq, Lk, H, Hkv, D, ranges=True, gradient=False):
+    """rows of one head per workgroup (+ 1: sorted), as the library chooses them"""
+    import ctypes as C
+    from pyflow_hip import lib as L
+    from pyflow_hip.lib import AttnRangesDesc, RowsView
+    d = AttnRangesDesc()
+    d.B, d.H, d.Hkv, d.Lq, d.Lk, d.D, d.scale = B, H, Hkv, Lq, Lk, D, 1.0
+    d.Q = d.O = d.K = d.V = d.dO = d.dQ = d.dK = d.dV = RowsView(64, 64, 64, 64)
+    d.LSE = 64
+    if ranges:
+        d.a_lo = d.a_hi = 64
+    return L.load().pf_attention_ranges_rows(C.byref(d), int(gradient))
+
+
+MODES = [(None, 0.0), (None, 20.0), (6, 0.0), (6, 20.0), (None, 300.0), (6, 300.0)]         # bias radius, cap (300: tanh itself)
+
+
+@pytest.mark.parametrize("radius,cap", MODES)
+@pytest.mark.parametrize("form,B,Lq,Lk,H,Hkv,D", [
+    (32, 2, 40, 300, 6, 2, 64), (32, 2, 40, 300, 6, 2, 128), (64, 2, 140, 90, 64, 16, 64), (64, 1, 140, 90, 64, 16, 128),
+    (128, 8, 127, 90, 128, 16, 64), (128, 4, 129, 90, 64, 16, 128)])
+def test_every_forward_form(form, B, Lq, Lk, H, Hkv, D, radius, cap):
+    assert _rows(B, Lq, Lk, H, Hkv, D) == form
+    host, dev, how, ref, _ = _case(B, Lq, Lk, H, Hkv, D, "random", radius, cap, seed=51, pos=radius is not None)
+    _check_forward(host, dev, how, ref)
+
+
+@pytest.mark.parametrize("form,B,Lq,Lk,H,Hkv,D", [
+    (129, 9, 130, 130, 64, 64, 64), (65, 5, 257, 257, 64, 16, 64), (129, 7, 257, 257, 64, 8, 128), (65, 2, 193, 193, 96, 12, 128)])
+@pytest.mark.parametrize("kind", ["documents", "documents causal", "random"])
+def test_sorted_tiles(form, B, Lq, Lk, H, Hkv, D, kind):
+    """row tiles that start in falling order of their keys: ties, rows that see nothing, a last tile of one row; every row is written
+    (the outputs start as NaN)"""
+    assert _rows(B, Lq, Lk, H, Hkv, D) == form
+    host, dev, how, ref, _ = _case(B, Lq, Lk, H, Hkv, D, kind, None, 0.0, seed=52)
+    out, lse = _check_forward(host, dev, how, ref)
+    again = _forward(dev, how)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("Lq,Lk", [(385, 385), (640, 100)])
+def test_sorted_tiles_are_each_taken_once(Lq, Lk):
+    """rows that all see the same keys (every count the same) and rows of which only a few see any: values tell the rows apart"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import KeyRanges
+    B, H, D = 6, 64, 64
+    assert _rows(B, Lq, Lk, H, H, D) % 2 == 1
+    g = torch.Generator().manual_seed(53)
+    q, k, v = (torch.randn(B, n, H, D, generator=g).bfloat16().cuda() for n in (Lq, Lk, Lk))
+    whole = torch.empty_like(q)
+    ops.attention_ranges(q, k, v, whole)
+    hi = torch.full((B, Lq), Lk, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    ops.attention_ranges(q, k, v, out, ranges=KeyRanges(torch.zeros_like(hi), hi))
+    assert torch.equal(out, whole)
+    hi[:, torch.randperm(Lq, generator=g).cuda()[:Lq * 7 // 8]] = 0
+    out.fill_(float("nan"))
+    ops.attention_ranges(q, k, v, out, ranges=KeyRanges(torch.zeros_like(hi), hi))
+    assert torch.equal(out, torch.where(hi[..., None, None] > 0, whole, 0))
+
+
+@pytest.mark.parametrize("radius,cap,with_dbias", [(r, c, True) for r, c in MODES] + [(r, c, False) for r, c in MODES if r is not None])
+@pytest.mark.parametrize("form,B,Lq,Lk,H,Hkv,D", [
+    (64, 2, 75, 140, 6, 2, 64), (64, 2, 75, 140, 6, 2, 128), (128, 8, 127, 90, 128, 16, 64), (128, 8, 129, 70, 128, 32, 128)])
+def test_every_gradient_form(form, B, Lq, Lk, H, Hkv, D, radius, cap, with_dbias):
+    from pyflow_hip import ops
+    assert _rows(B, Lq, Lk, H, Hkv, D, gradient=True) == form
+    host, dev, how, ref, g = _case(B, Lq, Lk, H, Hkv, D, "random", radius, cap, seed=54, pos=radius is not None)
+    if with_dbias:
+        _check_backward(host, dev, how, ref, g)
+        return
+    out, lse = _forward(dev, how)
+    do = torch.randn(host[0].shape, generator=g).bfloat16()
+    got = [torch.full_like(t, float("nan")) for t in dev]
+    ops.attention_ranges_backward(do.cuda(), *dev, out, lse, *got, **how)
+    want = attention_grad64(do, *host, out.cpu(), lse.cpu(), **ref)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        assert within(x, *want[name]) <= 1, name
+
+
+@pytest.mark.parametrize("radius,cap", [(None, 0.0), (None, 20.0), (6, 0.0)])
+def test_gradient_of_many_rows_in_parts(radius, cap):
+    """128 rows per workgroup at head_dim 128, and the key gradients' rows in parts"""
+    B, Lq, Lk, H, Hkv, D = 1, 2000, 70, 128, 2, 128
+    assert _rows(B, Lq, Lk, H, Hkv, D, gradient=True) == 128
+    host, dev, how, ref, g = _case(B, Lq, Lk, H, Hkv, D, "random", radius, cap, seed=55)
+    _check_backward(host, dev, how, ref, g)
+
+
+@pytest.mark.parametrize("radius", [None, 6])
+def test_hidden_values_in_the_large_gradient(radius):
+    """infinities and NaN in keys nobody sees, and in rows that see nothing, at 128 rows per workgroup and head_dim 128"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import KeyRanges
+    B, Lq, Lk, H, Hkv, D = 8, 129, 100, 128, 32, 128
+    assert _rows(B, Lq, Lk, H, Hkv, D, gradient=True) == 128
+    host, dev, how, ref, g = _case(B, Lq, Lk, H, Hkv, D, None, radius, 0.0, seed=56)
+    lo = torch.randint(10, Lk - 60, (B, Lq), generator=g)
+    hi = lo + torch.randint(0, 50, (B, Lq), generator=g)
+    hi[:, ::5] = lo[:, ::5]
+    empty = hi == lo
+    how["ranges"] = KeyRanges(lo.int().cuda(), hi.int().cuda())
+    ref["mask"] = how["ranges"].dense_mask(Lk).cpu()
+    unseen = ~ref["mask"].any(1)                   # [B, Lk]
+    assert unseen.any(1).all() and empty.any()
+    do = torch.randn(host[0].shape, generator=g).bfloat16()
+    clean_do = torch.where(empty[..., None, None], 0, do)
+    for t in dev[1:]:
+        t[unseen.cuda()] = float("nan")
+    dev[0][empty.cuda()], bad_do = float("inf"), do.cuda()
+    bad_do[empty.cuda()] = float("nan")
+    out, lse = _forward(dev, how)
+    dq, dk, dv = (torch.full_like(t, 7) for t in dev)
+    ops.attention_ranges_backward(bad_do, *dev, out, lse, dq, dk, dv, **how)
+    host = [torch.where(empty[..., None, None], 0, host[0]), *(torch.where(unseen[..., None, None], 0, t) for t in host[1:])]
+    want = attention_grad64(clean_do, *host, out.cpu(), lse.cpu(), **ref)
+    for name, x in (("dq", dq), ("dk", dk), ("dv", dv)):
+        assert within(x, *want[name]) <= 1, name
+
+
+def test_forms_of_the_general_cases():
+    """which forms the cases of the general tests reach, so that a moved threshold shows"""
+    from test_attention_ranges_gpu import CASES, MANY
+    assert {_rows(*c[:6], ranges=c[6] is not None) for c in CASES} == {32}
+    assert [_rows(*c[:6], ranges=c[6] is not None) for c in MANY] == [64, 64, 32, 64, 64, 64, 128, 128, 128, 64, 64]
+    assert [_rows(*c[:6], gradient=True) for c in MANY] == [64] * 6 + [128, 128, 64, 64, 64]
