@@ -100,14 +100,14 @@ CASES = [  # B, Lq, Lk, H, Hkv, D, kind, radius, cap
     (2, 90, 90, 4, 2, 64, "causal", 20, 64.5),
     (1, 3, 700, 4, 2, 128, "random", None, 5000.0),
 ]
-MANY = [  # enough workgroups of 128 rows for the first form
+MANY = [  # the many-row forms (and 16 x 1 rows: split keys)
     (4, 70, 70, 64, 64, 64, "causal", None, 0.0),
     (2, 129, 257, 64, 16, 128, "random", None, 0.0),
     (16, 1, 3, 16, 8, 64, None, None, 0.0),
     (3, 200, 200, 48, 12, 64, "documents", 9, 25.0),
     (8, 128, 64, 32, 32, 128, "padded", 64, 0.0),
     (2, 385, 385, 40, 8, 64, "prefix", None, 0.0),
-    (8, 130, 130, 64, 64, 64, "random", 33, 0.0),         # 128-row workgroups at either head size from here on
+    (8, 130, 130, 64, 64, 64, "random", 33, 0.0),         # 128-row workgroups: this one and the next two, the last of them forward only
     (8, 140, 90, 64, 16, 64, "documents causal", None, 12.0),
     (4, 70, 200, 128, 32, 128, "random", None, 20.0),
     (4, 130, 130, 32, 8, 128, "random", 100, 300.0),
