@@ -388,13 +388,16 @@ int pf_qk_norm_rope_axes_bwd(const pf_heads_desc* d, float* dwq, float* dwk, voi
  *   entry <= -1e30 hides its distance.  Head h reads key head h / (H / Hkv).  A row that sees nothing gets zeros and LSE =
  *   -inf, whatever Q, K and V hold; a hidden key never reaches a row's result, be it infinite or NaN.  LSE fp32 [B][H][Lq]
  *   (natural logarithm of sum exp t) or NULL.  D = 64 or 128.  O may be Q.
+ *   Caps up to 64 leave up to 3 x 2^-23 of the cap in a score, and so in LSE (cap 64, one visible key: 3e-6 rms, 9e-6 seen; cap 30, 30
+ *   keys: 7e-7 rms); precise != 0 takes tanh to 32 bits there too (2e-7 .. 4e-7 rms; 8000 packed rows of 16 / 4 heads of 128: 158
+ *   instead of 128 us).  Larger caps and calls that ask for dbias always do.
  *   workspace: pf_attention_ranges_workspace_bytes(d) bytes, 16-byte aligned (0 for most calls: only problems with few rows
  *   split the keys); not shared by launches that may overlap.  Rows of a tensor lie less than 2^25 elements apart.
  * pf_attention_ranges_which: 1 = 128 or 64 rows of one head per workgroup, 2 = 32 (row, head) pairs of one key head per workgroup with the
  *   keys split over waves and workgroups, -1 = invalid descriptor.
  * pf_attention_ranges_rows: rows of one head per workgroup: 128 or 64 (+ 1 where the row tiles start in falling order of their keys), 32
  *   for the split-key form; of the gradient's dQ: 128 or 64.  -1 = invalid descriptor.
- * pf_attention_ranges_bwd: given dO, O, LSE of the forward, writes dQ, dK, dV and (dbias != NULL) the bias's gradient fp32
+ * pf_attention_ranges_bwd: given dO (the gradient of O; none of LSE's own is taken), O, LSE of the forward, writes dQ, dK, dV and (dbias != NULL) the bias's gradient fp32
  *   [H][2 R + 1]; the same bits every time.  Gradients of shared key heads are summed over their H / Hkv query heads.  Rows that
  *   see nothing get zeros, keys nobody sees too.  dQ, dK, dV must not overlap the inputs. */
 typedef struct {
@@ -405,6 +408,7 @@ typedef struct {
     const float* bias; float* dbias;
     int bias_radius, B, H, Hkv, Lq, Lk, D;
     float scale, cap;
+    int precise;
     void* workspace; long long workspace_bytes;
 } pf_attn_ranges_desc;
 long long pf_attention_ranges_workspace_bytes(const pf_attn_ranges_desc* d);     /* -1 = invalid descriptor */

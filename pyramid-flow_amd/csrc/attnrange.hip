@@ -291,9 +291,11 @@ PF_DEVICE float other_half(float x) {
 
 // ---------------------------------------------------------------------------------------------- scores
 // cap tanh(z / cap) = cap (1 + 2 u) with u = -1 / (1 + 2^(z zc)), zc = 2 scale log2 e / cap: the kernels keep u where an uncapped
-// score would be (its factor is 2 cap log2 e), and the slope 1 - tanh^2 = -4 (u + u^2).  That leaves 2^-23 of the CAP in the
-// score, nothing for caps up to 64 (8e-6); SERIES (larger caps) takes tanh itself, below |x| = 0.3 by its odd series (next term
-// 0.0089 x^10: 5e-8).  The series in every call cost 19 us of 165 at 16 heads of 128 channels and 8000 packed rows.
+// score would be (its factor is 2 cap log2 e), and the slope 1 - tanh^2 = -4 (u + u^2).  That leaves up to 3 x 2^-23 of the CAP in the
+// score: nothing that a weight in bf16 shows for caps up to 64, but a 32-bit log-sum-exp does (one visible key, cap 64: 3e-6 rms, where
+// tanh leaves 2e-7; 30 keys, cap 30: 7e-7 and 4e-7).  SERIES (larger caps, the bias's gradient, and whoever asks for it) takes tanh
+// itself, below |x| = 0.3 by its odd series (next term 0.0089 x^10: 5e-8): 158 instead of 128 us at 16 heads of 128 channels and 8000
+// packed rows, 295 instead of 286 for 16 tokens over 32768 keys, so not in every call.
 PF_DEVICE float cap_u(float x) { return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x)); }
 PF_DEVICE float tanh_f(float x) {
     const float y = x * x;
@@ -1685,8 +1687,9 @@ bool few_rows(const pf_attn_ranges_desc* d) {
 bool small_fwd(int D, long long Lq, long long H, long long B) { return (Lq + 127) / 128 * H * B < (D == 64 ? 1024 : 512); }
 bool small_dq(int D, long long Lq, long long H, long long B) { return (Lq + 127) / 128 * H * B < (D == 64 ? 1024 : 2048); }
 int row_groups(int Lq, bool small) { return small ? (Lq + 63) / 64 : (Lq + 127) / 128; }
-// SERIES also where the bias's gradient is wanted: it is a 32-bit result, and cap_u's 2^-23 of the cap would be all of its error
-bool series(const pf_attn_ranges_desc* d) { return d->cap > 64.f || (d->cap > 0.f && d->dbias); }
+// SERIES also where the bias's gradient is wanted: it is a 32-bit result, and what cap_u leaves of the cap would be all of its error; and
+// where the caller asks for it
+bool series(const pf_attn_ranges_desc* d) { return d->cap > 64.f || (d->cap > 0.f && (d->dbias || d->precise)); }
 int mode(const pf_attn_ranges_desc* d) { return (d->cap > 0.f ? 1 : 0) + (d->bias ? 2 : 0) + (series(d) ? 4 : 0); }
 int row_blocks(const pf_attn_ranges_desc* d) { return (int)(((long long)d->Lq * (d->H / d->Hkv) + 31) / 32); }
 int splits(const pf_attn_ranges_desc* d) {

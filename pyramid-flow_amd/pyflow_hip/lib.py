@@ -90,7 +90,7 @@ class AttnRangesDesc(C.Structure):
                 ("bias", C.c_void_p), ("dbias", C.c_void_p),
                 ("bias_radius", C.c_int), ("B", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("Lq", C.c_int),
                 ("Lk", C.c_int), ("D", C.c_int),
-                ("scale", C.c_float), ("cap", C.c_float),
+                ("scale", C.c_float), ("cap", C.c_float), ("precise", C.c_int),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong)]
 
 

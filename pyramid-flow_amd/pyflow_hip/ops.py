@@ -430,7 +430,7 @@ def qk_norm_rope_axes_backward(dq, dk, q, k, wq, wk, rope, pos, dq_in, dk_in, dw
     check(lib.pf_qk_norm_rope_axes_bwd(C.byref(d), pwq, pwk, ws.data_ptr() if ws is not None else 0, nbytes, raw_stream()))
 
 
-def _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap):
+def _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap, precise=False):
     r = ranges
     _one_device(what, q, k, v, out, lse, bias, q_pos, *((r.a_lo,) if r is not None else ()))
     if q.dim() != 4 or k.dim() != 4:
@@ -443,7 +443,7 @@ def _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap):
     _rows(d.Q, q, q.shape, what)
     _rows(d.K, k, kv, what)
     _rows(d.V, v, kv, what)
-    d.scale, d.cap = D ** -0.5 if scale is None else scale, cap
+    d.scale, d.cap, d.precise = D ** -0.5 if scale is None else scale, cap, bool(precise)
     if lse is not None:
         d.LSE = _f32(lse, (B, H, Lq), what)
     if r is not None:
@@ -467,15 +467,16 @@ def _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap):
     return d
 
 
-def attention_ranges(q, k, v, out, ranges=None, scale=None, bias=None, q_pos=None, cap=0.0, lse=None, workspace=None):
+def attention_ranges(q, k, v, out, ranges=None, scale=None, bias=None, q_pos=None, cap=0.0, lse=None, workspace=None, precise=False):
     """out = softmax(t) v over the keys each row sees (plan.KeyRanges; None = all), t = cap tanh(scale q.k / cap) (cap 0: scale q.k)
     + bias[h][clamp(j - pos, -R, R) + R].  q, out [B, Lq, H, D] and k, v [B, Lk, Hkv, D] bf16 views, D 64 or 128, H a multiple of
     Hkv; scale defaults to D^-1/2; bias fp32 [H, 2 R + 1], R <= 512 (entries <= -1e30 hide their distance); q_pos int32 [B or 1,
     Lq] positions of the rows among the keys (default i + Lk - Lq); lse fp32 [B, H, Lq] receives log sum exp t.  A row that sees
-    nothing gets zeros (lse -inf).  out may be q.  Few rows over many keys (single tokens over a cache) split the keys."""
+    nothing gets zeros (lse -inf).  out may be q, and shares memory with no other input.  Few rows over many keys (single tokens over
+    a cache) split the keys.  precise: tanh to 32 bits also for caps up to 64, which otherwise leave up to 3 x 2^-23 of the cap in lse."""
     what = "attention_ranges"
     lib = L.load()
-    d = _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap)
+    d = _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap, precise)
     _rows(d.O, out, q.shape, what, out=True)
     need = lib.pf_attention_ranges_workspace_bytes(C.byref(d))
     if need > 0:
@@ -487,8 +488,9 @@ def attention_ranges(q, k, v, out, ranges=None, scale=None, bias=None, q_pos=Non
 
 def attention_ranges_backward(dout, q, k, v, out, lse, dq, dk, dv, ranges=None, scale=None, bias=None, q_pos=None, cap=0.0,
                               dbias=None, workspace=None):
-    """Gradients of attention_ranges from its result `out` and `lse`: dq, dk, dv (bf16, shapes of q, k, v) and, where given,
-    dbias (fp32, shape of bias).  The same bits every time."""
+    """Gradients of attention_ranges from its result `out` and `lse`: dq, dk, dv (bf16, shapes of q, k, v; they share memory with
+    nothing else) and, where given, dbias (fp32, shape of bias), for a gradient that arrives at `out` alone: one that arrives at `lse`
+    is not supported.  The same bits every time."""
     what = "attention_ranges_backward"
     lib = L.load()
     d = _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap)

@@ -317,3 +317,37 @@ def test_forms_of_the_general_cases():
     assert {_rows(*c[:6], ranges=c[6] is not None) for c in CASES} == {32}
     assert [_rows(*c[:6], ranges=c[6] is not None) for c in MANY] == [64, 64, 32, 64, 64, 64, 128, 128, 128, 64, 64]
     assert [_rows(*c[:6], gradient=True) for c in MANY] == [64] * 6 + [128, 128, 64, 64, 64]
+
+
+@pytest.mark.parametrize("radius", [None, 3])
+@pytest.mark.parametrize("cap", [5.0, 30.0, 64.0])
+@pytest.mark.parametrize("form,B,Lq,Lk,H,Hkv,D", [
+    (32, 1, 60, 1, 8, 8, 64), (32, 1, 3, 3000, 8, 2, 128), (64, 1, 64, 1, 64, 64, 64), (64, 1, 64, 40, 64, 64, 128), (128, 8, 128, 1, 128, 128, 64)])
+def test_precise_log_sum_exp(form, B, Lq, Lk, H, Hkv, D, cap, radius):
+    """with `precise` the log-sum-exp of capped scores is right to 32 bits of the scores; one visible key leaves nothing to average"""
+    from pyflow_hip import ops
+    assert _rows(B, Lq, Lk, H, Hkv, D) == form
+    g = torch.Generator().manual_seed(61)
+    # products and sums of these are exact in 32 bits, and so is the scale
+    q = torch.randint(-3, 4, (B, Lq, H, D), generator=g).bfloat16()
+    k, v = ((torch.randint(-4, 5, (B, Lk, Hkv, D), generator=g) / 4).bfloat16() for _ in range(2))
+    bias = None if radius is None else torch.randn(H, 2 * radius + 1, generator=g)
+    out, lse = torch.empty_like(q).cuda(), torch.empty(B, H, Lq, device="cuda")
+    ops.attention_ranges(q.cuda(), k.cuda(), v.cuda(), out, scale=0.125, cap=cap, bias=None if bias is None else bias.cuda(), lse=lse, precise=True)
+    want, want_lse, bound = attention64(q, k, v, scale=0.125, cap=cap, bias=bias)
+    assert within(out, want, bound) <= 1
+    # Half steps, relative to the capped score: 2 for scale / cap and its product, 1 for the series' end (5e-8), 4 for its sums or
+    # (beyond |x| = 0.3) the exponential and quotient, 2 for cap log2 e, 1 for the sum with the bias, 2 for the way back; 4 of the bias.
+    # The log-sum-exp itself 3; sums over several keys 40 more (their logarithm, at most 24 additions in a row).
+    z = torch.matmul(q.double().transpose(1, 2), k.double().repeat_interleave(H // Hkv, 2).permute(0, 2, 3, 1)).mul(0.125)
+    t = (cap * torch.tanh(z / cap)).abs().amax(-1)
+    steps = 12 * t + 3 * want_lse.abs() + (0 if Lk == 1 else 40) + (0 if bias is None else 4 * bias.abs().max().item())
+    error = (lse.double().cpu() - want_lse).abs()
+    assert (error <= 2.0 ** -24 * steps).all(), (error / steps).max() * 2.0 ** 24
+    loose = torch.empty_like(lse)
+    ops.attention_ranges(q.cuda(), k.cuda(), v.cuda(), out, scale=0.125, cap=cap, bias=None if bias is None else bias.cuda(), lse=loose)
+    # cap (1 + 2 u), u = -1 / (1 + e), in half steps of the cap (2^-24): e to 2 half steps moves 2 u by at most half of that: 1; 1 + e
+    # rounded, and u to a step of its own ([1/2, 1]: 2^-24), each twice: 2 and 2 at the lower end, where e counts for nothing, 1 and 2 in
+    # the middle; the product with 2 cap log2 e rounded before the cap is added again, a value of up to the cap (in the middle) or twice
+    # that (lower end): 1 or 2.  Together 1 + 1 + 2 + 1 or 0 + 2 + 2 + 2
+    assert ((loose.double().cpu() - want_lse).abs() <= 2.0 ** -24 * (steps + 6 * cap)).all()
