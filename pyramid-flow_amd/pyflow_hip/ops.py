@@ -388,6 +388,8 @@ def _heads_desc(what, q, k, q_out, k_out, wq, wk, rope, pos, eps, q_scale):
     if pos.dtype != torch.float32 or pos.dim() != 3 or pos.shape[0] not in (1, B) or pos.shape[1] != L:
         raise ValueError(f"{what}: positions must be float32 [B or 1, L, axes]")
     n_axes = pos.shape[2]
+    if rope.n_axes is not None and n_axes < rope.n_axes:
+        raise ValueError(f"{what}: positions of {n_axes} axes for a rotation by {rope.n_axes}")
     if pos.numel():
         if n_axes > 1 and pos.stride(2) != 1:
             raise ValueError(f"{what}: the axes of a position must be dense")

@@ -109,14 +109,15 @@ class SequencePlan:
 class RopeAxes:
     """Rotation of head channels by several position axes, for ops.qk_norm_rope_axes: pair p turns by
     ``pos[axis[p]] * freq[p]`` radians.  ``freq`` float64 and ``axis`` int32, both [n_pairs] device tensors; pairs are channels
-    (2 p, 2 p + 1), or (p, p + n_pairs) with ``halves``; channels behind 2 n_pairs pass through."""
+    (2 p, 2 p + 1), or (p, p + n_pairs) with ``halves``; channels behind 2 n_pairs pass through.  ``n_axes``: how many axes a position
+    has to have at least (None: the axes are on the device and stay unread; one that a position lacks is then taken as its last)."""
 
-    def __init__(self, freq, axis, halves=False):
+    def __init__(self, freq, axis, halves=False, n_axes=None):
         if freq.dtype is not torch.float64 or axis.dtype is not torch.int32 or freq.dim() != 1 or freq.shape != axis.shape:
             raise ValueError("RopeAxes: freq must be float64 [n_pairs] and axis int32 [n_pairs]")
         if not (freq.is_contiguous() and axis.is_contiguous()) or freq.get_device() != axis.get_device():
             raise ValueError("RopeAxes: freq and axis must be contiguous and on one device")
-        self.freq, self.axis, self.halves, self.n_pairs = freq, axis, bool(halves), freq.numel()
+        self.freq, self.axis, self.halves, self.n_pairs, self.n_axes = freq, axis, bool(halves), freq.numel(), n_axes
 
     @classmethod
     def build(cls, axes_dim, device, theta=10000.0, halves=False):
@@ -125,7 +126,7 @@ class RopeAxes:
             raise ValueError("RopeAxes: channels per axis must be positive and even")
         freq = torch.cat([1.0 / (theta ** (torch.arange(0, d, 2, dtype=torch.float64) / d)) for d in axes_dim])
         axis = torch.cat([torch.full((d // 2,), n, dtype=torch.int32) for n, d in enumerate(axes_dim)])
-        return cls(freq.to(device), axis.to(device), halves)
+        return cls(freq.to(device), axis.to(device), halves, n_axes=len(axes_dim))
 
 
 class KeyRanges:

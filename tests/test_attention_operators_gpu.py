@@ -1,0 +1,32 @@
+"""Calls of the attention-block operators at the ends of what their documentation allows."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.join(os.path.dirname(__file__), "helpers"))
+from ranges_ref import U, heads64  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def test_positions_with_too_few_axes_are_refused():
+    """a rotation by (t, h, w) at positions of one axis has no answer; more axes than it uses are fine"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import RopeAxes
+    g = torch.Generator().manual_seed(71)
+    q, pos = torch.randn(1, 9, 2, 64, generator=g).bfloat16(), torch.rand(1, 9, 4, generator=g) * 30
+    rope, dev, out = RopeAxes.build([16, 24, 24], "cuda"), q.cuda(), torch.empty(1, 9, 2, 64, dtype=torch.bfloat16, device="cuda")
+    for n in (1, 2):
+        p = pos[..., :n].contiguous().cuda()
+        with pytest.raises(ValueError, match="axes"):
+            ops.qk_norm_rope_axes(dev, None, out, None, None, None, rope, p)
+        with pytest.raises(ValueError, match="axes"):
+            ops.qk_norm_rope_axes_backward(dev, None, dev, None, None, None, rope, p, out, None)
+    for n in (3, 4):
+        ops.qk_norm_rope_axes(dev, None, out, None, None, None, rope, pos[..., :n].contiguous().cuda())
+        want = heads64(q, None, pos, rope.freq.cpu(), rope.axis.cpu(), False)
+        # one rounding to bf16; 2^-20 of the pair for the 32-bit sine, cosine and sum
+        pair = (want[..., 0::2].square() + want[..., 1::2].square()).sqrt().repeat_interleave(2, -1)
+        assert ((out.double().cpu() - want).abs() <= U * want.abs() + 2.0 ** -20 * pair + 1e-30).all()
