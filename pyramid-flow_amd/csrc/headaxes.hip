@@ -30,6 +30,7 @@ struct HArgs {
     int B, L, H, Hk, P, halves;
     float eps, q_scale;
     int chunks, per_chunk;              // wave-iterations of one token, split over `chunks` waves
+    long long first_wave;               // forward: of this launch
     float* parts;                       // backward: [workgroup][2][D] partial gain gradients
 };
 
@@ -113,7 +114,7 @@ template <int D>
 __global__ __launch_bounds__(256) void heads_fwd_kernel(const HArgs p) {
     constexpr int LPU = D / 8, UPW = 64 / LPU;
     const int lane = threadIdx.x & 63, sub = lane % LPU;
-    const long long wave = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long wave = p.first_wave + (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long tokb = wave / p.chunks;
     if (tokb >= (long long)p.B * p.L) return;
     const int chunk = (int)(wave - tokb * p.chunks);
@@ -346,11 +347,14 @@ extern "C" int pf_qk_norm_rope_axes(const pf_heads_desc* d, hipStream_t stream) 
     if (const char* e = check_heads(d, false)) return pf_set_err(e);
     if (d->B == 0 || d->L == 0 || d->H + d->Hkv == 0) return 0;
     if (const char* e = check_overlap(d, false)) return pf_set_err(e);
-    const HArgs a = heads_args(d);
-    const unsigned grid = (unsigned)(((long long)d->B * d->L * a.chunks + 3) / 4);
-    if (d->D == 64) heads_fwd_kernel<64><<<grid, 256, 0, stream>>>(a);
-    else heads_fwd_kernel<128><<<grid, 256, 0, stream>>>(a);
-    CHECK_LAUNCH();
+    HArgs a = heads_args(d);
+    constexpr long long MOST = 1 << 23;                         // workgroups of a launch: 2^32 threads wrap around without an error
+    for (long long left = ((long long)d->B * d->L * a.chunks + 3) / 4; left > 0; left -= MOST, a.first_wave += 4 * MOST) {
+        const unsigned grid = (unsigned)(left < MOST ? left : MOST);
+        if (d->D == 64) heads_fwd_kernel<64><<<grid, 256, 0, stream>>>(a);
+        else heads_fwd_kernel<128><<<grid, 256, 0, stream>>>(a);
+        CHECK_LAUNCH();
+    }
     return 0;
 }
 

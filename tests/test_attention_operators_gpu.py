@@ -30,3 +30,21 @@ def test_positions_with_too_few_axes_are_refused():
         # one rounding to bf16; 2^-20 of the pair for the 32-bit sine, cosine and sum
         pair = (want[..., 0::2].square() + want[..., 1::2].square()).sqrt().repeat_interleave(2, -1)
         assert ((out.double().cpu() - want).abs() <= U * want.abs() + 2.0 ** -20 * pair + 1e-30).all()
+
+
+def test_more_tokens_than_one_launch_has_threads_for():
+    """2^26 + 5 tokens of one head: a wave each would be more than 2^32 threads; first, last and some of the rows between, in place"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import RopeAxes
+    L, D = (1 << 26) + 5, 64
+    g = torch.Generator(device="cuda").manual_seed(72)
+    q = torch.empty(1, L, 1, D, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    pos = torch.empty(1, L, 1, device="cuda").uniform_(0, 1e4, generator=g)
+    rows = torch.cat([torch.arange(9), torch.randint(0, L, (200,), generator=torch.Generator().manual_seed(73)), torch.arange(L - 9, L),
+                      torch.arange((1 << 26) - 1030, (1 << 26) + 5)]).cuda()
+    before, w = q[:, rows].cpu(), torch.full((D,), 1.25)
+    rope = RopeAxes.build([D], "cuda")
+    ops.qk_norm_rope_axes(q, None, q, None, w.cuda(), None, rope, pos)
+    want = heads64(before, w, pos[:, rows].cpu(), rope.freq.cpu(), rope.axis.cpu(), False)
+    # one rounding; cos / sin, the norm and the products in 32 bits: 2^-18 of the row's largest
+    assert ((q[:, rows].double().cpu() - want).abs() <= U * want.abs() + 2.0 ** -18 * want.abs().amax(-1, keepdim=True)).all()
