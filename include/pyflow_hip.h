@@ -393,6 +393,7 @@ int pf_qk_norm_rope_axes_bwd(const pf_heads_desc* d, float* dwq, float* dwk, voi
  *   instead of 128 us).  Larger caps and calls that ask for dbias always do.
  *   workspace: pf_attention_ranges_workspace_bytes(d) bytes, 16-byte aligned (0 for most calls: only problems with few rows
  *   split the keys); not shared by launches that may overlap.  Rows of a tensor lie less than 2^25 elements apart.
+ *   Calls that would take 2^24 workgroups or more are refused (about 2^30 rows of all heads).
  * pf_attention_ranges_which: 1 = 128 or 64 rows of one head per workgroup, 2 = 32 (row, head) pairs of one key head per workgroup with the
  *   keys split over waves and workgroups, -1 = invalid descriptor.
  * pf_attention_ranges_rows: rows of one head per workgroup: 128 or 64 (+ 1 where the row tiles start in falling order of their keys), 32

@@ -1674,6 +1674,8 @@ const char* check_overlap(const pf_attn_ranges_desc* d, bool grad) {
     return nullptr;
 }
 
+constexpr long long MOST_WGS = (1 << 24) - 1;          // of 256 threads: 2^32 threads of a launch wrap around without an error
+
 // the form with 32 (row, head) pairs per workgroup and the keys split: where even 64-row workgroups would be few (1 x 700 rows over 1400
 // keys of 32 heads of 128, 192 in the count below: 87 us, rows 43; 64 rows over 8000 keys of 16 heads of 64, 16: 25 us, rows 82), and
 // where one block of 32 pairs holds all rows that share a key head (each key is then read once, not once per query head)
@@ -1864,10 +1866,11 @@ extern "C" int pf_attention_ranges_bf16(const pf_attn_ranges_desc* d, hipStream_
         return pf_set_err("pf_attention_ranges_bf16: workspace missing, unaligned or too small");
     RArgs a = range_args(d);
     const bool few = few_rows(d);
-    const long long grid = few ? (long long)row_blocks(d) * d->Hkv * d->B * splits(d) : (long long)row_groups(d->Lq, true) * d->H * d->B;
-    if (grid > 0x7fffffffLL) return pf_set_err("pf_attention_ranges_bf16: too many workgroups");
+    const int nqt = row_groups(d->Lq, small_fwd(d->D, d->Lq, d->H, d->B));
+    const long long grid = few ? (long long)row_blocks(d) * d->Hkv * d->B * splits(d) : (long long)nqt * d->H * d->B;
+    if (grid > MOST_WGS) return pf_set_err("pf_attention_ranges_bf16: 2^24 workgroups or more");
     if (const char* e = check_overlap(d, false)) return pf_set_err(e);
-    a.nqt = row_groups(d->Lq, small_fwd(d->D, d->Lq, d->H, d->B));
+    a.nqt = nqt;
     a.nrb = row_blocks(d);
     a.nsplit = few ? splits(d) : 1;
     a.parts = (float*)d->workspace;
@@ -1894,10 +1897,12 @@ extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t
     if (need && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need))
         return pf_set_err("pf_attention_ranges_bwd: workspace missing, unaligned or too small");
     if (d->B > 65535 || d->H > 65535) return pf_set_err("pf_attention_ranges_bwd: more than 65535 batch entries or heads");
-    if ((long long)row_groups(d->Lq, true) * d->H * d->B + (long long)((d->Lk + 127) / 128) * d->H * d->B * 16 > 0x7fffff00LL ||
-        (long long)(d->Lq + 63) / 64 * (d->H / (d->Hkv ? d->Hkv : 1)) > 0x7fffffffLL)
-        return pf_set_err("pf_attention_ranges_bwd: too many workgroups");
     if (!d->H) return 0;
+    const int nqt = row_groups(d->Lq, small_dq(d->D, d->Lq, d->H, d->B));
+    const long long key_wgs = (long long)((d->Lk + 127) / 128) * kv_splits(d) * d->Hkv * d->B;
+    if ((long long)nqt * d->H * d->B + key_wgs + 7 > MOST_WGS || (d->Lq + 63) / 64 > MOST_WGS ||
+        (long long)(d->Lq + 63) / 64 * (d->H / d->Hkv) > 0x7fffffffLL)
+        return pf_set_err("pf_attention_ranges_bwd: 2^24 workgroups or more");
     if (const char* e = check_overlap(d, true)) return pf_set_err(e);
     RArgs a = range_args(d);
     char* w = (char*)d->workspace;
@@ -1907,9 +1912,9 @@ extern "C" int pf_attention_ranges_bwd(const pf_attn_ranges_desc* d, hipStream_t
     a.dbias_parts = (float*)(w += s.tiles);
     a.kv_parts = (float*)(w += s.parts);
     a.kv_split = kv_splits(d);
-    a.key_wgs = a.nkt * a.kv_split * a.Hk * a.B;
+    a.key_wgs = (int)key_wgs;
     a.key_pad = (a.key_wgs + 7) / 8 * 8;
-    a.nqt = row_groups(d->Lq, small_dq(d->D, d->Lq, d->H, d->B));
+    a.nqt = nqt;
     a.dbias = d->dbias;
     int rc = 0;
     if (d->B) switch ((d->D == 64 ? 0 : 8) + mode(d)) {
