@@ -404,7 +404,7 @@ def qk_norm_rope_axes(q, k, q_out, k_out, wq, wk, rope, pos, eps=1e-6, q_scale=1
     positions `pos` (fp32 [B or 1, L, axes]; fractions allowed), q times q_scale.  q [B, L, H, D], k [B, L, Hkv, D] bf16 views
     (column blocks of a projection are fine), D 64 or 128; either pair may be None; an output may be its input."""
     d = _heads_desc("qk_norm_rope_axes", q, k, q_out, k_out, wq, wk, rope, pos, eps, q_scale)
-    check(L.load().pf_qk_norm_rope_axes(C.byref(d), raw_stream()))
+    PROFILER.launch("qk_norm_rope_axes", 4.0 * d.B * d.L * (d.H + d.Hkv) * d.D, lambda: check(L.load().pf_qk_norm_rope_axes(C.byref(d), raw_stream())))
 
 
 def qk_norm_rope_axes_backward(dq, dk, q, k, wq, wk, rope, pos, dq_in, dk_in, dwq=None, dwk=None, eps=1e-6, q_scale=1.0,
@@ -429,7 +429,8 @@ def qk_norm_rope_axes_backward(dq, dk, q, k, wq, wk, rope, pos, dq_in, dk_in, dw
     if pwq or pwk:
         ws = _scratch(what, lib.pf_qk_norm_rope_axes_bwd_workspace_bytes(C.byref(d)), workspace, (q if q is not None else k).device)
         nbytes = ws.numel() * ws.element_size() if ws is not None else 0
-    check(lib.pf_qk_norm_rope_axes_bwd(C.byref(d), pwq, pwk, ws.data_ptr() if ws is not None else 0, nbytes, raw_stream()))
+    PROFILER.launch("qk_norm_rope_axes_bwd", 2.0 * d.B * d.L * d.D * (d.H * (3 if d.wq else 2) + d.Hkv * (3 if d.wk else 2)),
+                    lambda: check(lib.pf_qk_norm_rope_axes_bwd(C.byref(d), pwq, pwk, ws.data_ptr() if ws is not None else 0, nbytes, raw_stream())))
 
 
 def _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap, precise=False):
@@ -469,6 +470,13 @@ def _ranges_desc(what, q, k, v, out, lse, ranges, scale, bias, q_pos, cap, preci
     return d
 
 
+def _pair_flops(d, ranges, per_channel):
+    """floating-point operations of the visible pairs; counted (which waits for the device) only while profiling"""
+    if not PROFILER.enabled:
+        return 0.0
+    return float(per_channel) * d.D * d.H * (d.B * d.Lq * d.Lk if ranges is None else ranges.pairs(d.B, d.Lk))
+
+
 def attention_ranges(q, k, v, out, ranges=None, scale=None, bias=None, q_pos=None, cap=0.0, lse=None, workspace=None, precise=False):
     """out = softmax(t) v over the keys each row sees (plan.KeyRanges; None = all), t = cap tanh(scale q.k / cap) (cap 0: scale q.k)
     + bias[h][clamp(j - pos, -R, R) + R].  q, out [B, Lq, H, D] and k, v [B, Lk, Hkv, D] bf16 views, D 64 or 128, H a multiple of
@@ -485,7 +493,7 @@ def attention_ranges(q, k, v, out, ranges=None, scale=None, bias=None, q_pos=Non
         _one_device(what, workspace)
         ws = _scratch(what, need, workspace, q.device)
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    PROFILER.launch("attention_ranges", 0.0, lambda: check(lib.pf_attention_ranges_bf16(C.byref(d), raw_stream())))
+    PROFILER.launch("attention_ranges", _pair_flops(d, ranges, 4), lambda: check(lib.pf_attention_ranges_bf16(C.byref(d), raw_stream())))
 
 
 def attention_ranges_backward(dout, q, k, v, out, lse, dq, dk, dv, ranges=None, scale=None, bias=None, q_pos=None, cap=0.0,
@@ -512,4 +520,4 @@ def attention_ranges_backward(dout, q, k, v, out, lse, dq, dk, dv, ranges=None, 
     ws = _scratch(what, need, workspace, q.device)
     if ws is not None:
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    PROFILER.launch("attention_ranges_bwd", 0.0, lambda: check(lib.pf_attention_ranges_bwd(C.byref(d), raw_stream())))
+    PROFILER.launch("attention_ranges_bwd", _pair_flops(d, ranges, 10), lambda: check(lib.pf_attention_ranges_bwd(C.byref(d), raw_stream())))

@@ -195,6 +195,16 @@ class KeyRanges:
         """the joint text-video mask of a SequencePlan"""
         return cls(plan.a_lo, plan.a_hi, torch.full_like(plan.b_hi, plan.Lt), plan.b_hi)
 
+    def pairs(self, B, Lk):
+        """visible (row, key) pairs of a head, all B batch entries together, over Lk keys (read back from the device)"""
+        lo, hi = (t.long().clamp(0, Lk) for t in (self.a_lo, self.a_hi))
+        n = (hi - lo).clamp(min=0)
+        if self.b_lo is not None:
+            lo2, hi2 = (t.long().clamp(0, Lk) for t in (self.b_lo, self.b_hi))
+            n2 = (hi2 - lo2).clamp(min=0)
+            n = n + n2 - (torch.minimum(hi, hi2) - torch.maximum(lo, lo2)).clamp(min=0) * (n > 0) * (n2 > 0)
+        return int(n.sum()) * (B if n.shape[0] == 1 else 1)
+
     def dense_mask(self, Lk):
         """[B or 1, Lq, Lk] bool -- test helper: the mask the ranges stand for"""
         j = torch.arange(Lk, device=self.a_lo.device)

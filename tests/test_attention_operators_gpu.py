@@ -48,3 +48,28 @@ def test_more_tokens_than_one_launch_has_threads_for():
     want = heads64(before, w, pos[:, rows].cpu(), rope.freq.cpu(), rope.axis.cpu(), False)
     # one rounding; cos / sin, the norm and the products in 32 bits: 2^-18 of the row's largest
     assert ((q[:, rows].double().cpu() - want).abs() <= U * want.abs() + 2.0 ** -18 * want.abs().amax(-1, keepdim=True)).all()
+
+
+def test_profiler_sees_the_operators():
+    """each call is one record under its operator's name: bytes of the norm and rotation, operations of the pairs that are seen"""
+    from pyflow_hip import ops
+    from pyflow_hip.plan import KeyRanges, RopeAxes
+    B, L, H, Hkv, D = 2, 70, 4, 2, 64
+    q, out, dq = (torch.zeros(B, L, H, D, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    k, v, dk, dv = (torch.zeros(B, L, Hkv, D, dtype=torch.bfloat16, device="cuda") for _ in range(4))
+    lse, w = torch.zeros(B, H, L, device="cuda"), torch.ones(D, device="cuda")
+    rope, pos, ranges = RopeAxes.build([D], "cuda"), torch.zeros(1, L, 1, device="cuda"), KeyRanges.causal(L, L, "cuda")
+    kept, ops.PROFILER.records, ops.PROFILER.enabled = ops.PROFILER.records, {}, True
+    try:
+        ops.qk_norm_rope_axes(q, k, q, k, w, w, rope, pos)
+        ops.attention_ranges(q, k, v, out, lse=lse)
+        ops.attention_ranges(q, k, v, out, ranges=ranges, lse=lse)
+        ops.attention_ranges_backward(out, q, k, v, out, lse, dq, dk, dv, ranges=ranges)
+        ops.qk_norm_rope_axes_backward(dq, dk, q, k, w, None, rope, pos, dq, dk)
+        torch.cuda.synchronize()
+        seen = {n: (s["launches"], s["work_total"]) for n, s in ops.PROFILER.summary().items()}
+    finally:
+        ops.PROFILER.records, ops.PROFILER.enabled = kept, False
+    causal = B * L * (L + 1) // 2
+    assert seen == {"qk_norm_rope_axes": (1, 4.0 * B * L * (H + Hkv) * D), "attention_ranges": (2, 4.0 * D * H * (B * L * L + causal)),
+                    "attention_ranges_bwd": (1, 10.0 * D * H * causal), "qk_norm_rope_axes_bwd": (1, 2.0 * B * L * D * (3 * H + 2 * Hkv))}
