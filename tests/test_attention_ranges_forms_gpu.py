@@ -351,3 +351,32 @@ def test_precise_log_sum_exp(form, B, Lq, Lk, H, Hkv, D, cap, radius):
     # the middle; the product with 2 cap log2 e rounded before the cap is added again, a value of up to the cap (in the middle) or twice
     # that (lower end): 1 or 2.  Together 1 + 1 + 2 + 1 or 0 + 2 + 2 + 2
     assert ((loose.double().cpu() - want_lse).abs() <= 2.0 ** -24 * (steps + 6 * cap)).all()
+
+
+@pytest.mark.parametrize("radius,cap", [(None, 0.0), (4, 0.0), (None, 5000.0)])
+@pytest.mark.parametrize("form,B,Lq,H,D", [(128, 8, 65, 128, 64), (128, 8, 65, 64, 128), (64, 1, 65, 64, 64), (64, 1, 65, 64, 128), (32, 1, 65, 4, 64)])
+def test_sums_near_the_end_of_the_range(form, B, Lq, H, D, radius, cap):
+    """sums that end just below 2^128 (their reciprocal is subnormal), one that reaches it, and one key after another that outgrows all
+    before it by 2^60"""
+    from pyflow_hip import ops
+    Lk = 400
+    g = torch.Generator().manual_seed(91)
+    for keys in ({0: -127.0, 64: 0.5, 130: -1.0}, {0: -127.0, 70: 0.5, 140: 0.5, 210: 0.5}, {0: -120.0, 80: -60.0, 160: 0.0, 240: 60.0, 399: 120.0},
+                 {0: 60.0, 200: -60.0, 399: -62.0}):
+        q, k = torch.zeros(B, Lq, H, D), torch.zeros(B, Lk, 1, D)
+        q[..., 0], k[..., 0] = 1.0, -250.0
+        for j, s in keys.items():
+            k[:, j, :, 0] = s
+        v = torch.rand(B, Lk, 1, D, generator=g) * 2 - 1
+        q, k, v = (t.bfloat16() for t in (q, k, v))
+        bias = None if radius is None else torch.zeros(H, 2 * radius + 1)
+        out, lse = torch.full(q.shape, float("nan"), dtype=torch.bfloat16, device="cuda"), torch.full((B, H, Lq), float("nan"), device="cuda")
+        # one set of keys for all heads, read by each through its own (expanded) key head: what decides the form is H / Hkv = 1
+        kk, vv = (t.cuda().expand(B, Lk, H, D) for t in (k, v))
+        ops.attention_ranges(q.cuda(), kk, vv, out, scale=math.log(2.0), cap=cap, lse=lse, bias=None if bias is None else bias.cuda())
+        assert _rows(B, Lq, Lk, H, H, D, ranges=False) == form
+        want, want_lse, bound = attention64(q[:1], k[:1].expand(1, Lk, H, D), v[:1].expand(1, Lk, H, D), scale=math.log(2.0), cap=cap, bias=bias)
+        # as for the halves: scores of up to 250 ln 2 carry 2^-23 of themselves, three times
+        assert within(out[:1], want, bound + 2.0 ** -23 * 175 * 3) <= 1
+        assert within(lse[:1], want_lse, torch.full((), 2.0 ** -23 * 175 * 3).double()) <= 1
+        assert torch.isfinite(out).all()
