@@ -458,12 +458,16 @@ PF_DEVICE void exact_dkv(const RArgs& p, int b, int hk, int j) {
 // not see one of them, a bias hides some distance, or the last row, which a short tile repeats with weights of 0, is not finite.
 // Where none of this is so, a result that is not finite is right as it is: one infinite entry of dout costs nothing (16 heads of 64
 // over 4 key heads, 2048 rows, nothing hidden: 106 us with and 112 without it, 2320 when all keys were computed again).
-template <int D>
+template <int D, bool BIAS>
 PF_DEVICE bool strangers(const RArgs& p, int b, int hk, int w0) {
-    const int lane = threadIdx.x & 63, w1 = min(w0 + 32, p.Lk), rest = p.Lq & 63;
+    int lane = threadIdx.x & 63;
+    // nothing of this is worked out early and kept in registers through the caller's loop (4 x 3000 causal rows of 32 heads of 128 with a
+    // bias 1611 instead of 1677 us; without a bias there is no such gain)
+    if (BIAS) asm volatile("" : "+v"(lane));
+    const int w1 = min(w0 + 32, p.Lk), rest = p.Lq & 63;
     const int* const tiles = p.tiles + (long long)b * p.nq64 * 8;
     bool bad = false;
-    if (p.bias)
+    if (BIAS && p.bias)
         for (long long i = (long long)hk * p.G * (2 * p.R + 1) + lane; i < (long long)(hk + 1) * p.G * (2 * p.R + 1); i += 64) bad = bad || p.bias[i] <= HIDDEN;
     for (int n = lane; n < p.nq64 - (rest ? 1 : 0); n += 64) {
         const int* x = tiles + n * 8LL;
@@ -1101,7 +1105,7 @@ __global__ __launch_bounds__(256) void range_kvjoin_kernel(const RArgs p) {
         bad = bad || !(fabsf(k[c]) < __builtin_inff()) || !(fabsf(v[c]) < __builtin_inff());
         k[c] *= p.dscale;
     }
-    if (__builtin_amdgcn_ballot_w64(bad) != 0 && strangers<D>(p, b, hk, j & ~31)) {
+    if (__builtin_amdgcn_ballot_w64(bad) != 0 && strangers<D, true>(p, b, hk, j & ~31)) {
         exact_dkv<D>(p, b, hk, j);
         return;
     }
@@ -1593,7 +1597,7 @@ __global__ __launch_bounds__(256, D == 64 && !(MODE & 2) ? 3 : 2) void range_dkv
     }
     const bool bad = key < p.Lk && (any_nonfinite<D / 32>(dk) || any_nonfinite<D / 32>(dv));
     unsigned long long redo = __builtin_amdgcn_ballot_w64(bad);
-    if (redo != 0 && !strangers<D>(p, b, hk, w0)) redo = 0;
+    if (redo != 0 && !strangers<D, BIAS>(p, b, hk, w0)) redo = 0;
     redo = (redo | (redo >> 32)) & 0xffffffffull;
     if (key < p.Lk && !((redo >> (lane & 31)) & 1)) {
         store_cols<D>(p.dk.p + b * p.dk.bs + key * p.dk.ld + hk * p.dk.hs, dk, p.dscale);
