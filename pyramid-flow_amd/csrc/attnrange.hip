@@ -568,8 +568,8 @@ PF_DEVICE void add_bias(const RArgs& p, f32x16_t& s, float zs, const float* tab,
 // Which (head, tile) a workgroup takes.  Every XCD has a contiguous run of heads (their K and V stay in its L2), walks the first
 // half of each head's tiles -- the ones that causal and frame-wise masks make long -- for all of its heads and then the second
 // halves: the launch ends on short workgroups.  Tile numbers here count from the heavy end.  (Against head after
-// head, at the time: 1308 instead of 1415 us for 30 heads of the 15488-row video sequence, today 1240; gradients at 7808 rows 1333
-// instead of 1500, today 1280.)
+// head, at the time: 1308 instead of 1415 us for 30 heads of the 15488-row video sequence, today 1222 .. 1330 by the card; gradients at
+// 7808 rows 1333 instead of 1500, today 1260 .. 1325.)
 //
 // `resident` > 0: the first workgroups of an XCD go to its 32 compute units in turn, so those that start together on one unit are 32
 // apart; every other 32 come in reverse, which pairs long ones with short ones.
